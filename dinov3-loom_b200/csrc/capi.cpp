@@ -1,5 +1,6 @@
 // capi.cpp - the exported C ABI (include/dinov3.h, include/dinov3_kernels.h). Every entry point
 // converts C++ exceptions into a status code and a thread-local message.
+#include <algorithm>
 #include <cstring>
 #include <new>
 #include <string>
@@ -493,5 +494,250 @@ int dv3k_matmul_swiglu_folded(const uint16_t *x, uint32_t rows, const uint16_t *
 }
 
 uint32_t dv3k_gateup_source_row(uint32_t packed_row) { return dv3::gateup_source_row(packed_row); }
+
+// ------------------------------------------------------------------------------------------
+// Packed sequences and the paged cache
+// ------------------------------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+// A stride of an extent of one row or head is never used: 8 stands for whatever it is.
+int64_t used_stride(int64_t stride, uint32_t extent) { return extent > 1 ? stride : 8; }
+
+bool strides_ok(int64_t row, uint32_t rows, int64_t head, uint32_t heads) {
+  constexpr int64_t kMost = int64_t{1} << 38;  // a tensor map's strides stay below 2^40 bytes
+  row = used_stride(row, rows);
+  head = used_stride(head, heads);
+  return row > 0 && head > 0 && row % 8 == 0 && head % 8 == 0 && row < kMost && head < kMost;
+}
+
+// No two (row, head) vectors of `dim` elements share memory.
+bool rows_apart(int64_t row, uint32_t rows, int64_t head, uint32_t heads, uint32_t dim) {
+  if (rows > 1 && row < dim) return false;
+  if (heads > 1 && head < dim) return false;
+  if (rows <= 1 || heads <= 1) return true;
+  using wide = __int128;
+  return static_cast<wide>(head) * (heads - 1) + dim <= row ||
+         static_cast<wide>(row) * (rows - 1) + dim <= head;
+}
+
+const char *check_heads(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t dtype) {
+  if (dtype > DV3K_BF16) return "dtype must be DV3K_F16 or DV3K_BF16";
+  if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
+  if (kv_heads == 0 || kv_heads > 65535) return "kv_heads must be 1..65535";
+  if (q_heads % kv_heads != 0 || q_heads / kv_heads > 128)
+    return "q_heads must be a multiple of kv_heads, at most 128 times it";
+  return nullptr;
+}
+
+const char *check_cache(const void *k, const void *v, int64_t k_page, int64_t v_page,
+                        const int32_t *table, int64_t table_stride, uint32_t n_seq,
+                        uint32_t max_pages, uint32_t n_pages, uint32_t page_size, uint32_t kv_heads,
+                        uint32_t head_dim) {
+  if (page_size == 0 || page_size > 65536) return "page_size must be 1..65536";
+  if (n_pages > 0x7fffffffu) return "n_pages must be below 2^31";
+  if (static_cast<uint64_t>(max_pages) * page_size > 0x7fffffffull)
+    return "max_pages x page_size must be below 2^31";
+  if (n_pages > 0 && (!k || !v)) return "null cache";
+  if (!all_aligned(k, v)) return "pointers must be 16-byte aligned";
+  const int64_t least = static_cast<int64_t>(kv_heads) * page_size * head_dim;
+  if (n_pages > 1 && (k_page < least || v_page < least || k_page % 8 != 0 || v_page % 8 != 0))
+    return "pages must not overlap, a multiple of 8 elements apart";
+  if (n_seq > 0 && max_pages > 0 && !table) return "null page_table";
+  if ((reinterpret_cast<uintptr_t>(table) & 3u) != 0) return "page_table must be 4-byte aligned";
+  if (n_seq > 1 && table_stride < static_cast<int64_t>(max_pages))
+    return "table_stride must be at least max_pages";
+  return nullptr;
+}
+
+bool scale_ok(float s) { return s > 0.f && s <= 3.0e38f; }
+
+dv3::PagedAttention paged_args(const dv3k_paged_attention &a) {
+  dv3::PagedAttention p = {};
+  p.q = static_cast<const uint16_t *>(a.q);
+  p.k_cache = static_cast<const uint16_t *>(a.k_cache);
+  p.v_cache = static_cast<const uint16_t *>(a.v_cache);
+  p.out = static_cast<uint16_t *>(a.out);
+  p.lse = a.lse;
+  p.lens = a.lens;
+  p.page_table = a.page_table;
+  p.workspace = a.workspace;
+  p.q_seq = used_stride(a.q_seq, a.n_seq);
+  p.q_head = used_stride(a.q_head, a.q_heads);
+  p.out_seq = used_stride(a.out_seq, a.n_seq);
+  p.out_head = used_stride(a.out_head, a.q_heads);
+  p.k_page = used_stride(a.k_page, a.n_pages);
+  p.v_page = used_stride(a.v_page, a.n_pages);
+  p.table_stride = used_stride(a.table_stride, a.n_seq);
+  p.status = a.status;
+  p.page = dv3::page_div(a.page_size);
+  p.n_seq = a.n_seq;
+  p.max_len = static_cast<uint32_t>(
+      std::min<uint64_t>(a.max_len, static_cast<uint64_t>(a.max_pages) * a.page_size));
+  p.max_pages = a.max_pages;
+  p.n_pages = a.n_pages;
+  p.q_heads = a.q_heads;
+  p.kv_heads = a.kv_heads;
+  p.head_dim = a.head_dim;
+  p.scale = a.scale;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
+  if (!a) return bad_args("null arguments");
+  if (const char *e = check_heads(a->q_heads, a->kv_heads, a->head_dim, a->dtype)) return bad_args(e);
+  if (a->q_heads == 0) return bad_args("q_heads must be positive");
+  if (a->causal > 1 || a->reserved != 0) return bad_args("causal must be 0 or 1, reserved 0");
+  if (!scale_ok(a->scale)) return bad_args("scale must be positive and finite");
+  if (a->total_q > 0x7fffff00u || a->total_k > 0x7fffff00u || a->n_seq > 0x7fffff00u)
+    return bad_args("too many rows or sequences");
+  if (!strides_ok(a->q_token, a->total_q, a->q_head, a->q_heads) ||
+      !strides_ok(a->k_token, a->total_k, a->k_head, a->kv_heads) ||
+      !strides_ok(a->v_token, a->total_k, a->v_head, a->kv_heads) ||
+      !strides_ok(a->out_token, a->total_q, a->out_head, a->q_heads))
+    return bad_args("strides must be positive multiples of 8 elements");
+  if (!rows_apart(a->out_token, a->total_q, a->out_head, a->q_heads, a->head_dim))
+    return bad_args("rows and heads of out overlap");
+  if (a->total_q == 0 || a->n_seq == 0) return DV3_OK;
+  if (!a->q || !a->out || !a->cu_q || !a->cu_k || (a->total_k > 0 && (!a->k || !a->v)))
+    return bad_args("null tensor");
+  if (!all_aligned(a->q, a->k, a->v, a->out)) return bad_args("pointers must be 16-byte aligned");
+  dv3::PackedAttention p = {};
+  p.q = static_cast<const uint16_t *>(a->q);
+  p.k = static_cast<const uint16_t *>(a->k);
+  p.v = static_cast<const uint16_t *>(a->v);
+  p.out = static_cast<uint16_t *>(a->out);
+  p.lse = a->lse;
+  p.cu_q = a->cu_q;
+  p.cu_k = a->cu_k;
+  p.q_token = used_stride(a->q_token, a->total_q);
+  p.q_head = used_stride(a->q_head, a->q_heads);
+  p.k_token = used_stride(a->k_token, a->total_k);
+  p.k_head = used_stride(a->k_head, a->kv_heads);
+  p.v_token = used_stride(a->v_token, a->total_k);
+  p.v_head = used_stride(a->v_head, a->kv_heads);
+  p.out_token = used_stride(a->out_token, a->total_q);
+  p.out_head = used_stride(a->out_head, a->q_heads);
+  p.status = a->status;
+  p.n_seq = a->n_seq;
+  p.total_q = a->total_q;
+  p.total_k = a->total_k;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  p.causal = a->causal != 0;
+  p.scale = a->scale;
+  return launch_status(
+      dv3::launch_attention_packed(p, a->dtype == DV3K_BF16, static_cast<cudaStream_t>(stream)),
+      "attention_packed");
+}
+
+int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {
+  if (!a) return bad_args("null arguments");
+  if (const char *e = check_heads(a->q_heads, a->kv_heads, a->head_dim, a->dtype)) return bad_args(e);
+  if (a->reserved != 0) return bad_args("reserved must be 0");
+  if ((a->q == nullptr) != (a->q_heads == 0) && a->total > 0)
+    return bad_args("q and q_heads go together");
+  if (a->rot_dim % 16 != 0 || a->rot_dim > a->head_dim)
+    return bad_args("rot_dim must be a multiple of 16 up to head_dim");
+  if (a->total > 0x7fffff00u || a->n_seq > 0x7fffff00u) return bad_args("too many rows or sequences");
+  if (!a->cu_new && a->total != a->n_seq)
+    return bad_args("without cu_new every sequence has one row: total must equal n_seq");
+  if ((a->q_heads > 0 && (!strides_ok(a->q_token, a->total, a->q_head, a->q_heads) ||
+                          !strides_ok(a->q_out_token, a->total, a->q_out_head, a->q_heads))) ||
+      !strides_ok(a->k_token, a->total, a->k_head, a->kv_heads) ||
+      !strides_ok(a->v_token, a->total, a->v_head, a->kv_heads))
+    return bad_args("strides must be positive multiples of 8 elements");
+  if (a->q_heads > 0 &&
+      !rows_apart(a->q_out_token, a->total, a->q_out_head, a->q_heads, a->head_dim))
+    return bad_args("rows and heads of q_out overlap");
+  if (const char *e = check_cache(a->k_cache, a->v_cache, a->k_page, a->v_page, a->page_table,
+                                  a->table_stride, a->n_seq, a->max_pages, a->n_pages,
+                                  a->page_size, a->kv_heads, a->head_dim))
+    return bad_args(e);
+  if (a->total == 0 || a->n_seq == 0) return DV3_OK;
+  if (!a->k || !a->v || !a->lens || (a->q_heads > 0 && !a->q_out) ||
+      (a->rot_dim > 0 && (!a->cos || !a->sin)))
+    return bad_args("null tensor");
+  if (!all_aligned(a->q, a->k, a->v, a->q_out, a->cos, a->sin))
+    return bad_args("pointers must be 16-byte aligned");
+  dv3::RopeAppend p = {};
+  p.q = static_cast<const uint16_t *>(a->q);
+  p.k = static_cast<const uint16_t *>(a->k);
+  p.v = static_cast<const uint16_t *>(a->v);
+  p.q_out = static_cast<uint16_t *>(a->q_out);
+  p.k_cache = static_cast<uint16_t *>(a->k_cache);
+  p.v_cache = static_cast<uint16_t *>(a->v_cache);
+  p.cu_new = a->cu_new;
+  p.lens = a->lens;
+  p.page_table = a->page_table;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.q_token = used_stride(a->q_token, a->total);
+  p.q_head = used_stride(a->q_head, a->q_heads);
+  p.k_token = used_stride(a->k_token, a->total);
+  p.k_head = used_stride(a->k_head, a->kv_heads);
+  p.v_token = used_stride(a->v_token, a->total);
+  p.v_head = used_stride(a->v_head, a->kv_heads);
+  p.qo_token = used_stride(a->q_out_token, a->total);
+  p.qo_head = used_stride(a->q_out_head, a->q_heads);
+  p.k_page = used_stride(a->k_page, a->n_pages);
+  p.v_page = used_stride(a->v_page, a->n_pages);
+  p.table_stride = used_stride(a->table_stride, a->n_seq);
+  p.status = a->status;
+  p.page = dv3::page_div(a->page_size);
+  p.n_seq = a->n_seq;
+  p.total = a->total;
+  p.max_pages = a->max_pages;
+  p.n_pages = a->n_pages;
+  p.positions = a->positions;
+  p.rot_dim = a->rot_dim;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  return launch_status(
+      dv3::launch_rope_append(p, a->dtype == DV3K_BF16, static_cast<cudaStream_t>(stream)),
+      "rope_append");
+}
+
+size_t dv3k_attention_paged_workspace(const dv3k_paged_attention *a) {
+  if (!a || check_heads(a->q_heads, a->kv_heads, a->head_dim, DV3K_F16) || a->q_heads == 0 ||
+      a->n_seq == 0 || a->n_seq > 0x7fffff00u)
+    return 0;
+  return dv3::attention_paged_workspace(paged_args(*a));
+}
+
+int dv3k_attention_paged(const dv3k_paged_attention *a, void *stream) {
+  if (!a) return bad_args("null arguments");
+  if (const char *e = check_heads(a->q_heads, a->kv_heads, a->head_dim, a->dtype)) return bad_args(e);
+  if (a->q_heads == 0) return bad_args("q_heads must be positive");
+  if (!scale_ok(a->scale)) return bad_args("scale must be positive and finite");
+  if (a->n_seq > 0x7fffff00u) return bad_args("too many sequences");
+  if (!strides_ok(a->q_seq, a->n_seq, a->q_head, a->q_heads) ||
+      !strides_ok(a->out_seq, a->n_seq, a->out_head, a->q_heads))
+    return bad_args("strides must be positive multiples of 8 elements");
+  if (!rows_apart(a->out_seq, a->n_seq, a->out_head, a->q_heads, a->head_dim))
+    return bad_args("rows and heads of out overlap");
+  if (const char *e = check_cache(a->k_cache, a->v_cache, a->k_page, a->v_page, a->page_table,
+                                  a->table_stride, a->n_seq, a->max_pages, a->n_pages,
+                                  a->page_size, a->kv_heads, a->head_dim))
+    return bad_args(e);
+  if (a->n_seq == 0) return DV3_OK;
+  if (!a->q || !a->out || !a->lens) return bad_args("null tensor");
+  if (!all_aligned(a->q, a->out, a->workspace)) return bad_args("pointers must be 16-byte aligned");
+  const dv3::PagedAttention p = paged_args(*a);
+  if (const size_t need = dv3::attention_paged_workspace(p);
+      need > 0 && (!a->workspace || a->workspace_bytes < need))
+    return bad_args("workspace must hold dv3k_attention_paged_workspace bytes");
+  return launch_status(
+      dv3::launch_attention_paged(p, a->dtype == DV3K_BF16, static_cast<cudaStream_t>(stream)),
+      "attention_paged");
+}
 
 }  // extern "C"

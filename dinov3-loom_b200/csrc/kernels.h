@@ -183,6 +183,60 @@ cudaError_t launch_attention(const AttentionMaps &maps, uint32_t rows, uint32_t 
                              size_t l2_next_bytes = 0, const void *discard = nullptr,
                              size_t discard_bytes = 0);
 
+// ---- packed sequences and the paged cache (attention_packed.cu, rope_append.cu,
+// attention_paged.cu). Strides are in elements; the arguments have been checked. ----
+struct PackedAttention {
+  const uint16_t *q, *k, *v;
+  uint16_t *out;
+  float *lse;  // [total_q][q_heads] or null
+  const int32_t *cu_q, *cu_k;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  uint32_t *status;
+  uint32_t n_seq, total_q, total_k, q_heads, kv_heads, head_dim;
+  bool causal;
+  float scale;
+};
+cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream);
+
+// A page size and its shift (32 where it is no power of two).
+struct PageDiv {
+  uint32_t size, shift;
+};
+inline PageDiv page_div(uint32_t size) {
+  PageDiv d{size, 32};
+  for (uint32_t s = 0; s < 32; ++s)
+    if (size == 1u << s) d.shift = s;
+  return d;
+}
+
+struct RopeAppend {
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out, *k_cache, *v_cache;
+  const int32_t *cu_new, *lens, *page_table;  // cu_new null: one row per sequence
+  const float *cos, *sin;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head, k_page, v_page,
+      table_stride;
+  uint32_t *status;
+  PageDiv page;
+  uint32_t n_seq, total, max_pages, n_pages, positions, rot_dim, q_heads, kv_heads, head_dim;
+};
+cudaError_t launch_rope_append(const RopeAppend &p, bool bf16, cudaStream_t stream);
+
+struct PagedAttention {
+  const uint16_t *q, *k_cache, *v_cache;
+  uint16_t *out;
+  float *lse;  // [n_seq][q_heads] or null
+  const int32_t *lens, *page_table;
+  void *workspace;
+  int64_t q_seq, q_head, out_seq, out_head, k_page, v_page, table_stride;
+  uint32_t *status;
+  PageDiv page;
+  uint32_t n_seq, max_len, max_pages, n_pages, q_heads, kv_heads, head_dim;
+  float scale;
+};
+size_t attention_paged_workspace(const PagedAttention &p);  // bytes, on the current device
+cudaError_t launch_attention_paged(const PagedAttention &p, bool bf16, cudaStream_t stream);
+
 // ---- bandwidth kernels (elementwise.cu) ----
 // l2_next/l2_next_bytes: weights of a later kernel to prefetch into L2 (see GemmArgs).
 cudaError_t launch_patchify(const float *images, uint32_t n_images, const float *prefix,

@@ -22,6 +22,8 @@ constexpr uint32_t kErrEpilogueWait = 1u << 2;
 constexpr uint32_t kErrAttentionWait = 1u << 3;
 constexpr uint32_t kErrSelfTestWait = 1u << 4;   // the bounded-wait self-test's expired wait
 constexpr uint32_t kErrSelfTestAbort = 1u << 5;  // the self-test's second role unwound on abort
+constexpr uint32_t kErrPage = 1u << 6;      // a page outside the pool or behind the page table's end
+constexpr uint32_t kErrPosition = 1u << 7;  // a position before 0 or behind the rotation tables
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -12,6 +12,10 @@ Python face of the C ABI in include/dinov3.h, mirroring the reference crate's AP
 `pixels` are normalised NCHW float32 images, n x 3 x 224 x 224 (any shape with that many
 floats). Errors raise DINOv3Error carrying the library's status code and message (the
 reference's error texts). All compute runs in the CUDA library; there is no CPU path.
+
+For sequences beside the model's own forward (images of other sizes packed into one batch, a
+decoder behind the tokens), on CUDA tensors: attention_packed, rope_append, attention_paged
+(sequence.py).
 """
 from __future__ import annotations
 
@@ -31,6 +35,7 @@ OK, INVALID_ARGUMENT, WEIGHTS, DEVICE, POISONED = range(5)
 __all__ = [
     "DINOv3", "DINOv3Error", "Options", "ForwardTimings", "Distribution", "LibraryMissing",
     "IMAGE_ELEMENTS", "TOKENS", "HIDDEN", "pack_f16", "hub_weights",
+    "attention_packed", "rope_append", "attention_paged",
 ]
 
 
@@ -262,3 +267,14 @@ def hub_weights(offline: bool = False) -> str:
     buf = ctypes.create_string_buffer(4096)
     _check(_lib.load().dv3_hub_weights(1 if offline else 0, buf, len(buf)))
     return buf.value.decode()
+
+
+
+def __getattr__(name):
+    # the sequence operators take torch tensors: torch is imported when the first one is named
+    if name in ("attention_packed", "rope_append", "attention_paged"):
+        from . import sequence
+
+        globals()[name] = getattr(sequence, name)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -194,6 +194,99 @@ int dv3k_down_splitk_noalloc(const uint16_t *a, uint32_t rows, const uint16_t *w
 int dv3k_matmul_swiglu(const uint16_t *h, uint32_t rows, const uint16_t *gateup_w,
                        const float *gateup_b, uint16_t *act, uint32_t *status, void *stream);
 
+/* ---- Packed sequences and a paged key-value cache (no counterpart in the reference, whose
+ * attention is dv3k_attention's: 201 tokens, 6 heads x 64, f16, no mask). For images of other
+ * sizes packed into one batch, and for a decoder that reads the tokens.
+ *
+ * Beyond the common rules:
+ *   - `dtype` is DV3K_F16 or DV3K_BF16 and holds for every 16-bit tensor of the call; head_dim is
+ *     64 or 128; q_heads is a multiple of kv_heads, at most 128 times it, and query head h reads
+ *     key-value head h / (q_heads / kv_heads). Scores, the softmax's maximum and sum and every
+ *     product's sum are f32; the weights are rounded to `dtype` before the product with v.
+ *   - A row tensor [rows][heads][head_dim] is given by its row (token) and head strides in
+ *     elements, multiples of 8, with head_dim contiguous. Rows or heads of an output do not
+ *     overlap, nor does an output overlap an input (but q_out of dv3k_rope_append may be q).
+ *   - `cu` arrays [n_seq + 1] (i32, device) hold the first row of each sequence and the end of the
+ *     last, ascending. Sequences may be empty. Rows before cu[0] or from cu[n_seq] on are left as
+ *     they were. Values outside the tensor are clamped to it.
+ *   - A cache is [n_pages][kv_heads][page_size][head_dim], pages k_page / v_page elements apart
+ *     (multiples of 8). page_table [n_seq][max_pages] (i32, device, rows table_stride apart)
+ *     names each sequence's pages in order; entries behind the last page in use are not read. A
+ *     page may stand in several rows (a shared prefix) while nobody appends to it.
+ *   - status word 0 collects bit 6 (a page id outside 0..n_pages-1, or a position behind the
+ *     table's max_pages) and bit 7 (a position before 0 or behind the rotation tables). Such tokens
+ *     are skipped: not appended, not attended to.
+ *   - `lens`, `cu` and the page table are read on the device: a captured call replays on their
+ *     new values.
+ *   - Infinities and NaN in rows and slots that a query does not see do not reach its result. */
+enum { DV3K_F16 = 0, DV3K_BF16 = 1 };
+
+/* Attention of each sequence's queries to its keys:
+ *   out[i][h] = sum_j w_ij v[j][g] / sum_j w_ij,  w_ij = exp(scale (q[i][h] . k[j][g] - max_j)),
+ * over the sequence's keys j < b, where causal over j <= i + b - a of them (a queries, b keys: the
+ * last query sees the last key). A row that sees no key gets 0, and -inf in lse. lse (f32
+ * [total_q][q_heads], optional) gets log sum_j exp(scale q . k_j). scale > 0. */
+typedef struct {
+  const void *q, *k, *v;
+  void *out;
+  float *lse;
+  const int32_t *cu_q, *cu_k;
+  uint32_t *status;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  uint32_t n_seq, total_q, total_k, q_heads, kv_heads, head_dim, dtype, causal;
+  float scale;
+  uint32_t reserved; /* 0 */
+} dv3k_packed_attention;
+int dv3k_attention_packed(const dv3k_packed_attention *args, void *stream);
+
+/* Rotate new queries and keys by their positions and append the keys and values to the cache.
+ * Row t of sequence s (cu_new; NULL: row t is sequence t's only one and total == n_seq) stands at
+ * position p = lens[s] - (the sequence's new rows) + (its index among them): lens counts the
+ * appended rows already, so that the same array serves dv3k_attention_paged afterwards.
+ *   q_out[t][h][c] = q[c] cos[p][c] - q[c + rot/2] sin[p][c],
+ *   q_out[t][h][c + rot/2] = q[c + rot/2] cos[p][c] + q[c] sin[p][c]   for c < rot/2,
+ * and as it is for c >= rot; k the same into slot p % page_size of page page_table[s][p /
+ * page_size], v unchanged. cos, sin: f32 [positions][rot_dim / 2]; rot_dim is a multiple of 16 up
+ * to head_dim, or 0 (no rotation, tables NULL). q NULL (with q_heads 0): append only. Two rows of
+ * one call that name the same slot leave either's value there. */
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out, *k_cache, *v_cache;
+  const int32_t *cu_new, *lens, *page_table;
+  const float *cos, *sin;
+  uint32_t *status;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, q_out_token, q_out_head, k_page,
+      v_page, table_stride;
+  uint32_t n_seq, total, max_pages, n_pages, page_size, positions, rot_dim, q_heads, kv_heads,
+      head_dim, dtype;
+  uint32_t reserved; /* 0 */
+} dv3k_rope_append_args;
+int dv3k_rope_append(const dv3k_rope_append_args *args, void *stream);
+
+/* Attention of one query row per sequence to its lens[s] cached tokens (the form of
+ * dv3k_attention_packed for a = 1): q, out [n_seq][q_heads][head_dim], lse f32 [n_seq][q_heads]
+ * optional. lens[s] <= 0 gives 0 and -inf.
+ *   - max_len is the caller's bound of lens (max_pages page_size will do). It sets how far a
+ *     sequence is split over the SMs; longer sequences are computed all the same, only slower.
+ *   - workspace: dv3k_attention_paged_workspace(args) bytes on the current device (0: NULL will do),
+ *     16-byte aligned, scratch of this call. Calls that may overlap on the GPU (on two streams, or
+ *     in two graphs) need one each. It reads n_seq, max_len,
+ *     max_pages, page_size, q_heads, kv_heads and head_dim. */
+typedef struct {
+  const void *q, *k_cache, *v_cache;
+  void *out;
+  float *lse;
+  const int32_t *lens, *page_table;
+  void *workspace;
+  uint32_t *status;
+  int64_t q_seq, q_head, out_seq, out_head, k_page, v_page, table_stride;
+  uint64_t workspace_bytes;
+  uint32_t n_seq, max_len, max_pages, n_pages, page_size, q_heads, kv_heads, head_dim, dtype;
+  float scale;
+} dv3k_paged_attention;
+int dv3k_attention_paged(const dv3k_paged_attention *args, void *stream);
+size_t dv3k_attention_paged_workspace(const dv3k_paged_attention *args);
+
 /* Row of the reference's concatenated gate||up matrix ([3072][384], src/weights.rs:103-108)
  * that packed row `packed_row` (< 3072) of gateup_w holds. Host function. */
 uint32_t dv3k_gateup_source_row(uint32_t packed_row);
