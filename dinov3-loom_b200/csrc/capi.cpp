@@ -552,7 +552,7 @@ const char *check_cache(const void *k, const void *v, int64_t k_page, int64_t v_
   return nullptr;
 }
 
-bool scale_ok(float s) { return s > 0.f && s <= 3.0e38f; }
+bool scale_ok(float s) { return s > 0.f && s <= 1.0e30f; }
 
 dv3::PagedAttention paged_args(const dv3k_paged_attention &a) {
   dv3::PagedAttention p = {};
