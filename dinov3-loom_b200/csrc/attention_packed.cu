@@ -1,95 +1,785 @@
 // attention_packed.cu - attention over packed sequences of different lengths, grouped heads, full
-// or causal.
+// or causal, on tcgen05 tensor cores.
 //
 // For query row i of a sequence with a queries and b keys, and query head h reading key-value head
 // h / (q_heads / kv_heads): o = sum_j w_j v_j / sum_j w_j, w_j = exp(scale (q . k_j - max)), over
 // the keys j < b, and j <= i + b - a where causal (the last query sees the last key). A row that
 // sees no key gives 0 (and -inf as its log-sum).
 //
-// One warp per (row, query head): the running maximum and sum of the softmax, in f32, one pass
-// over the keys.
+// Tiles. A 128-row query tile holds 128 / group tokens with all `group` query heads that read one
+// key-value head (one TMA box of group heads x tokens), so grouped heads share every K and V tile
+// and a short sequence still fills its rows; a work item is two such tiles of one sequence and
+// key-value head against that sequence's visible keys, 128 at a time. Persistent CTAs, one per
+// SM, walk the items longest first (below).
+//
+// Roles (384 threads):
+//   warps 0-3  softmax and output of tile 0, warps 4-7 of tile 1: one query row per thread (its
+//              TMEM lane). All 128 scores of a step are held in registers: running maximum, w =
+//              2^(s c - m c) with c = scale log2(e), f32 sum of the unrounded weights, P (rounded to
+//              the element type) back to TMEM over the consumed scores. The reference m only moves
+//              when the maximum has grown by more than 2^8 over it: any m gives the same quotient,
+//              and sums and weights up to 2^8 too large lose nothing in f32, f16 or bf16; the row's
+//              output is then rescaled in TMEM. At an item's end O / sum is written, 32 bytes a
+//              store.
+//   warp 8     TMA producer: Q tiles, then K and V tiles in turn through one ring of stages.
+//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = N = 128), then O_t += P_t V with
+//              P from TMEM and V as the MN-major B operand. Each walks the ring by itself, so the
+//              softmax of one tile overlaps the products of the other.
+//   warp 11    scheduler, and guard of V: a key that a row does not see has weight 0, but 0 times
+//              an infinity or NaN is NaN. Only the tiles at an item's end (from the first that some
+//              row sees in part) can hold such keys; there it tests V in shared memory, sets what
+//              is not finite to 0 and leaves a note, and the rows that do see those keys add them
+//              at the end from global memory.
+// TMEM: S_0 | S_1 | O_0 | O_1, 128 columns each.
+//
+// Every wait is bounded; on a timeout the kernel records kErrAttentionWait, raises the CTA's
+// abort flag, lets its own copies and MMAs in flight land, frees TMEM and returns.
+#include <atomic>
+
 #include "sequence.cuh"
 
 namespace dv3 {
 
 namespace {
-constexpr int kWarps = 4;
+constexpr int kThreads = 384;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;  // TMEM allocator; issues tile 0's MMAs, warp 10 tile 1's
+constexpr int kGuardWarp = 11;
+constexpr int kKeys = 128;      // keys per step
+constexpr int kBuckets = 128;   // of the scheduler's order
+constexpr int kTmemCols = 512;
+constexpr int kTmemO = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.f;   // log2 units by which a row's maximum may pass its reference
+
+// One work item as the scheduler publishes it.
+struct Item {
+  int32_t q_row;    // first query row
+  int32_t q_count;  // its tokens (0: nothing to do)
+  int32_t k_row;    // first key row of the sequence
+  int32_t k_len;
+  int32_t visible;  // keys the first token sees, less than 1 if none; a later one sees one more if causal
+  int32_t head;     // key-value head
+  int32_t last;     // 1: no more items
+  int32_t fix;      // set by the guard: V held something that is not finite
+};
+
+template <int kDim>
+struct Layout {
+  static constexpr int kHalves = kDim / 64;         // 64-channel (128-byte) columns of a tile
+  static constexpr int kHalfBytes = 128 * 128;      // 128 rows of one
+  static constexpr int kTileBytes = kHalves * kHalfBytes;
+  static constexpr int kStages = kDim == 128 ? 5 : 8;
+  static constexpr int kRingOff = 2 * kTileBytes;   // Q_0 | Q_1 | stages
+  static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
+  // barriers: q_full[2] q_empty[2] s_full[2] p_full[2] o_full[2] drain[2] sched_full[2]
+  // sched_empty[2] kv_full[stages] kv_empty[stages] v_ok[stages] (by V tile, not by stage: a stage
+  // of an odd ring holds K and V in turn)
+  static constexpr int kBars = 16 + 3 * kStages;
+  static constexpr int kItemOff = kBarOff + kBars * 8;
+  static constexpr int kMiscOff = kItemOff + 2 * static_cast<int>(sizeof(Item));  // TMEM slot, abort
+  static constexpr int kOrderOff = kMiscOff + 16;
+  static constexpr int kBytes = 1024 + kOrderOff + 2 * kBuckets * 4;
+  static_assert(kBytes <= 227 * 1024, "shared memory budget");
+};
+
+// Instruction descriptor with the element type (see idesc_f16_f32): bf16 is format 1.
+__host__ __device__ constexpr uint32_t idesc_f32(bool bf16, uint32_t m, uint32_t n, bool b_mn_major) {
+  return idesc_f16_f32(m, n, b_mn_major) | (bf16 ? (1u << 7) | (1u << 10) : 0u);
+}
+// MN-major 128-byte-swizzle tile whose 64-element columns lie `column_bytes` apart (the leading
+// byte offset); 8-row groups of K are 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t smem_addr, uint32_t column_bytes) {
+  return (sw128_desc(smem_addr) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(column_bytes >> 4) << 16);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Items in an order that ends evenly: with two tiles of `tokens` query tokens an item, sequence s has
+// n_s = ceil(len / tokens) of them, and the later ones of a causal sequence see the most keys. They
+// are ordered by level (index within the sequence) downwards over all sequences, levels taken `width`
+// at a time as one of 128 buckets, and by sequence within a bucket.
+struct Order {
+  uint32_t *starts;  // first tile of each bucket, top bucket first; [kBuckets]
+  uint32_t total;    // tiles
+  uint32_t width;
+  // where the last search stood
+  int bucket;
+  uint32_t seq, before;
+};
+}  // namespace
+
+struct PackedArgs {
+  const uint16_t *v;
+  uint16_t *out;
+  float *lse;
+  const int32_t *cu_q, *cu_k;
+  int64_t v_token, v_head, out_token, out_head;
+  uint32_t *status;
+  uint32_t n_seq, total_q, total_k, q_heads, kv_heads, group;
+  uint32_t tokens;  // per tile
+  uint32_t width;   // levels per bucket
+  uint32_t wide;    // out rows are 32-byte aligned
+  bool causal;
+  float scale_log2;
+};
+
+namespace {
+__device__ __forceinline__ uint32_t tiles_of(const PackedArgs &p, uint32_t s) {
+  uint32_t a, b;
+  sequence_rows(p.cu_q, s, p.total_q, &a, &b);
+  return (b - a + 2 * p.tokens - 1) / (2 * p.tokens);
+}
+
+// The item of tile `tile` and key-value head `head`; whole warp.
+__device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_t tile, uint32_t head) {
+  const uint32_t lane = threadIdx.x & 31u;
+  Item it = {};
+  it.head = static_cast<int32_t>(head);
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < kBuckets / 32; ++i) mine += o.starts[lane * (kBuckets / 32) + i] <= tile;
+  const int at = static_cast<int>(__reduce_add_sync(0xffffffffu, mine)) - 1;
+  const uint32_t rest = tile - o.starts[at], base = (kBuckets - 1 - at) * o.width;
+  if (at != o.bucket || rest < o.before) {
+    o.bucket = at;
+    o.seq = 0;
+    o.before = 0;
+  }
+  for (; o.seq < p.n_seq; o.seq += 32) {
+    const uint32_t s = o.seq + lane;
+    const uint32_t n = s < p.n_seq ? tiles_of(p, s) : 0u;
+    const uint32_t c = n > base ? min(n - base, at == 0 ? n : o.width) : 0u;
+    uint32_t sum = c;
+#pragma unroll
+    for (int i = 1; i < 32; i *= 2) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, sum, i);
+      if (lane >= static_cast<uint32_t>(i)) sum += x;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, rest < o.before + sum);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const uint32_t first = o.before + __shfl_sync(0xffffffffu, sum - c, src);
+      const uint32_t level = base + __shfl_sync(0xffffffffu, c, src) - 1 - (rest - first);
+      uint32_t q0, q1, k0, k1;
+      const uint32_t seq = o.seq + src;
+      sequence_rows(p.cu_q, seq, p.total_q, &q0, &q1);
+      sequence_rows(p.cu_k, seq, p.total_k, &k0, &k1);
+      const uint32_t t0 = level * 2 * p.tokens;
+      it.q_row = static_cast<int32_t>(q0 + t0);
+      it.q_count = static_cast<int32_t>(min(q1 - q0 - t0, 2 * p.tokens));
+      it.k_row = static_cast<int32_t>(k0);
+      it.k_len = static_cast<int32_t>(k1 - k0);
+      it.visible = p.causal ? static_cast<int32_t>(k1 - k0) - static_cast<int32_t>(q1 - q0) +
+                                  static_cast<int32_t>(t0) + 1
+                            : it.k_len;
+      return it;
+    }
+    o.before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return it;  // not reached while cu is ascending
+}
+
+// What a tile's rows see: steps of 128 keys, and the keys of its first token.
+struct Reach {
+  int steps;  // of this tile
+  int first;  // keys that its first token sees (at least 0)
+};
+__device__ __forceinline__ Reach reach_of(const Item &it, int tile, int tokens, bool causal) {
+  const int begin = tile * tokens, end = min(it.q_count, begin + tokens);
+  Reach r = {0, 0};
+  if (begin >= end) return r;
+  const int most = causal ? min(it.k_len, it.visible + end - 1) : it.k_len;
+  r.first = max(0, causal ? min(it.k_len, it.visible + begin) : it.k_len);
+  r.steps = most > 0 ? (most + kKeys - 1) / kKeys : 0;
+  return r;
+}
+
+// Whether 16 bytes of 16-bit floats are all finite: x * 0 summed is NaN otherwise.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t times_zero(uint32_t x, uint32_t acc) {
+  if constexpr (kBf16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(x), "r"(0u));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(x), "r"(0u));
+  return acc;
+}
+template <bool kBf16>
+__device__ __forceinline__ bool finite16(uint32_t half) {
+  const uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
+  return (half & e) != e;
+}
+
+// Scores, weights and sums of one step for this thread's row. `vis`: keys of this step that the row
+// sees (used where kMasked). Returns through m (reference, log2 units), sum.
+template <bool kBf16, bool kMasked>
+__device__ __forceinline__ void softmax_step(uint32_t tl, uint32_t to, int dim, float c, int vis,
+                                             bool first, float &m, float &sum, uint64_t *o_full,
+                                             uint32_t o_parity, volatile int *abort_flag, bool &ok) {
+  uint32_t v[4][32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_ld32(tl + 32 * i, v[i]);
+  tmem_wait_ld(v[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) tmem_regs_ready(v[i]);
+  if constexpr (kMasked) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (32 * i + e >= vis) v[i][e] = 0xff800000u;  // -inf
+  }
+  float top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top[i] = __uint_as_float(v[i][0]);
+#pragma unroll
+    for (int e = 1; e + 1 < 32; e += 2)
+      top[i] = max3(top[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
+    top[i] = fmaxf(top[i], __uint_as_float(v[i][31]));
+  }
+  const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+  if (first) {
+    m = now;
+  } else {
+    const bool grown = now > m + kSlack;
+    if (__any_sync(0xffffffffu, grown)) {
+      // rescale this row's output (factor 1 for rows that stay); the previous product must be done
+      const float next = grown ? now : m;
+      const float f = grown ? ex2_approx(m - next) : 1.f;
+      sum *= f;
+      m = next;
+      if (!__all_sync(0xffffffffu, mbar_wait(o_full, o_parity, abort_flag))) {
+        ok = false;
+        return;
+      }
+      tc_fence_after();
+      for (int d = 0; d < dim; d += 16) {
+        uint32_t x[16];
+        tmem_ld16(to + d, x);
+        tmem_ld_wait();
+        tmem_regs_ready16(x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+        tmem_st16(to + d, x);
+      }
+    }
+  }
+  const float base = m == -INFINITY ? 0.f : m;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float a = ex2_approx(fmaf(__uint_as_float(v[i][2 * e]), c, -base));
+      const float b = ex2_approx(fmaf(__uint_as_float(v[i][2 * e + 1]), c, -base));
+      s0 += a;
+      s1 += b;
+      w[e] = Elem<kBf16>::pack(a, b);
+    }
+    tmem_st16(tl + 16 * i, w);
+  }
+  sum += s0 + s1;
+}
 }  // namespace
 
 template <bool kBf16, int kDim>
-__global__ void __launch_bounds__(kWarps * 32) attention_packed_kernel(const PackedAttention p) {
-  constexpr int kWords = kDim / 64;  // 32-bit words of a row per lane
-  const uint32_t lane = threadIdx.x % 32;
-  const uint64_t work = static_cast<uint64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-  const uint32_t t = static_cast<uint32_t>(work / p.q_heads), h = static_cast<uint32_t>(work % p.q_heads);
-  if (t >= p.total_q) return;
-  const int s = warp_find_sequence(p.cu_q, p.n_seq, t);
-  if (s < 0) return;
-  uint32_t q0, q1, k0, k1;
-  sequence_rows(p.cu_q, s, p.total_q, &q0, &q1);
-  sequence_rows(p.cu_k, s, p.total_k, &k0, &k1);
-  if (t < q0 || t >= q1) return;
-  int64_t visible = k1 - k0;
-  if (p.causal) visible = min(visible, visible - (q1 - q0) + (t - q0) + 1);
-  const uint32_t g = h / (p.q_heads / p.kv_heads);
-  float q[2 * kWords], o[2 * kWords] = {};
-  const uint32_t *qr = reinterpret_cast<const uint32_t *>(p.q + t * p.q_token + h * p.q_head) + lane * kWords;
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    const float2 x = Elem<kBf16>::unpack(qr[i]);
-    q[2 * i] = x.x * p.scale * kLog2e;
-    q[2 * i + 1] = x.y * p.scale * kLog2e;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < visible; ++j) {
-    const uint32_t *kr = reinterpret_cast<const uint32_t *>(p.k + (k0 + j) * p.k_token + g * p.k_head) + lane * kWords;
-    const uint32_t *vr = reinterpret_cast<const uint32_t *>(p.v + (k0 + j) * p.v_token + g * p.v_head) + lane * kWords;
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      const float2 x = Elem<kBf16>::unpack(kr[i]);
-      d = fmaf(q[2 * i], x.x, fmaf(q[2 * i + 1], x.y, d));
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_packed_kernel(const __grid_constant__ CUtensorMap tmq,
+                            const __grid_constant__ CUtensorMap tmk,
+                            const __grid_constant__ CUtensorMap tmv,
+                            const __grid_constant__ PackedArgs p) {
+  using L = Layout<kDim>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
+  uint64_t *q_empty = q_full + 2, *s_full = q_full + 4, *p_full = q_full + 6, *o_full = q_full + 8;
+  uint64_t *drain = q_full + 10, *sched_full = q_full + 12, *sched_empty = q_full + 14;
+  uint64_t *kv_full = q_full + 16, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages;
+  volatile Item *items = reinterpret_cast<volatile Item *>(smem + L::kItemOff);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kMiscOff);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  uint32_t *order = reinterpret_cast<uint32_t *>(smem + L::kOrderOff);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&drain[i], 1);
+      mbar_init(&sched_full[i], 1);
+      mbar_init(&sched_empty[i], 8 + 2 + 1);  // softmax warps, issuers, producer
     }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 2);  // both issuers
+      mbar_init(&v_ok[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    tma_prefetch_map(&tmq);
+    tma_prefetch_map(&tmk);
+    tma_prefetch_map(&tmv);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  for (int i = threadIdx.x; i < 2 * kBuckets; i += kThreads) order[i] = 0;
+  __syncthreads();
+  // Per bucket: sequences that end in it, and their levels there.
+  for (uint32_t s = threadIdx.x; s < p.n_seq; s += kThreads) {
+    const uint32_t n = tiles_of(p, s);
+    const uint32_t b = min(n / p.width, kBuckets - 1u);
+    atomicAdd(&order[kBuckets - 1 - b], 1u);
+    atomicAdd(&order[kBuckets + kBuckets - 1 - b], n - b * p.width);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int tokens = static_cast<int>(p.tokens);
+
+  if (warp == kGuardWarp) {
+    // Starts of the buckets, top first: levels of a bucket = those of sequences ending in it, and
+    // `width` for each sequence that ends in a higher one.
+    Order o = {order, 0, p.width, -1, 0, 0};
+    {
+      constexpr int kPer = kBuckets / 32;
+      uint32_t ends[kPer], levels[kPer], higher = 0;
 #pragma unroll
-    for (int i = 16; i > 0; i /= 2) d += __shfl_xor_sync(0xffffffffu, d, i);
-    const float top = fmaxf(m, d), base = top == -INFINITY ? 0.f : top;
-    const float keep = exp2f(m - base), w = exp2f(d - base);
-    l = fmaf(l, keep, w);
-    m = top;
+      for (int i = 0; i < kPer; ++i) {
+        ends[i] = order[lane * kPer + i];
+        levels[i] = order[kBuckets + lane * kPer + i];
+        higher += ends[i];
+      }
+      const uint32_t own = higher;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      const float2 x = Elem<kBf16>::unpack(vr[i]);
-      o[2 * i] = fmaf(o[2 * i], keep, w * x.x);
-      o[2 * i + 1] = fmaf(o[2 * i + 1], keep, w * x.y);
+      for (int i = 1; i < 32; i *= 2) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, higher, i);
+        if (lane >= i) higher += x;
+      }
+      higher -= own;
+      uint32_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t n = levels[i] + higher * p.width;
+        higher += ends[i];
+        ends[i] = sum;  // start within this lane
+        sum += n;
+      }
+      uint32_t before = sum;
+#pragma unroll
+      for (int i = 1; i < 32; i *= 2) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, before, i);
+        if (lane >= i) before += x;
+      }
+      o.total = __shfl_sync(0xffffffffu, before, 31);
+      before -= sum;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) order[lane * kPer + i] = before + ends[i];
+      __syncwarp();
+    }
+    const uint64_t n_items = static_cast<uint64_t>(o.total) * p.kv_heads;
+    bool ok = true;
+    // Publish item k of this CTA: up the order and down again in turn, so that no CTA always gets
+    // the longest of each round.
+    auto publish = [&](uint32_t k) {
+      const uint64_t at = static_cast<uint64_t>(k) * gridDim.x +
+                          (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      Item it = {};
+      if (at < n_items)
+        it = find_item(p, o, static_cast<uint32_t>(at / p.kv_heads), static_cast<uint32_t>(at % p.kv_heads));
+      // the up-and-down order may leave one CTA an item in a round in which others have none
+      it.last = static_cast<uint64_t>(k) * gridDim.x >= n_items;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sched_empty[k & 1], ((k >> 1) & 1) ^ 1u, abort_flag));
+      if (ok && lane == 0) {
+        volatile Item *d = &items[k & 1];
+        d->q_row = it.q_row;
+        d->q_count = it.q_count;
+        d->k_row = it.k_row;
+        d->k_len = it.k_len;
+        d->visible = it.visible;
+        d->head = it.head;
+        d->last = it.last;
+        d->fix = 0;
+        mbar_arrive(&sched_full[k & 1]);
+      }
+      return it;
+    };
+    uint32_t ring = 0, phase = 0, v_ring = 0;
+    Item it = publish(0);
+    for (uint32_t k = 0; ok && !it.last; ++k) {
+      const Item next = publish(k + 1);
+      if (!ok) break;
+      const Reach r0 = reach_of(it, 0, tokens, p.causal), r1 = reach_of(it, 1, tokens, p.causal);
+      const int steps = max(r0.steps, r1.steps), partial = r0.first / kKeys;
+      for (int j = 0; j < steps; ++j) {
+        if (++ring == kStages) ring = 0, phase ^= 1;  // the step's K stage
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[ring], phase, abort_flag));
+        if (!ok) break;
+        if (j >= partial) {
+          uint4 *x = reinterpret_cast<uint4 *>(smem + L::kRingOff + ring * L::kTileBytes);
+          uint32_t acc = 0;
+#pragma unroll 8
+          for (int i = lane; i < L::kTileBytes / 16; i += 32) {
+            const uint4 w = x[i];
+            acc = times_zero<kBf16>(w.x, acc);
+            acc = times_zero<kBf16>(w.y, acc);
+            acc = times_zero<kBf16>(w.z, acc);
+            acc = times_zero<kBf16>(w.w, acc);
+          }
+          if (__any_sync(0xffffffffu, !finite16<kBf16>(acc & 0xffffu) || !finite16<kBf16>(acc >> 16))) {
+            for (int i = lane; i < L::kTileBytes / 16; i += 32) {
+              uint4 w = x[i];
+              uint32_t *u = reinterpret_cast<uint32_t *>(&w);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (!finite16<kBf16>(u[e] & 0xffffu)) u[e] &= 0xffff0000u;
+                if (!finite16<kBf16>(u[e] >> 16)) u[e] &= 0x0000ffffu;
+              }
+              x[i] = w;
+            }
+            items[k & 1].fix = 1;
+            fence_proxy_async_smem();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ok[v_ring]);
+        if (++v_ring == kStages) v_ring = 0;
+        if (++ring == kStages) ring = 0, phase ^= 1;
+      }
+      it = next;
+    }
+    if (!ok && lane == 0) {
+      report(p.status, kErrAttentionWait);
+      *abort_flag = 1;
+    }
+  } else if (warp == kProducerWarp) {
+    if (lane == 0) {
+      uint32_t ring = 0, phase = 0, armed = 0, parity = 0;
+      uint32_t q_phase[2] = {0, 0};
+      bool q_armed[2] = {false, false}, ok = true;
+      auto load_kv = [&](const CUtensorMap *map, int row, int head) {
+        if (!mbar_wait(&kv_empty[ring], phase ^ 1u, abort_flag)) return false;
+        uint8_t *dst = smem + L::kRingOff + ring * L::kTileBytes;
+        mbar_arrive_expect_tx(&kv_full[ring], L::kTileBytes);
+#pragma unroll
+        for (int h = 0; h < L::kHalves; ++h)
+          tma_load_3d(dst + h * L::kHalfBytes, map, &kv_full[ring], 64 * h, head, row);
+        armed |= 1u << ring;
+        parity = (parity & ~(1u << ring)) | (phase << ring);
+        if (++ring == kStages) ring = 0, phase ^= 1;
+        return true;
+      };
+      for (uint32_t k = 0; ok; ++k) {
+        ok = mbar_wait(&sched_full[k & 1], (k >> 1) & 1, abort_flag);
+        if (!ok) break;
+        Item it;
+        it.q_row = items[k & 1].q_row;
+        it.q_count = items[k & 1].q_count;
+        it.k_row = items[k & 1].k_row;
+        it.k_len = items[k & 1].k_len;
+        it.visible = items[k & 1].visible;
+        it.head = items[k & 1].head;
+        it.last = items[k & 1].last;
+        mbar_arrive(&sched_empty[k & 1]);
+        if (it.last) break;
+        const Reach r[2] = {reach_of(it, 0, tokens, p.causal), reach_of(it, 1, tokens, p.causal)};
+        const int steps = max(r[0].steps, r[1].steps);
+        for (int j = 0; ok && j < steps; ++j) {
+          ok = load_kv(&tmk, it.k_row + j * kKeys, it.head);
+          if (j == 0) {
+            for (int t = 0; ok && t < 2; ++t) {
+              if (r[t].steps == 0) continue;
+              ok = mbar_wait(&q_empty[t], q_phase[t] ^ 1u, abort_flag);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&q_full[t], p.tokens * p.group * 128u * L::kHalves);
+#pragma unroll
+              for (int h = 0; h < L::kHalves; ++h)
+                tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &tmq, &q_full[t], 64 * h,
+                            it.head * static_cast<int>(p.group), it.q_row + t * tokens);
+              q_armed[t] = true;
+              q_phase[t] ^= 1;
+            }
+          }
+          ok = ok && load_kv(&tmv, it.k_row + j * kKeys, it.head);
+        }
+      }
+      if (!ok) {
+        report(p.status, kErrAttentionWait);
+        *abort_flag = 1;
+      }
+      // Copies still in flight (only after an abort) land before shared memory is released.
+      for (int i = 0; i < kStages; ++i)
+        if ((armed >> i) & 1u) mbar_drain(&kv_full[i], (parity >> i) & 1u);
+      for (int t = 0; t < 2; ++t)
+        if (q_armed[t]) mbar_drain(&q_full[t], q_phase[t] ^ 1u);
+    }
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    if (lane == 0) {
+      const int t = warp - kMmaWarp;
+      constexpr uint32_t idesc_s = idesc_f32(kBf16, 128, kKeys, false);
+      constexpr uint32_t idesc_o = idesc_f32(kBf16, 128, kDim, true);
+      const uint32_t d_s = tmem + t * 128, d_o = tmem + kTmemO + t * 128;
+      const uint32_t q_at = smem_u32(smem + t * L::kTileBytes);
+      uint32_t ring = 0, phase = 0, v_ring = 0, v_phase = 0, p_phase = 0, q_phase = 0;
+      bool ok = true;
+      // S = Q K^T of the stage at `ring`, or only its release where this tile has no more steps.
+      auto scores = [&](bool mine, bool last) {
+        if (!mbar_wait(&kv_full[ring], phase, abort_flag)) return false;
+        if (mine) {
+          tc_fence_after();
+          const uint32_t k_at = smem_u32(smem + L::kRingOff + ring * L::kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < kDim / 16; ++kk) {
+            const uint32_t off = (kk / 4) * L::kHalfBytes + (kk % 4) * 32;
+            umma_f16(d_s, sw128_desc(q_at + off), sw128_desc(k_at + off), idesc_s, kk > 0);
+          }
+          umma_commit(&s_full[t]);
+          umma_commit(&kv_empty[ring]);
+          if (last) umma_commit(&q_empty[t]);
+        } else {
+          mbar_arrive(&kv_empty[ring]);
+        }
+        if (++ring == kStages) ring = 0, phase ^= 1;
+        return true;
+      };
+      for (uint32_t k = 0; ok; ++k) {
+        ok = mbar_wait(&sched_full[k & 1], (k >> 1) & 1, abort_flag);
+        if (!ok) break;
+        Item it;
+        it.q_count = items[k & 1].q_count;
+        it.k_len = items[k & 1].k_len;
+        it.visible = items[k & 1].visible;
+        it.last = items[k & 1].last;
+        mbar_arrive(&sched_empty[k & 1]);
+        if (it.last) break;
+        const int mine = reach_of(it, t, tokens, p.causal).steps;
+        const int steps = max(mine, reach_of(it, 1 - t, tokens, p.causal).steps);
+        if (steps == 0) continue;
+        if (mine > 0) {
+          ok = mbar_wait(&q_full[t], q_phase, abort_flag);
+          q_phase ^= 1;
+        }
+        ok = ok && scores(mine > 0, mine == 1);
+        for (int j = 0; ok && j < steps; ++j) {
+          // the step's V
+          ok = mbar_wait(&kv_full[ring], phase, abort_flag) && mbar_wait(&v_ok[v_ring], v_phase, abort_flag);
+          if (!ok) break;
+          if (++v_ring == kStages) v_ring = 0, v_phase ^= 1;
+          if (j < mine) {
+            ok = mbar_wait(&p_full[t], p_phase, abort_flag);
+            if (!ok) break;
+            p_phase ^= 1;
+            tc_fence_after();
+            const uint32_t v_at = smem_u32(smem + L::kRingOff + ring * L::kTileBytes);
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
+                          j > 0 || kk > 0);
+            umma_commit(&o_full[t]);
+            umma_commit(&kv_empty[ring]);
+          } else {
+            mbar_arrive(&kv_empty[ring]);
+          }
+          if (++ring == kStages) ring = 0, phase ^= 1;
+          if (j + 1 < steps) ok = scores(j + 1 < mine, j + 2 == mine);
+        }
+      }
+      if (!ok) {
+        report(p.status, kErrAttentionWait);
+        *abort_flag = 1;
+      }
+      umma_commit(&drain[t]);  // every MMA this thread issued has completed before TMEM is freed
+      mbar_drain(&drain[t], 0);
+    }
+  } else {
+    const int t = warp >> 2, q = warp & 3;
+    const int row = q * 32 + lane;
+    const int token = row / static_cast<int>(p.group), sub = row % static_cast<int>(p.group);
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t tl = tmem + lanes + t * 128, to = tmem + lanes + kTmemO + t * 128;
+    const float c = p.scale_log2;
+    uint32_t s_phase = 0, o_count = 0;  // products of this tile so far
+    bool ok = true;
+    for (uint32_t k = 0; ok; ++k) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&sched_full[k & 1], (k >> 1) & 1, abort_flag));
+      if (!ok) break;
+      Item it;
+      it.q_row = items[k & 1].q_row;
+      it.q_count = items[k & 1].q_count;
+      it.k_row = items[k & 1].k_row;
+      it.k_len = items[k & 1].k_len;
+      it.visible = items[k & 1].visible;
+      it.head = items[k & 1].head;
+      it.last = items[k & 1].last;
+      __syncwarp();
+      const Reach r = reach_of(it, t, tokens, p.causal);
+      const int whole = r.first / kKeys;  // steps that every row of the tile sees in full
+      const int mine = t * tokens + token;  // token within the item
+      const int sees = p.causal ? min(it.k_len, it.visible + mine) : it.k_len;
+      float m = -INFINITY, sum = 0.f;
+      for (int j = 0; j < r.steps; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], s_phase, abort_flag));
+        if (!ok) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        if (j < whole)
+          softmax_step<kBf16, false>(tl, to, kDim, c, kKeys, j == 0, m, sum, &o_full[t],
+                                     (o_count - 1) & 1u, abort_flag, ok);
+        else
+          softmax_step<kBf16, true>(tl, to, kDim, c, sees - j * kKeys, j == 0, m, sum, &o_full[t],
+                                    (o_count - 1) & 1u, abort_flag, ok);
+        if (!ok) break;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
+        ++o_count;
+      }
+      if (!ok) break;
+      if (r.steps > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], (o_count - 1) & 1u, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const int fix = r.steps > 0 ? items[k & 1].fix : 0;
+      __syncwarp();
+      // From here on the slot is not read again; the next item but one may be written into it.
+      if (lane == 0) mbar_arrive(&sched_empty[k & 1]);
+      if (it.last) break;
+      const bool live = token < tokens && mine < it.q_count;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
+      const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
+      uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
+      if (live && p.lse) p.lse[out_row * p.q_heads + head] = (m + log2f(sum)) * kLn2;
+#pragma unroll
+      for (int d = 0; d < kDim; d += 32) {
+        uint32_t x[32];
+        if (r.steps > 0) {
+          tmem_load32(to + d, x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = 0;
+        }
+        if (fix && live) {
+          // what the guard took out of the steps that are seen in part
+          const int from = reach_of(it, 0, tokens, p.causal).first / kKeys * kKeys;
+          for (int kk = from; kk < sees; ++kk) {
+            const uint32_t *v = reinterpret_cast<const uint32_t *>(
+                p.v + (static_cast<int64_t>(it.k_row) + kk) * p.v_token + it.head * p.v_head + d);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint32_t w = v[e];
+              const float2 f = Elem<kBf16>::unpack(w);
+              if (!finite16<kBf16>(w & 0xffffu)) x[2 * e] = __float_as_uint(__uint_as_float(x[2 * e]) + f.x);
+              if (!finite16<kBf16>(w >> 16)) x[2 * e + 1] = __float_as_uint(__uint_as_float(x[2 * e + 1]) + f.y);
+            }
+          }
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          w[e] = Elem<kBf16>::pack(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv);
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<uint4 *>(dst + d + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+    if (!ok && lane == 0) {
+      report(p.status, kErrAttentionWait);
+      *abort_flag = 1;
     }
   }
-  const float inv = visible > 0 ? 1.f / l : 0.f;
-  uint32_t *out = reinterpret_cast<uint32_t *>(p.out + t * p.out_token + h * p.out_head) + lane * kWords;
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) out[i] = Elem<kBf16>::pack(o[2 * i] * inv, o[2 * i + 1] * inv);
-  if (p.lse && lane == 0)
-    p.lse[static_cast<int64_t>(t) * p.q_heads + h] = visible > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
 }
 
-cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream) {
-  const uint64_t work = static_cast<uint64_t>(p.total_q) * p.q_heads;
-  if (work == 0 || p.n_seq == 0) return cudaSuccess;
-  const uint64_t grid = (work + kWarps - 1) / kWarps;
-  if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  const dim3 g(static_cast<uint32_t>(grid)), b(kWarps * 32);
-  if (p.head_dim == 64) {
-    if (bf16)
-      attention_packed_kernel<true, 64><<<g, b, 0, stream>>>(p);
-    else
-      attention_packed_kernel<false, 64><<<g, b, 0, stream>>>(p);
-  } else {
-    if (bf16)
-      attention_packed_kernel<true, 128><<<g, b, 0, stream>>>(p);
-    else
-      attention_packed_kernel<false, 128><<<g, b, 0, stream>>>(p);
+namespace {
+template <bool kBf16, int kDim>
+cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v,
+                   const PackedArgs &a, int dev, uint32_t grid, cudaStream_t stream) {
+  static std::atomic<bool> configured[64] = {};
+  if (dev >= 0 && dev < 64 && !configured[dev].load(std::memory_order_acquire)) {
+    // setting the attribute twice (two threads racing here) is harmless
+    const cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<kBf16, kDim>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               Layout<kDim>::kBytes);
+    if (e != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
   }
+  attention_packed_kernel<kBf16, kDim>
+      <<<dim3(grid), dim3(kThreads), Layout<kDim>::kBytes, stream>>>(q, k, v, a);
   return cudaGetLastError();
+}
+}  // namespace
+
+cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,
+                                    std::string *err) {
+  if (p.total_q == 0 || p.n_seq == 0) return cudaSuccess;
+  const uint32_t group = p.q_heads / p.kv_heads, tokens = 128 / group;
+  CUtensorMap q, k, v;
+  const bool maps =
+      encode_map_rows(&q, p.q, bf16, p.head_dim, p.q_heads, p.total_q, p.q_head, p.q_token, group, tokens, err) &&
+      // without keys the maps stand on q: no load reads through them
+      encode_map_rows(&k, p.total_k ? p.k : p.q, bf16, p.head_dim, p.kv_heads, p.total_k ? p.total_k : 1, p.k_head,
+                      p.k_token, 1, kKeys, err) &&
+      encode_map_rows(&v, p.total_k ? p.v : p.q, bf16, p.head_dim, p.kv_heads, p.total_k ? p.total_k : 1, p.v_head,
+                      p.v_token, 1, kKeys, err);
+  if (!maps) return cudaErrorInvalidValue;
+  PackedArgs a = {};
+  a.v = p.v;
+  a.out = p.out;
+  a.lse = p.lse;
+  a.cu_q = p.cu_q;
+  a.cu_k = p.cu_k;
+  a.v_token = p.v_token;
+  a.v_head = p.v_head;
+  a.out_token = p.out_token;
+  a.out_head = p.out_head;
+  a.status = p.status;
+  a.n_seq = p.n_seq;
+  a.total_q = p.total_q;
+  a.total_k = p.total_k;
+  a.q_heads = p.q_heads;
+  a.kv_heads = p.kv_heads;
+  a.group = group;
+  a.tokens = tokens;
+  a.causal = p.causal;
+  a.scale_log2 = p.scale * kLog2e;
+  const uint64_t levels = (static_cast<uint64_t>(p.total_q) + 2 * tokens - 1) / (2 * tokens);
+  a.width = static_cast<uint32_t>((levels + kBuckets - 1) / kBuckets);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  // at most one partly filled item per sequence
+  const uint64_t most = (levels + p.n_seq) * p.kv_heads;
+  const uint32_t sms = static_cast<uint32_t>(sm_count(dev));
+  const uint32_t grid = most < sms ? static_cast<uint32_t>(most) : sms;
+  if (p.head_dim == 64)
+    return bf16 ? launch<true, 64>(q, k, v, a, dev, grid, stream) : launch<false, 64>(q, k, v, a, dev, grid, stream);
+  return bf16 ? launch<true, 128>(q, k, v, a, dev, grid, stream) : launch<false, 128>(q, k, v, a, dev, grid, stream);
 }
 
 }  // namespace dv3

@@ -503,8 +503,8 @@ uint32_t dv3k_gateup_source_row(uint32_t packed_row) { return dv3::gateup_source
 
 namespace {
 
-// A stride of an extent of one row or head is never used: 8 stands for whatever it is.
-int64_t used_stride(int64_t stride, uint32_t extent) { return extent > 1 ? stride : 8; }
+// A stride of an extent of one row or head is never used: 128 stands for whatever it is.
+int64_t used_stride(int64_t stride, uint32_t extent) { return extent > 1 ? stride : 128; }
 
 bool strides_ok(int64_t row, uint32_t rows, int64_t head, uint32_t heads) {
   constexpr int64_t kMost = int64_t{1} << 38;  // a tensor map's strides stay below 2^40 bytes
@@ -633,9 +633,11 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
   p.scale = a->scale;
-  return launch_status(
-      dv3::launch_attention_packed(p, a->dtype == DV3K_BF16, static_cast<cudaStream_t>(stream)),
-      "attention_packed");
+  std::string err;
+  const cudaError_t e = dv3::launch_attention_packed(p, a->dtype == DV3K_BF16,
+                                                     static_cast<cudaStream_t>(stream), &err);
+  if (!err.empty()) return bad_args(err.c_str());
+  return launch_status(e, "attention_packed");
 }
 
 int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {

@@ -46,6 +46,13 @@ bool encode_map_f16_images(CUtensorMap *map, const void *base, uint64_t cols, ui
 bool encode_map_f32_slabs(CUtensorMap *map, const void *base, uint64_t cols, uint64_t rows,
                           uint64_t slabs, uint32_t box_rows, std::string *err);
 
+// 3D 16-bit view [rows][heads][dim] with the given strides in elements (multiples of 8), box = 64
+// columns x box_heads x box_rows, 128-byte swizzle: a tile's rows are (row, head) pairs, heads
+// innermost. Rows past the tensor read as zeros.
+bool encode_map_rows(CUtensorMap *map, const void *base, bool bf16, uint64_t dim, uint64_t heads,
+                     uint64_t rows, uint64_t head_stride, uint64_t row_stride, uint32_t box_heads,
+                     uint32_t box_rows, std::string *err);
+
 // ---- GEMM operations (gemm.cu) ----
 // Resid*: x += lambda (A W^T + b) on 128-column tiles. ResidLN*: the same on full 384-column
 // rows, followed in the same kernel by the LayerNorm of the updated row into ln_out (f16) or
@@ -196,7 +203,9 @@ struct PackedAttention {
   bool causal;
   float scale;
 };
-cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream);
+// cudaErrorInvalidValue with *err set where a tensor map cannot be built.
+cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,
+                                    std::string *err);
 
 // A page size and its shift (32 where it is no power of two).
 struct PageDiv {

@@ -149,4 +149,28 @@ bool encode_map_f32_slabs(CUtensorMap *map, const void *base, uint64_t cols, uin
   return true;
 }
 
+bool encode_map_rows(CUtensorMap *map, const void *base, bool bf16, uint64_t dim, uint64_t heads,
+                     uint64_t rows, uint64_t head_stride, uint64_t row_stride, uint32_t box_heads,
+                     uint32_t box_rows, std::string *err) {
+  auto fn = encode_fn(err);
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {dim, heads, rows};
+  const cuuint64_t strides[2] = {head_stride * 2, row_stride * 2};
+  const cuuint32_t box[3] = {64, box_heads, box_rows};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void *>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    if (err) {
+      char buf[128];
+      std::snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+      *err = buf;
+    }
+    return false;
+  }
+  return true;
+}
+
 }  // namespace dv3
