@@ -6,22 +6,27 @@ Every source in csrc/ is compiled by nvcc with `-gencode arch=compute_100a,code=
 (`-Xptxas -v` output lands in _build/ptxas.log) and linked with the static CUDA runtime into
 dinov3_b200/libdinov3.so. The library does not link libcuda (driver entry points are looked up
 at run time), so it loads on a machine without a GPU. Objects are rebuilt when a source or
-header is newer than them.
+header is newer than them. Where torch is installed, binding/sequence.cpp is compiled into
+dinov3_b200/_sequence.so (the tensor arguments of dinov3_b200/sequence.py); nothing else needs it.
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "dinov3_b200", "libdinov3.so")
+BINDING = os.path.join(HERE, "binding", "sequence.cpp")
+BINDING_LIB = os.path.join(HERE, "dinov3_b200", "_sequence.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -51,11 +56,32 @@ def _compile(src: str, force: bool):
     return obj, r.stdout
 
 
+def _build_binding(force: bool):
+    found = importlib.util.find_spec("torch")
+    if found is None:
+        return
+    torch = found.submodule_search_locations[0]
+    newest = max(os.path.getmtime(f) for f in [BINDING, *glob.glob(os.path.join(ROOT, "include", "*.h"))])
+    if not force and os.path.exists(BINDING_LIB) and os.path.getmtime(BINDING_LIB) >= newest:
+        return
+    include = [os.path.join(ROOT, "include"), os.path.join(torch, "include"),
+               os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"]]
+    cmd = [NVCC, "-O2", "-std=c++17", "-shared", "-cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+           *("-I" + d for d in include), BINDING, "-o", BINDING_LIB, "-L" + os.path.join(torch, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding failed:\n{r.stdout}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
+        binding = ex.submit(_build_binding, force)
         results = list(ex.map(lambda s: _compile(s, force), srcs))
+        binding.result()
     objs = [o for o, _ in results]
     log = "".join(out for _, out in results)
     if log:

@@ -22,10 +22,9 @@
 //              output is then rescaled in TMEM. At an item's end O / sum is written, 32 bytes a
 //              store.
 //   warp 8     TMA producer: Q tiles, then K and V tiles in turn through one ring of stages.
-//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = N = 128), then O_t += P_t V with
-//              P from TMEM and V as the MN-major B operand. Each walks the ring by itself, so the
-//              softmax of one tile overlaps the products of the other.
-//   warp 11    scheduler, and guard of V: a key that a row does not see has weight 0, but 0 times
+//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = N = 128), and O_t += P_t V with P
+//              from TMEM and V as the MN-major B operand, one tile at a time.
+//   warp 11    scheduler (publishes items one ahead), and guard of V: a key that a row does not see has weight 0, but 0 times
 //              an infinity or NaN is NaN. Only the tiles at an item's end (from the first that some
 //              row sees in part) can hold such keys; there it tests V in shared memory, sets what
 //              is not finite to 0 and leaves a note, and the rows that do see those keys add them
@@ -72,12 +71,12 @@ struct Layout {
   static constexpr int kStages = kDim == 128 ? 5 : 8;
   static constexpr int kRingOff = 2 * kTileBytes;   // Q_0 | Q_1 | stages
   static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
-  // barriers: q_full[2] q_empty[2] s_full[2] p_full[2] o_full[2] drain[2] sched_full[2]
-  // sched_empty[2] kv_full[stages] kv_empty[stages] v_ok[stages] (by V tile, not by stage: a stage
+  // barriers: q_full[2] q_empty[2] s_full[2] p_full[4] (first halves, second halves) o_full[2]
+  // drain[2] sched_full[3] sched_empty[3] kv_full[stages] kv_empty[stages] v_ok[stages] (by V tile, not by stage: a stage
   // of an odd ring holds K and V in turn)
-  static constexpr int kBars = 16 + 3 * kStages;
+  static constexpr int kBars = 20 + 3 * kStages;
   static constexpr int kItemOff = kBarOff + kBars * 8;
-  static constexpr int kMiscOff = kItemOff + 2 * static_cast<int>(sizeof(Item));  // TMEM slot, abort
+  static constexpr int kMiscOff = kItemOff + 3 * static_cast<int>(sizeof(Item));  // TMEM slot, abort, turn
   static constexpr int kOrderOff = kMiscOff + 16;
   static constexpr int kBytes = 1024 + kOrderOff + 2 * kBuckets * 4;
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
@@ -92,6 +91,36 @@ __host__ __device__ constexpr uint32_t idesc_f32(bool bf16, uint32_t m, uint32_t
 __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t smem_addr, uint32_t column_bytes) {
   return (sw128_desc(smem_addr) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(column_bytes >> 4) << 16);
 }
+
+// Two f32 at once (Blackwell's packed f32 operations, one issue slot for both).
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  return pair(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Registers of a warpgroup: the kernel starts with 168 a thread (384 x 168 = 64512); the softmax
+// warps hold a step's 128 scores and take 216, the other four keep 72 (256 x 216 + 128 x 72 = 64512).
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -215,11 +244,11 @@ __device__ __forceinline__ bool finite16(uint32_t half) {
 }
 
 // Scores, weights and sums of one step for this thread's row. `vis`: keys of this step that the row
-// sees (used where kMasked). Returns through m (reference, log2 units), sum.
+// sees (used where kMasked). Returns through m (reference, log2 units), sum. The weights are handed
+// over in two halves (p_full[0], p_full[2]), so that the product with V starts under the second.
 template <bool kBf16, bool kMasked>
 __device__ __forceinline__ void softmax_step(uint32_t tl, uint32_t to, int dim, float c, int vis,
-                                             bool first, float &m, float &sum, uint64_t *o_full,
-                                             uint32_t o_parity, volatile int *abort_flag, bool &ok) {
+                                             bool first, float &m, float &sum, uint64_t *p_full) {
   uint32_t v[4][32];
 #pragma unroll
   for (int i = 0; i < 4; ++i) tmem_ld32(tl + 32 * i, v[i]);
@@ -248,16 +277,12 @@ __device__ __forceinline__ void softmax_step(uint32_t tl, uint32_t to, int dim, 
   } else {
     const bool grown = now > m + kSlack;
     if (__any_sync(0xffffffffu, grown)) {
-      // rescale this row's output (factor 1 for rows that stay); the previous product must be done
+      // rescale this row's output (factor 1 for rows that stay); the previous product is done: the
+      // same thread issued it before these scores
       const float next = grown ? now : m;
       const float f = grown ? ex2_approx(m - next) : 1.f;
       sum *= f;
       m = next;
-      if (!__all_sync(0xffffffffu, mbar_wait(o_full, o_parity, abort_flag))) {
-        ok = false;
-        return;
-      }
-      tc_fence_after();
       for (int d = 0; d < dim; d += 16) {
         uint32_t x[16];
         tmem_ld16(to + d, x);
@@ -270,21 +295,33 @@ __device__ __forceinline__ void softmax_step(uint32_t tl, uint32_t to, int dim, 
     }
   }
   const float base = m == -INFINITY ? 0.f : m;
-  float s0 = 0.f, s1 = 0.f;
+  const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
+  uint64_t s0 = 0, s1 = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float a = ex2_approx(fmaf(__uint_as_float(v[i][2 * e]), c, -base));
-      const float b = ex2_approx(fmaf(__uint_as_float(v[i][2 * e + 1]), c, -base));
-      s0 += a;
-      s1 += b;
-      w[e] = Elem<kBf16>::pack(a, b);
+      const uint64_t x2 = fma2(pair(v[i][2 * e], v[i][2 * e + 1]), c2, base2);
+      const float2 x = unpair(x2);
+      const uint64_t w2 = pair(ex2_approx(x.x), ex2_approx(x.y));
+      if (e & 1)
+        s1 = add2(s1, w2);
+      else
+        s0 = add2(s0, w2);
+      const float2 f = unpair(w2);
+      w[e] = Elem<kBf16>::pack(f.x, f.y);
     }
     tmem_st16(tl + 16 * i, w);
+    if (i == 1 || i == 3) {
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (threadIdx.x % 32 == 0) mbar_arrive(p_full + (i == 1 ? 0 : 2));
+    }
   }
-  sum += s0 + s1;
+  const float2 part = unpair(add2(s0, s1));
+  sum += part.x + part.y;
 }
 }  // namespace
 
@@ -299,12 +336,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
-  uint64_t *q_empty = q_full + 2, *s_full = q_full + 4, *p_full = q_full + 6, *o_full = q_full + 8;
-  uint64_t *drain = q_full + 10, *sched_full = q_full + 12, *sched_empty = q_full + 14;
-  uint64_t *kv_full = q_full + 16, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages;
+  uint64_t *q_empty = q_full + 2, *s_full = q_full + 4, *p_full = q_full + 6, *o_full = q_full + 10;
+  uint64_t *drain = q_full + 12, *sched_full = q_full + 14, *sched_empty = q_full + 17;
+  uint64_t *kv_full = q_full + 20, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages;
   volatile Item *items = reinterpret_cast<volatile Item *>(smem + L::kItemOff);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kMiscOff);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  uint32_t *turn = tmem_slot + 2;
   uint32_t *order = reinterpret_cast<uint32_t *>(smem + L::kOrderOff);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -313,18 +351,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);  // the tile's softmax warps
+      mbar_init(&p_full[2 + i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&drain[i], 1);
+    }
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&sched_full[i], 1);
-      mbar_init(&sched_empty[i], 8 + 2 + 1);  // softmax warps, issuers, producer
+      mbar_init(&sched_empty[i], 8 + 3);  // softmax warps, producer, issuers
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 2);  // both issuers
+      mbar_init(&kv_empty[i], 2);  // both tiles
       mbar_init(&v_ok[i], 1);
     }
     *abort_flag = 0;
+    *turn = 0;
     fence_mbar_init();
   }
   if (warp == kProducerWarp && lane == 0) {
@@ -352,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tokens = static_cast<int>(p.tokens);
 
   if (warp == kGuardWarp) {
+    fewer_registers();
     // Starts of the buckets, top first: levels of a bucket = those of sequences ending in it, and
     // `width` for each sequence that ends in a higher one.
     Order o = {order, 0, p.width, -1, 0, 0};
@@ -404,9 +447,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         it = find_item(p, o, static_cast<uint32_t>(at / p.kv_heads), static_cast<uint32_t>(at % p.kv_heads));
       // the up-and-down order may leave one CTA an item in a round in which others have none
       it.last = static_cast<uint64_t>(k) * gridDim.x >= n_items;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sched_empty[k & 1], ((k >> 1) & 1) ^ 1u, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(&sched_empty[k % 3], ((k / 3) & 1) ^ 1u, abort_flag));
       if (ok && lane == 0) {
-        volatile Item *d = &items[k & 1];
+        volatile Item *d = &items[k % 3];
         d->q_row = it.q_row;
         d->q_count = it.q_count;
         d->k_row = it.k_row;
@@ -415,10 +458,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         d->head = it.head;
         d->last = it.last;
         d->fix = 0;
-        mbar_arrive(&sched_full[k & 1]);
+        mbar_arrive(&sched_full[k % 3]);
       }
       return it;
     };
+    if (!ok && lane == 0) {
+      report(p.status, kErrAttentionWait);
+      *abort_flag = 1;
+    }
     uint32_t ring = 0, phase = 0, v_ring = 0;
     Item it = publish(0);
     for (uint32_t k = 0; ok && !it.last; ++k) {
@@ -452,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               x[i] = w;
             }
-            items[k & 1].fix = 1;
+            items[k % 3].fix = 1;
             fence_proxy_async_smem();
           }
         }
@@ -468,6 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       *abort_flag = 1;
     }
   } else if (warp == kProducerWarp) {
+    fewer_registers();
     if (lane == 0) {
       uint32_t ring = 0, phase = 0, armed = 0, parity = 0;
       uint32_t q_phase[2] = {0, 0};
@@ -485,17 +533,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       for (uint32_t k = 0; ok; ++k) {
-        ok = mbar_wait(&sched_full[k & 1], (k >> 1) & 1, abort_flag);
+        ok = mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag);
         if (!ok) break;
         Item it;
-        it.q_row = items[k & 1].q_row;
-        it.q_count = items[k & 1].q_count;
-        it.k_row = items[k & 1].k_row;
-        it.k_len = items[k & 1].k_len;
-        it.visible = items[k & 1].visible;
-        it.head = items[k & 1].head;
-        it.last = items[k & 1].last;
-        mbar_arrive(&sched_empty[k & 1]);
+        it.q_row = items[k % 3].q_row;
+        it.q_count = items[k % 3].q_count;
+        it.k_row = items[k % 3].k_row;
+        it.k_len = items[k % 3].k_len;
+        it.visible = items[k % 3].visible;
+        it.head = items[k % 3].head;
+        it.last = items[k % 3].last;
+        mbar_arrive(&sched_empty[k % 3]);
         if (it.last) break;
         const Reach r[2] = {reach_of(it, 0, tokens, p.causal), reach_of(it, 1, tokens, p.causal)};
         const int steps = max(r[0].steps, r[1].steps);
@@ -529,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (q_armed[t]) mbar_drain(&q_full[t], q_phase[t] ^ 1u);
     }
   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    fewer_registers();
     if (lane == 0) {
       const int t = warp - kMmaWarp;
       constexpr uint32_t idesc_s = idesc_f32(kBf16, 128, kKeys, false);
@@ -537,66 +586,114 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q_at = smem_u32(smem + t * L::kTileBytes);
       uint32_t ring = 0, phase = 0, v_ring = 0, v_phase = 0, p_phase = 0, q_phase = 0;
       bool ok = true;
-      // S = Q K^T of the stage at `ring`, or only its release where this tile has no more steps.
-      auto scores = [&](bool mine, bool last) {
-        if (!mbar_wait(&kv_full[ring], phase, abort_flag)) return false;
-        if (mine) {
-          tc_fence_after();
-          const uint32_t k_at = smem_u32(smem + L::kRingOff + ring * L::kTileBytes);
-#pragma unroll
-          for (int kk = 0; kk < kDim / 16; ++kk) {
-            const uint32_t off = (kk / 4) * L::kHalfBytes + (kk % 4) * 32;
-            umma_f16(d_s, sw128_desc(q_at + off), sw128_desc(k_at + off), idesc_s, kk > 0);
-          }
-          umma_commit(&s_full[t]);
-          umma_commit(&kv_empty[ring]);
-          if (last) umma_commit(&q_empty[t]);
-        } else {
-          mbar_arrive(&kv_empty[ring]);
+      // One tile at a time puts its products on the tensor cores. Left to interleave, both tiles'
+      // would end together, both softmaxes would start together, and the tiles would stay in step,
+      // the tensor cores idle under the softmax and the other way round (2.30 ms for 16384 causal
+      // tokens against 2.12); taken in turn, one falls half a step behind the other by itself.
+      auto take = [&] {
+        if (atomicCAS(turn, 0u, 1u) == 0u) return true;
+        const uint64_t t0 = globaltimer();
+        while (true) {
+#pragma unroll 1
+          for (int i = 0; i < 64; ++i)
+            if (atomicCAS(turn, 0u, 1u) == 0u) return true;
+          if (*abort_flag || globaltimer() - t0 > kWaitTimeoutNs) return false;
         }
-        if (++ring == kStages) ring = 0, phase ^= 1;
-        return true;
+      };
+      auto give = [&] { *reinterpret_cast<volatile uint32_t *>(turn) = 0u; };
+      // S = Q K^T of stage `stage`, the last of a turn.
+      auto scores = [&](uint32_t stage) {
+        const uint32_t k_at = smem_u32(smem + L::kRingOff + stage * L::kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < kDim / 16; ++kk) {
+          const uint32_t off = (kk / 4) * L::kHalfBytes + (kk % 4) * 32;
+          umma_f16(d_s, sw128_desc(q_at + off), sw128_desc(k_at + off), idesc_s, kk > 0);
+        }
+        give();
+      };
+      // One commit, for the softmax, covers the scores and all before: the softmax releases the
+      // stages when it sees it (a commit holds the issuing thread about 100 cycles).
+      auto hand_over = [&](bool last) {
+        umma_commit(&s_full[t]);
+        if (last) umma_commit(&q_empty[t]);
+      };
+      // Half of O += P V.
+      auto product = [&](uint32_t v_at, int half, bool first) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) {
+          const int kk = half * (kKeys / 32) + i;
+          umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
+                      !first || kk > 0);
+        }
       };
       for (uint32_t k = 0; ok; ++k) {
-        ok = mbar_wait(&sched_full[k & 1], (k >> 1) & 1, abort_flag);
+        ok = mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag);
         if (!ok) break;
         Item it;
-        it.q_count = items[k & 1].q_count;
-        it.k_len = items[k & 1].k_len;
-        it.visible = items[k & 1].visible;
-        it.last = items[k & 1].last;
-        mbar_arrive(&sched_empty[k & 1]);
+        it.q_count = items[k % 3].q_count;
+        it.k_len = items[k % 3].k_len;
+        it.visible = items[k % 3].visible;
+        it.last = items[k % 3].last;
+        mbar_arrive(&sched_empty[k % 3]);
         if (it.last) break;
         const int mine = reach_of(it, t, tokens, p.causal).steps;
         const int steps = max(mine, reach_of(it, 1 - t, tokens, p.causal).steps);
         if (steps == 0) continue;
+        uint32_t k_stage = ring;
+        ok = mbar_wait(&kv_full[ring], phase, abort_flag);
+        if (!ok) break;
+        if (++ring == kStages) ring = 0, phase ^= 1;
         if (mine > 0) {
-          ok = mbar_wait(&q_full[t], q_phase, abort_flag);
+          ok = mbar_wait(&q_full[t], q_phase, abort_flag) && take();
+          if (!ok) break;
           q_phase ^= 1;
+          tc_fence_after();
+          scores(k_stage);
+          hand_over(mine == 1);
+        } else {
+          mbar_arrive(&kv_empty[k_stage]);
         }
-        ok = ok && scores(mine > 0, mine == 1);
-        for (int j = 0; ok && j < steps; ++j) {
-          // the step's V
+        for (int j = 0; j < steps; ++j) {
+          // this step's V, and the next step's K behind it
+          const uint32_t v_stage = ring;
           ok = mbar_wait(&kv_full[ring], phase, abort_flag) && mbar_wait(&v_ok[v_ring], v_phase, abort_flag);
           if (!ok) break;
           if (++v_ring == kStages) v_ring = 0, v_phase ^= 1;
-          if (j < mine) {
-            ok = mbar_wait(&p_full[t], p_phase, abort_flag);
-            if (!ok) break;
-            p_phase ^= 1;
-            tc_fence_after();
-            const uint32_t v_at = smem_u32(smem + L::kRingOff + ring * L::kTileBytes);
-#pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
-                          j > 0 || kk > 0);
-            umma_commit(&o_full[t]);
-            umma_commit(&kv_empty[ring]);
-          } else {
-            mbar_arrive(&kv_empty[ring]);
-          }
           if (++ring == kStages) ring = 0, phase ^= 1;
-          if (j + 1 < steps) ok = scores(j + 1 < mine, j + 2 == mine);
+          const bool more = j + 1 < steps;
+          if (more) {
+            k_stage = ring;
+            ok = mbar_wait(&kv_full[ring], phase, abort_flag);
+            if (!ok) break;
+            if (++ring == kStages) ring = 0, phase ^= 1;
+          }
+          if (j >= mine) {
+            mbar_arrive(&kv_empty[v_stage]);
+            if (more) mbar_arrive(&kv_empty[k_stage]);
+            continue;
+          }
+          const uint32_t v_at = smem_u32(smem + L::kRingOff + v_stage * L::kTileBytes);
+          ok = mbar_wait(&p_full[t], p_phase, abort_flag) && take();
+          if (!ok) break;
+          tc_fence_after();
+          product(v_at, 0, j == 0);
+          // where the second half is there by now, the turn is kept
+          if (!mbar_test(&p_full[2 + t], p_phase)) {
+            give();
+            ok = mbar_wait(&p_full[2 + t], p_phase, abort_flag) && take();
+            if (!ok) break;
+          }
+          p_phase ^= 1;
+          tc_fence_after();
+          product(v_at, 1, j == 0);
+          if (j + 1 < mine) {
+            scores(k_stage);
+            hand_over(j + 2 == mine);
+          } else {
+            give();
+            umma_commit(&o_full[t]);
+            if (more) mbar_arrive(&kv_empty[k_stage]);
+          }
         }
       }
       if (!ok) {
@@ -607,25 +704,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_drain(&drain[t], 0);
     }
   } else {
+    more_registers();
     const int t = warp >> 2, q = warp & 3;
     const int row = q * 32 + lane;
     const int token = row / static_cast<int>(p.group), sub = row % static_cast<int>(p.group);
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tl = tmem + lanes + t * 128, to = tmem + lanes + kTmemO + t * 128;
     const float c = p.scale_log2;
-    uint32_t s_phase = 0, o_count = 0;  // products of this tile so far
+    uint32_t s_phase = 0, o_phase = 0, ring = 0;
+    // Release the stage at `ring`, for this tile, once its last product with it is known to be done.
+    auto release = [&] {
+      if (q == 0 && lane == 0) mbar_arrive(&kv_empty[ring]);
+      if (++ring == kStages) ring = 0;
+    };
     bool ok = true;
     for (uint32_t k = 0; ok; ++k) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&sched_full[k & 1], (k >> 1) & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag));
       if (!ok) break;
       Item it;
-      it.q_row = items[k & 1].q_row;
-      it.q_count = items[k & 1].q_count;
-      it.k_row = items[k & 1].k_row;
-      it.k_len = items[k & 1].k_len;
-      it.visible = items[k & 1].visible;
-      it.head = items[k & 1].head;
-      it.last = items[k & 1].last;
+      it.q_row = items[k % 3].q_row;
+      it.q_count = items[k % 3].q_count;
+      it.k_row = items[k % 3].k_row;
+      it.k_len = items[k % 3].k_len;
+      it.visible = items[k % 3].visible;
+      it.head = items[k % 3].head;
+      it.last = items[k % 3].last;
       __syncwarp();
       const Reach r = reach_of(it, t, tokens, p.causal);
       const int whole = r.first / kKeys;  // steps that every row of the tile sees in full
@@ -637,28 +740,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after();
+        if (j > 0) release();  // the previous step's V
+        release();             // this step's K
         if (j < whole)
-          softmax_step<kBf16, false>(tl, to, kDim, c, kKeys, j == 0, m, sum, &o_full[t],
-                                     (o_count - 1) & 1u, abort_flag, ok);
+          softmax_step<kBf16, false>(tl, to, kDim, c, kKeys, j == 0, m, sum, &p_full[t]);
         else
-          softmax_step<kBf16, true>(tl, to, kDim, c, sees - j * kKeys, j == 0, m, sum, &o_full[t],
-                                    (o_count - 1) & 1u, abort_flag, ok);
-        if (!ok) break;
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
-        ++o_count;
+          softmax_step<kBf16, true>(tl, to, kDim, c, sees - j * kKeys, j == 0, m, sum, &p_full[t]);
       }
       if (!ok) break;
       if (r.steps > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], (o_count - 1) & 1u, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag));
         if (!ok) break;
+        o_phase ^= 1;
         tc_fence_after();
+        release();
       }
-      const int fix = r.steps > 0 ? items[k & 1].fix : 0;
+      // the issuer releases the stages of steps that only the other tile has
+      ring = (ring + 2 * (max(r.steps, reach_of(it, 1 - t, tokens, p.causal).steps) - r.steps)) % kStages;
+      const int fix = r.steps > 0 ? items[k % 3].fix : 0;
       __syncwarp();
       // From here on the slot is not read again; the next item but one may be written into it.
-      if (lane == 0) mbar_arrive(&sched_empty[k & 1]);
+      if (lane == 0) mbar_arrive(&sched_empty[k % 3]);
       if (it.last) break;
       const bool live = token < tokens && mine < it.q_count;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;

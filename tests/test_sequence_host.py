@@ -1,17 +1,21 @@
 """Argument checks of the packed and paged entry points, which launch nothing and need no GPU."""
 import ctypes
 import os
+import struct
 import subprocess
 
 import pytest
 
 import dinov3_b200 as dv
-from dinov3_b200 import _lib, sequence
+from dinov3_b200 import _lib
 
 from conftest import ROOT
 
 BUF = ctypes.create_string_buffer(4096)
 BASE = (ctypes.addressof(BUF) + 63) & ~63
+
+# The argument structs of dinov3_kernels.h: pointers and 8-byte integers first, then 4-byte ones.
+PACKED_STRUCT, APPEND_STRUCT, PAGED_STRUCT = struct.Struct("8Q8q8IfI"), struct.Struct("12Q11q12I"), struct.Struct("9Q7qQ9If")
 
 PACKED = ["q", "k", "v", "out", "lse", "cu_q", "cu_k", "status", "q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token",
           "out_head", "n_seq", "total_q", "total_k", "q_heads", "kv_heads", "head_dim", "dtype", "causal", "scale", "reserved"]
@@ -55,7 +59,7 @@ HEADS = [("dtype", dict(dtype=2)), ("head_dim", dict(head_dim=80)), ("kv_heads",
     ("aligned", dict(out=BASE + 8)), ("too many", dict(total_q=1 << 31)),
 ])
 def test_packed_refusals(text, changes):
-    refused("dv3k_attention_packed", sequence._PACKED, PACKED, packed_ok, text, **changes)
+    refused("dv3k_attention_packed", PACKED_STRUCT, PACKED, packed_ok, text, **changes)
 
 
 CACHE = [("page_size", dict(page_size=0)), ("page_size", dict(page_size=1 << 17)), ("2^31", dict(max_pages=1 << 30)), ("n_pages", dict(n_pages=1 << 31)),
@@ -69,7 +73,7 @@ CACHE = [("page_size", dict(page_size=0)), ("page_size", dict(page_size=1 << 17)
     ("null", dict(k=0)), ("null", dict(lens=0)), ("null", dict(q_out=0)), ("null", dict(sin=0)), ("aligned", dict(cos=BASE + 4)),
 ])
 def test_append_refusals(text, changes):
-    refused("dv3k_rope_append", sequence._APPEND, APPEND, append_ok, text, **changes)
+    refused("dv3k_rope_append", APPEND_STRUCT, APPEND, append_ok, text, **changes)
 
 
 @pytest.mark.parametrize("text,changes", HEADS + CACHE + [
@@ -77,7 +81,7 @@ def test_append_refusals(text, changes):
     ("null", dict(out=0)), ("null", dict(lens=0)), ("aligned", dict(q=BASE + 8)), ("aligned", dict(workspace=BASE + 8)),
 ])
 def test_paged_refusals(text, changes):
-    refused("dv3k_attention_paged", sequence._PAGED, PAGED, paged_ok, text, **changes)
+    refused("dv3k_attention_paged", PAGED_STRUCT, PAGED, paged_ok, text, **changes)
 
 
 def test_null_arguments_and_nothing_to_do():
@@ -86,14 +90,14 @@ def test_null_arguments_and_nothing_to_do():
         assert getattr(lib, name)(None, None) == dv.INVALID_ARGUMENT and "null" in _lib.last_error()
     assert lib.dv3k_attention_paged_workspace(None) == 0
     for changes in (dict(n_seq=0), dict(total_q=0, q=0, out=0)):
-        assert call("dv3k_attention_packed", sequence._PACKED, PACKED, dict(packed_ok, **changes))[0] == 0
+        assert call("dv3k_attention_packed", PACKED_STRUCT, PACKED, dict(packed_ok, **changes))[0] == 0
     for changes in (dict(n_seq=0), dict(total=0, q=0, k=0)):
-        assert call("dv3k_rope_append", sequence._APPEND, APPEND, dict(append_ok, **changes))[0] == 0
-    assert call("dv3k_attention_paged", sequence._PAGED, PAGED, dict(paged_ok, n_seq=0, q=0))[0] == 0
+        assert call("dv3k_rope_append", APPEND_STRUCT, APPEND, dict(append_ok, **changes))[0] == 0
+    assert call("dv3k_attention_paged", PAGED_STRUCT, PAGED, dict(paged_ok, n_seq=0, q=0))[0] == 0
 
 
-def test_python_packs_the_header_s_structs(tmp_path):
-    """Field order and size of the argument structs, as the C compiler lays them out."""
+def test_structs_match_the_header(tmp_path):
+    """Field order and size of the argument structs used here, as the C compiler lays them out."""
     lines = []
     for struct, fields in (("dv3k_packed_attention", PACKED), ("dv3k_rope_append_args", APPEND), ("dv3k_paged_attention", PAGED)):
         lines += [f'printf("%zu ", offsetof({struct}, {f}));' for f in fields] + [f'printf("%zu\\n", sizeof({struct}));']
@@ -101,7 +105,7 @@ def test_python_packs_the_header_s_structs(tmp_path):
     source.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "dinov3_kernels.h"\nint main(void) {\n' + "\n".join(lines) + "\nreturn 0;\n}\n")
     subprocess.run(["gcc", "-std=c11", "-I" + os.path.join(ROOT, "include"), str(source), "-o", str(tmp_path / "layout")], check=True)
     rows = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.splitlines()
-    for row, pack, fields in zip(rows, (sequence._PACKED, sequence._APPEND, sequence._PAGED), (PACKED, APPEND, PAGED)):
+    for row, pack, fields in zip(rows, (PACKED_STRUCT, APPEND_STRUCT, PAGED_STRUCT), (PACKED, APPEND, PAGED)):
         offsets = [int(x) for x in row.split()]
         assert offsets[-1] == pack.size and len(offsets) == len(fields) + 1
         for i, f in enumerate(fields):
@@ -109,3 +113,14 @@ def test_python_packs_the_header_s_structs(tmp_path):
             values[i] = 1
             at = next(j for j, b in enumerate(pack.pack(*values)) if b)
             assert offsets[i] <= at < offsets[i] + 8 and at < offsets[i + 1], f
+
+
+def test_tensor_binding_is_built_and_refuses_what_is_no_cuda_tensor():
+    torch = pytest.importorskip("torch")
+    q, cu = torch.zeros(4, 4, 64, dtype=torch.float16), torch.tensor([0, 4], dtype=torch.int32)
+    cache, n = torch.zeros(2, 4, 8, 64, dtype=torch.float16), torch.tensor([4], dtype=torch.int32)
+    for call in (lambda: dv.attention_packed(q, q, q, cu), lambda: dv.attention_packed(q, None, q, cu), lambda: dv.rope_append(q, q, q, cache, cache, n[None], n),
+                 lambda: dv.attention_paged(q[:1], cache, cache, n[None], n)):
+        with pytest.raises(dv.DINOv3Error) as e:
+            call()
+        assert e.value.code == dv.INVALID_ARGUMENT and ("CUDA tensor" in str(e.value) or "must be a tensor" in str(e.value))
