@@ -7,18 +7,22 @@
 // `status` and its tokens count as absent.
 //
 // Bound by the one read of K and V: a key costs 4 head_dim bytes and 4 head_dim flops for each of
-// the group's query heads, far below the tensor cores' rate. So the kernel is a stream: a CTA takes
-// one (sequence, key-value head, split of the length), and 64-key tiles of K and V run through a
-// ring of shared-memory stages by 16-byte cp.async (any page size; a tile's row addresses are looked
-// up one tile ahead). Each of the four warps owns 16 keys of a tile and its own running maximum,
-// sum and output, so warps meet only at the ring's barrier: S = Q K^T and O += P V are m16n8k16
-// tensor-core products with the group's up to 16 query heads as M (rows past the group are zero),
-// P stays in registers. Groups of more than 16 heads take one CTA per 16.
-//
-// A sequence is cut into chunks of whole tiles, dealt round-robin to the grid's splits, so that a
-// long sequence fills the GPU and a long one among short ones does not end last. With more than
-// one split each CTA leaves (max, sum, unnormalised output) in the workspace, and a second launch
-// joins them in split order; nothing depends on the order in which CTAs end.
+// the group's query heads, far below the tensor cores' rate. So the kernel is a stream of 64-key
+// tiles of K and V through a ring of shared-memory stages by 16-byte cp.async (any page size; a
+// tile's row addresses are looked up a tile before its loads are issued), and the CTAs (four an SM
+// at 64 channels, two at 128) run on without a break:
+//   - A unit is one (sequence, key-value head); groups of more than 16 query heads make one for
+//     each 16. The tiles of all units stand in one row, and each CTA takes an equal stretch of
+//     it, whatever the lengths: the loads of a stretch's next unit are under way while this one is
+//     finished. A unit that lies in one stretch is written out; of one that does not each CTA
+//     leaves (max, sum, unnormalised output) in the workspace, at most two a CTA, and a second
+//     launch joins them in order. Nothing depends on the order in which CTAs end.
+//   - Where no sequence passes 256 keys, stretches are whole units and there is nothing to join.
+// Within a tile each of the four warps computes the scores of 16 keys for the group's up to 16
+// query heads (m16n8k16 tensor-core products, rows past the group zero), the warps agree on the
+// running maximum in shared memory, and each then multiplies all 64 weights with its quarter of V's
+// channels: no warp's output has to be added to another's at a unit's end, which for short
+// sequences cost more than the keys (26.6 us against NNNN for 256 images of 201 tokens).
 #include <atomic>
 
 #include "sequence.cuh"
@@ -32,15 +36,21 @@ constexpr int kStages = 3;
 constexpr int kRing = 4;      // tiles whose row addresses are kept: kStages + the one being looked up
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+constexpr uint32_t kLeast = 4;  // tiles that a CTA takes at least
+
+// Stages | row addresses | weights of a tile [16][64], 128-byte rows
 template <int kDim>
 constexpr int smem_bytes() {
-  return kStages * 2 * kTile * kDim * 2 + kRing * kTile * 2 * 8;
+  return kStages * 2 * kTile * kDim * 2 + kRing * kTile * 2 * 8 + 16 * kTile * 2;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(valid ? 16 : 0)
                : "memory");
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -75,33 +85,52 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// How the lengths are cut: chunks of `chunk` tiles dealt round-robin to `splits` CTAs.
-struct Split {
-  uint32_t splits, chunk, head_blocks;
+// The grid, and how it cuts the work.
+struct Plan {
+  uint32_t grid, head_blocks, rows;  // rows: query heads of a unit at most
+  bool units;                        // stretches are whole units
 };
 
-// A chunk is 4 tiles (256 keys) to 16, so that the grid has about four waves of CTAs: less than
-// four leave a ragged tail, and chunks under 256 keys spend more on their start than on the
-// stream. The splits are capped so that the partial results stay small beside the cache, whatever
-// bound of the lengths the caller gave: beyond 32 waves the chunks go round.
-Split split_of(const PagedAttention &p) {
+Plan plan_of(const PagedAttention &p) {
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t slots = static_cast<uint64_t>(sm_count(dev)) * (p.head_dim == 64 ? 4 : 2);
   const uint32_t group = p.q_heads / p.kv_heads;
-  Split s;
+  Plan s;
   s.head_blocks = p.kv_heads * ((group + 15) / 16);
+  s.rows = group < 16 ? group : 16;
   const uint64_t units = static_cast<uint64_t>(p.n_seq) * s.head_blocks;
-  const uint64_t tiles = p.max_len > 0 ? (static_cast<uint64_t>(p.max_len) + kTile - 1) / kTile : 1;
-  uint64_t chunk = (tiles * units + 4 * slots - 1) / (4 * slots);
-  chunk = chunk < 4 ? 4 : chunk > 16 ? 16 : chunk;
-  uint64_t splits = (tiles + chunk - 1) / chunk;
-  const uint64_t most = (32 * slots + units - 1) / units;
-  if (splits > most) splits = most;
-  if (splits > 1024) splits = 1024;
-  s.splits = static_cast<uint32_t>(splits);
-  s.chunk = static_cast<uint32_t>(chunk);
+  const uint64_t tiles = (static_cast<uint64_t>(p.max_len) + kTile - 1) / kTile;
+  s.units = tiles <= kLeast;
+  // as many CTAs as run at once, but none for less than a unit or kLeast tiles
+  const uint64_t most = s.units ? units : units * ((tiles + kLeast - 1) / kLeast);
+  s.grid = static_cast<uint32_t>(most < slots ? most : slots);
   return s;
+}
+
+// Workspace: the first tile of each sequence in the row of all tiles [n_seq + 1] (u64, written by
+// CTA 0), then (max, sum) and the output of [grid][2][rows] partial results.
+__host__ __device__ inline size_t starts_bytes(uint32_t n_seq) {
+  return ((static_cast<size_t>(n_seq) + 1) * 8 + 15) / 16 * 16;
+}
+struct Partials {
+  uint64_t *starts;
+  float2 *ml;
+  float *o;
+};
+__device__ __forceinline__ Partials partials_of(const PagedAttention &p, const Plan &pl) {
+  Partials w;
+  uint8_t *at = static_cast<uint8_t *>(p.workspace);
+  w.starts = reinterpret_cast<uint64_t *>(at);
+  w.ml = reinterpret_cast<float2 *>(at + starts_bytes(p.n_seq));
+  const size_t n = (static_cast<size_t>(pl.grid) * 2 * pl.rows + 1) / 2 * 2;
+  w.o = reinterpret_cast<float *>(w.ml + n);
+  return w;
+}
+// Tiles of a stretch.
+__device__ __forceinline__ uint64_t stretch_of(uint64_t total, uint32_t grid) {
+  const uint64_t n = (total + grid - 1) / grid;
+  return n < kLeast ? kLeast : n;
 }
 
 // Tokens of sequence s that the page table has room for.
@@ -118,56 +147,137 @@ __device__ __forceinline__ uint32_t cached_tokens(const PagedAttention &p, uint3
 }  // namespace
 
 template <bool kBf16, int kDim>
-__global__ void __launch_bounds__(kThreads)
-    attention_paged_kernel(const PagedAttention p, const Split sp) {
+__global__ void __launch_bounds__(kThreads, kDim == 64 ? 4 : 2)
+    attention_paged_kernel(const PagedAttention p, const Plan pl) {
   constexpr int kChunks = kDim / 8;            // 16-byte chunks of a row
   constexpr int kRowsPass = kThreads / kChunks;
   constexpr int kTileBytes = kTile * kDim * 2;  // of K or of V
   constexpr int kSteps = kDim / 16;
+  constexpr int kCols = kDim / 4 / 16;  // 16-channel columns of a warp's quarter
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float tops[4][16], sums[4][16];
+  __shared__ uint64_t found[2][3];  // the stretch's two ends: sequence, head block, tile
+  __shared__ uint64_t scan[4];
   int64_t(*rows)[kTile][2] = reinterpret_cast<int64_t(*)[kTile][2]>(smem + kStages * 2 * kTileBytes);
-  const uint32_t smem0 = smem_u32(smem);
+  const uint32_t smem0 = smem_u32(smem), w_at = smem0 + kStages * 2 * kTileBytes + kRing * kTile * 16;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t group = p.q_heads / p.kv_heads, blocks = pl.head_blocks / p.kv_heads;
+  auto tiles_of = [&](uint32_t s) { return (cached_tokens(p, s, false) + kTile - 1) / kTile; };
 
-  const uint32_t split = blockIdx.x % sp.splits;
-  const uint32_t hb = blockIdx.x / sp.splits % sp.head_blocks;
-  const uint32_t s = blockIdx.x / sp.splits / sp.head_blocks;
-  const uint32_t group = p.q_heads / p.kv_heads, blocks = sp.head_blocks / p.kv_heads;
-  const uint32_t g = hb / blocks, h0 = g * group + hb % blocks * 16;
-  const uint32_t heads = min(16u, (g + 1) * group - h0);
+  // The stretch of this CTA: from (s, hb, t) up to but without (end_s, end_hb, end_t).
+  uint64_t per = 0;  // tiles of a stretch
+  if (pl.units) {
+    const uint64_t n = static_cast<uint64_t>(p.n_seq) * pl.head_blocks;
+    if (tid < 2) {
+      const uint64_t u = n * (blockIdx.x + tid) / pl.grid;
+      found[tid][0] = u / pl.head_blocks;
+      found[tid][1] = u % pl.head_blocks;
+      found[tid][2] = 0;
+    }
+  } else {
+    const uint32_t each = (p.n_seq + kThreads - 1) / kThreads;
+    const uint32_t from = min(tid * each, p.n_seq), to = min(from + each, p.n_seq);
+    uint64_t mine = 0;
+    for (uint32_t s = from; s < to; ++s) mine += tiles_of(s);
+    mine *= pl.head_blocks;
+    uint64_t sum = mine;
+#pragma unroll
+    for (int i = 1; i < 32; i *= 2) {
+      const uint64_t x = __shfl_up_sync(0xffffffffu, sum, i);
+      if (lane >= static_cast<uint32_t>(i)) sum += x;
+    }
+    if (lane == 31) scan[warp] = sum;
+    __syncthreads();
+    uint64_t total = 0, before = sum - mine;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    per = stretch_of(total, pl.grid);
+    const uint64_t first = per * blockIdx.x, beyond = first + per;
+    const uint64_t ends[2] = {first < total ? first : total, beyond < total ? beyond : total};
+    if (tid < 2 && ends[tid] == total) {
+      found[tid][0] = p.n_seq;
+      found[tid][1] = found[tid][2] = 0;
+    }
+    uint64_t *starts = static_cast<uint64_t *>(p.workspace);
+    uint64_t at = before;
+    for (uint32_t s = from; s < to; ++s) {
+      if (blockIdx.x == 0) starts[s] = at;
+      const uint64_t n = tiles_of(s), next = at + n * pl.head_blocks;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (ends[e] >= at && ends[e] < next) {
+          found[e][0] = s;
+          found[e][1] = (ends[e] - at) / n;
+          found[e][2] = (ends[e] - at) % n;
+        }
+      at = next;
+    }
+    if (blockIdx.x == 0 && tid == 0) starts[p.n_seq] = total;
+  }
+  __syncthreads();
+  const uint32_t end_s = static_cast<uint32_t>(found[1][0]), end_hb = static_cast<uint32_t>(found[1][1]),
+                 end_t = static_cast<uint32_t>(found[1][2]);
 
-  const uint32_t len = cached_tokens(p, s, tid == 0 && split == 0 && hb == 0);
-  const uint32_t tiles = (len + kTile - 1) / kTile;
-  const uint32_t n_chunks = (tiles + sp.chunk - 1) / sp.chunk;
-  if (split >= n_chunks && !(split == 0 && sp.splits == 1)) return;
-  // This CTA's tiles: chunks split, split + splits, ...; the last chunk of the sequence may be short.
-  const uint32_t mine = split < n_chunks ? (n_chunks - 1 - split) / sp.splits + 1 : 0;
-  uint32_t count = mine * sp.chunk;
-  if (mine > 0 && (n_chunks - 1) % sp.splits == split) count -= n_chunks * sp.chunk - tiles;
-  auto tile_at = [&](uint32_t i) {
-    return (split + i / sp.chunk * sp.splits) * sp.chunk + i % sp.chunk;
+  // A place in the row of tiles; the loads run ahead of the products with a place of their own.
+  struct Place {
+    uint32_t s, hb, t, len, tiles, end;  // end: tiles of this unit up to the stretch's end
   };
+  auto enter = [&](Place &x) {  // the unit at (s, hb); its end, 0 past the stretch
+    x.end = 0;
+    if (x.s >= p.n_seq || (x.s == end_s && x.hb > end_hb) || x.s > end_s) return;
+    x.len = cached_tokens(p, x.s, false);
+    x.tiles = (x.len + kTile - 1) / kTile;
+    x.end = x.s == end_s && x.hb == end_hb ? end_t : x.tiles;
+  };
+  auto past = [&](const Place &x) {  // the unit is not of the stretch any more
+    return x.s >= p.n_seq || x.s > end_s || (x.s == end_s && (x.hb > end_hb || (x.hb == end_hb && end_t == 0)));
+  };
+  auto next_unit = [&](Place &x) {
+    x.t = 0;
+    if (++x.hb == pl.head_blocks) {
+      x.hb = 0;
+      ++x.s;
+    }
+    enter(x);
+  };
+  Place ld = {static_cast<uint32_t>(found[0][0]), static_cast<uint32_t>(found[0][1]),
+              static_cast<uint32_t>(found[0][2]), 0, 0, 0};
+  enter(ld);
+  Place at = ld;
+  auto settle = [&] {  // to the next tile there is
+    while (ld.t >= ld.end && !past(ld)) next_unit(ld);
+  };
+  settle();
 
-  // The element offset of each row of a tile in the two caches, -1 where there is none.
-  const int32_t *table = p.page_table + static_cast<int64_t>(s) * p.table_stride;
-  auto look_up = [&](uint32_t i, uint32_t r, int64_t &k_at, int64_t &v_at) {
+  // The element offsets of row r of the tile at `ld` in the two caches, -1 where there is none.
+  auto look_up = [&](uint32_t r, int64_t &k_at, int64_t &v_at) {
     k_at = v_at = -1;
-    if (i >= count) return;
-    const uint32_t j = tile_at(i) * kTile + r;
-    if (j >= len) return;
+    if (ld.t >= ld.end) return;
+    const uint32_t j = ld.t * kTile + r;
+    if (j >= ld.len) return;
     const uint32_t page = page_of(p.page, j);
-    const int32_t id = __ldg(table + page);
+    const int32_t id = __ldg(p.page_table + static_cast<int64_t>(ld.s) * p.table_stride + page);
     if (id < 0 || static_cast<uint32_t>(id) >= p.n_pages) {
       report(p.status, kErrPage);
       return;
     }
-    const int64_t row = (static_cast<int64_t>(g) * p.page.size + (j - page * p.page.size)) * kDim;
+    const int64_t row = (static_cast<int64_t>(ld.hb / blocks) * p.page.size + (j - page * p.page.size)) * kDim;
     k_at = id * p.k_page + row;
     v_at = id * p.v_page + row;
   };
+  uint32_t known = 0;  // tiles looked up
+  auto advance = [&] {
+    if (ld.t >= ld.end) return;
+    ++known;
+    ++ld.t;
+    settle();
+  };
   const uint32_t c = tid % kChunks, r0 = tid / kChunks;
   auto load_tile = [&](uint32_t i) {
-    if (i < count) {
+    if (i < known) {
       const uint32_t kb = smem0 + i % kStages * 2 * kTileBytes;
 #pragma unroll
       for (int r = r0, n = 0; n < kTile / kRowsPass; ++n, r += kRowsPass) {
@@ -180,214 +290,219 @@ __global__ void __launch_bounds__(kThreads)
     cp_async_commit();
   };
 
-  for (uint32_t x = tid; x < kStages * kTile; x += kThreads) {
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) {
     int64_t k_at, v_at;
-    look_up(x / kTile, x % kTile, k_at, v_at);
-    rows[x / kTile][x % kTile][0] = k_at;
-    rows[x / kTile][x % kTile][1] = v_at;
+    if (tid < kTile) {
+      look_up(tid, k_at, v_at);
+      rows[i][tid][0] = k_at;
+      rows[i][tid][1] = v_at;
+    }
+    advance();
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load_tile(i);
 
-  // Q as the products' A operand: rows lane / 4 and lane / 4 + 8, columns 2 (lane % 4) of each half
-  const uint32_t ra = lane / 4, cq = 2 * (lane % 4);
-  uint32_t q[kSteps][4];
-  {
-    const uint16_t *qa = p.q + static_cast<int64_t>(s) * p.q_seq + static_cast<int64_t>(h0 + ra) * p.q_head + cq;
-    const uint16_t *qb = qa + 8 * p.q_head;
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      q[k][0] = ra < heads ? *reinterpret_cast<const uint32_t *>(qa + 16 * k) : 0u;
-      q[k][1] = ra + 8 < heads ? *reinterpret_cast<const uint32_t *>(qb + 16 * k) : 0u;
-      q[k][2] = ra < heads ? *reinterpret_cast<const uint32_t *>(qa + 16 * k + 8) : 0u;
-      q[k][3] = ra + 8 < heads ? *reinterpret_cast<const uint32_t *>(qb + 16 * k + 8) : 0u;
-    }
-  }
-  float o[kDim / 8][4];
-#pragma unroll
-  for (int n = 0; n < kDim / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const uint32_t ra = lane / 4, cq = 2 * (lane % 4), key0 = warp * 16;
   const float c2 = p.scale * kLog2e;
+  uint32_t i = 0;  // tiles done
+  while (!past(at)) {
+    const uint32_t g = at.hb / blocks, h0 = g * group + at.hb % blocks * 16;
+    const uint32_t heads = min(16u, (g + 1) * group - h0);
+    const bool whole = at.t == 0 && at.end == at.tiles;
+    const uint32_t slot = i == 0 ? 0 : 1;  // the stretch's first unit, or its last
+    if (tid == 0 && at.hb == 0) cached_tokens(p, at.s, true);  // tells of a length past the table
+    if (at.t >= at.end) __syncthreads();                       // `sums` may still be read
 
-  const uint32_t key0 = warp * 16;
-  for (uint32_t i = 0; i < count; ++i) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();  // tile i is in; tile i - 1's stage and the oldest addresses are free
-    load_tile(i + kStages - 1);
-    int64_t k_at, v_at;
-    if (tid < kTile) look_up(i + kStages, tid, k_at, v_at);
-
-    const uint32_t kb = smem0 + i % kStages * 2 * kTileBytes, vb = kb + kTileBytes;
-    float sc[2][4];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+    // Q as the products' A operand: rows lane / 4 and lane / 4 + 8, columns 2 (lane % 4) of each half
+    uint32_t q[kSteps][4];
     {
-      // four 8x8 matrices: keys 0-7 and 8-15 of the warp, both halves of 16 channels
-      const uint32_t r = key0 + (lane / 16) * 8 + lane % 8;
+      const uint16_t *qa = p.q + static_cast<int64_t>(at.s) * p.q_seq + static_cast<int64_t>(h0 + ra) * p.q_head + cq;
+      const uint16_t *qb = qa + 8 * p.q_head;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        uint32_t b[4];
-        ldsm4(kb + r * kDim * 2 + (((2 * k + (lane / 8 & 1)) ^ (r & 7)) * 16), b);
-        mma16816<kBf16>(sc[0], q[k], b[0], b[1]);
-        mma16816<kBf16>(sc[1], q[k], b[2], b[3]);
+        q[k][0] = ra < heads ? *reinterpret_cast<const uint32_t *>(qa + 16 * k) : 0u;
+        q[k][1] = ra + 8 < heads ? *reinterpret_cast<const uint32_t *>(qb + 16 * k) : 0u;
+        q[k][2] = ra < heads ? *reinterpret_cast<const uint32_t *>(qa + 16 * k + 8) : 0u;
+        q[k][3] = ra + 8 < heads ? *reinterpret_cast<const uint32_t *>(qb + 16 * k + 8) : 0u;
       }
     }
+    float o[2 * kCols][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int64_t *at = rows[i % kRing][key0 + n * 8 + cq];
-      if (at[0] < 0) sc[n][0] = sc[n][2] = -INFINITY;
-      if (at[2] < 0) sc[n][1] = sc[n][3] = -INFINITY;
-    }
-    uint32_t pa[4];
-    float keep[2];
-    bool moved = false;
+    for (int n = 0; n < 2 * kCols; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (; at.t < at.end; ++at.t, ++i) {
+      cp_async_wait<kStages - 2>();
+      __syncthreads();  // tile i is in; tile i - 1's stage, weights and the oldest addresses are free
+      load_tile(i + kStages - 1);
+      int64_t k_at, v_at;
+      if (tid < kTile) look_up(tid, k_at, v_at);
+      advance();
+
+      const uint32_t kb = smem0 + i % kStages * 2 * kTileBytes, vb = kb + kTileBytes;
+      float sc[2][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float top = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top, m[h]);
-      const float base = top == -INFINITY ? 0.f : top * c2;
-      keep[h] = ex2_approx(m[h] * c2 - base);
-      moved |= top != m[h];
-      m[h] = top;
-      const float p0 = ex2_approx(fmaf(sc[0][2 * h], c2, -base)), p1 = ex2_approx(fmaf(sc[0][2 * h + 1], c2, -base));
-      const float p2 = ex2_approx(fmaf(sc[1][2 * h], c2, -base)), p3 = ex2_approx(fmaf(sc[1][2 * h + 1], c2, -base));
-      l[h] = fmaf(l[h], keep[h], (p0 + p1) + (p2 + p3));
-      pa[h] = Elem<kBf16>::pack(p0, p1);
-      pa[2 + h] = Elem<kBf16>::pack(p2, p3);
-    }
-    if (__any_sync(0xffffffffu, moved)) {
+      for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      {
+        // four 8x8 matrices: keys 0-7 and 8-15 of the warp, both halves of 16 channels
+        const uint32_t r = key0 + (lane / 16) * 8 + lane % 8;
 #pragma unroll
-      for (int n = 0; n < kDim / 8; ++n) {
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t b[4];
+          ldsm4(kb + r * kDim * 2 + (((2 * k + (lane / 8 & 1)) ^ (r & 7)) * 16), b);
+          mma16816<kBf16>(sc[0], q[k], b[0], b[1]);
+          mma16816<kBf16>(sc[1], q[k], b[2], b[3]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int64_t *row = rows[i % kRing][key0 + n * 8 + cq];
+        if (row[0] < 0) sc[n][0] = sc[n][2] = -INFINITY;
+        if (row[2] < 0) sc[n][1] = sc[n][3] = -INFINITY;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (lane % 4 == 0) tops[warp][ra + 8 * h] = top;
+      }
+      __syncthreads();
+      float keep[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t r = ra + 8 * h;
+        const float top = fmaxf(m[h], fmaxf(fmaxf(tops[0][r], tops[1][r]), fmaxf(tops[2][r], tops[3][r])));
+        const float base = top == -INFINITY ? 0.f : top * c2;
+        keep[h] = ex2_approx(fmaf(m[h], c2, -base));
+        m[h] = top;
+        const float p0 = ex2_approx(fmaf(sc[0][2 * h], c2, -base)), p1 = ex2_approx(fmaf(sc[0][2 * h + 1], c2, -base));
+        const float p2 = ex2_approx(fmaf(sc[1][2 * h], c2, -base)), p3 = ex2_approx(fmaf(sc[1][2 * h + 1], c2, -base));
+        l[h] = fmaf(l[h], keep[h], (p0 + p1) + (p2 + p3));
+        const uint32_t row = w_at + r * (kTile * 2) + (cq * 2);
+        sts32(row + (((2 * warp) ^ (r & 7)) * 16), Elem<kBf16>::pack(p0, p1));
+        sts32(row + (((2 * warp + 1) ^ (r & 7)) * 16), Elem<kBf16>::pack(p2, p3));
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 2 * kCols; ++n) {
         o[n][0] *= keep[0];
         o[n][1] *= keep[0];
         o[n][2] *= keep[1];
         o[n][3] *= keep[1];
       }
-    }
-    {
-      // keys 0-7 and 8-15 of the warp, two 8-channel columns
-      const uint32_t r = key0 + lane % 16;
+      {
+        const uint32_t r = lane % 16;
 #pragma unroll
-      for (int n = 0; n < kDim / 16; ++n) {
-        uint32_t b[4];
-        ldsm4t(vb + r * kDim * 2 + (((2 * n + lane / 16) ^ (r & 7)) * 16), b);
-        mma16816<kBf16>(o[2 * n], pa, b[0], b[1]);
-        mma16816<kBf16>(o[2 * n + 1], pa, b[2], b[3]);
+        for (int k = 0; k < kTile / 16; ++k) {
+          uint32_t w[4];
+          ldsm4(w_at + r * (kTile * 2) + (((2 * k + lane / 16) ^ (r & 7)) * 16), w);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) {
+            // keys 0-7 and 8-15 of the step, two 8-channel columns
+            uint32_t b[4];
+            ldsm4t(vb + (k * 16 + r) * kDim * 2 + (((warp * (kDim / 32) + 2 * n + lane / 16) ^ (r & 7)) * 16), b);
+            mma16816<kBf16>(o[2 * n], w, b[0], b[1]);
+            mma16816<kBf16>(o[2 * n + 1], w, b[2], b[3]);
+          }
+        }
+      }
+      if (tid < kTile) {
+        rows[(i + kStages) % kRing][tid][0] = k_at;
+        rows[(i + kStages) % kRing][tid][1] = v_at;
       }
     }
-    if (tid < kTile) {
-      rows[(i + kStages) % kRing][tid][0] = k_at;
-      rows[(i + kStages) % kRing][tid][1] = v_at;
+
+    // The unit's end: the row sums of the four warps, then this warp's quarter of the channels.
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (lane % 4 == 0) sums[warp][ra + 8 * h] = l[h];
     }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t r = ra + 8 * h;
+      if (r >= heads) continue;
+      const float sum = (sums[0][r] + sums[1][r]) + (sums[2][r] + sums[3][r]);
+      const uint32_t col = warp * (kDim / 4) + cq;
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint16_t *dst = p.out + static_cast<int64_t>(at.s) * p.out_seq + (h0 + r) * p.out_head + col;
+#pragma unroll
+        for (int n = 0; n < 2 * kCols; ++n)
+          *reinterpret_cast<uint32_t *>(dst + 8 * n) = Elem<kBf16>::pack(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+        if (p.lse && col == 0)
+          p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = (m[h] * c2 + log2f(sum)) * kLn2;
+      } else {
+        const Partials w = partials_of(p, pl);
+        const size_t row = (static_cast<size_t>(blockIdx.x) * 2 + slot) * pl.rows + r;
+#pragma unroll
+        for (int n = 0; n < 2 * kCols; ++n)
+          *reinterpret_cast<float2 *>(w.o + row * kDim + col + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if (col == 0) w.ml[row] = make_float2(m[h] * c2, sum);
+      }
+    }
+    next_unit(at);
   }
   pdl_trigger();
-
-  // Join the four warps: their maxima and sums, then the outputs scaled to the common maximum.
   cp_async_wait<0>();
-  __syncthreads();
-  float *wo = reinterpret_cast<float *>(smem);                      // [4][16][kDim]
-  float(*wml)[16][2] = reinterpret_cast<float(*)[16][2]>(rows);     // [4][16] (max, sum)
-  static_assert(4 * 16 * kDim * 4 <= kStages * 2 * kTileBytes && 4 * 16 * 2 * 4 <= kRing * kTile * 16, "reuse");
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (lane % 4 == 0) {
-      wml[warp][ra + 8 * h][0] = m[h];
-      wml[warp][ra + 8 * h][1] = l[h];
-    }
-#pragma unroll
-    for (int n = 0; n < kDim / 8; ++n)
-      *reinterpret_cast<float2 *>(wo + (warp * 16 + ra + 8 * h) * kDim + n * 8 + cq) =
-          make_float2(o[n][2 * h], o[n][2 * h + 1]);
-  }
-  __syncthreads();
-  constexpr int kQuads = kDim / 4;
-  for (uint32_t x = tid; x < heads * kQuads; x += kThreads) {
-    const uint32_t h = x / kQuads, d = x % kQuads * 4;
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, wml[w][h][0]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = top == -INFINITY ? 1.f : ex2_approx((wml[w][h][0] - top) * c2);
-      const float4 v = *reinterpret_cast<const float4 *>(wo + (w * 16 + h) * kDim + d);
-      sum = fmaf(wml[w][h][1], f, sum);
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
-    }
-    const int64_t row = static_cast<int64_t>(s) * p.q_heads + h0 + h;
-    if (sp.splits == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint2 *>(p.out + static_cast<int64_t>(s) * p.out_seq + (h0 + h) * p.out_head + d) =
-          make_uint2(Elem<kBf16>::pack(acc.x * inv, acc.y * inv), Elem<kBf16>::pack(acc.z * inv, acc.w * inv));
-      if (p.lse && d == 0) p.lse[row] = (top * c2 + log2f(sum)) * kLn2;
-    } else {
-      const int64_t rows_total = static_cast<int64_t>(p.n_seq) * p.q_heads;
-      float *part = static_cast<float *>(p.workspace);
-      *reinterpret_cast<float4 *>(part + (row * sp.splits + split) * kDim + d) = acc;
-      if (d == 0)
-        reinterpret_cast<float2 *>(part + rows_total * sp.splits * kDim)[row * sp.splits + split] =
-            make_float2(top * c2, sum);
-    }
-  }
 }
 
-// Joins the splits of one (sequence, query head): out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-// Eight warps take every eighth split, then meet in shared memory, always in the same order.
+// Joins the units that several stretches share, a CTA for each (sequence, query head):
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the CTAs i in order; and writes the rows
+// of empty sequences. Four warps take every fourth, then meet in shared memory.
 template <bool kBf16, int kDim>
-__global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedAttention p, const Split sp) {
-  constexpr int kWarps = 8;
+__global__ void __launch_bounds__(128) attention_paged_join_kernel(const PagedAttention p, const Plan pl) {
   constexpr int kLane = kDim / 32;  // channels per lane
-  __shared__ float po[kWarps][kDim];
-  __shared__ float2 pml[kWarps];
+  __shared__ float po[4][kDim];
+  __shared__ float pl4[4];
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t row = blockIdx.x;
   const uint32_t s = blockIdx.x / p.q_heads, h = blockIdx.x % p.q_heads;
+  const uint32_t group = p.q_heads / p.kv_heads, blocks = pl.head_blocks / p.kv_heads;
+  const uint32_t hb = h / group * blocks + h % group / 16, r = h % group % 16;
   pdl_wait();
-  const uint32_t tiles = (cached_tokens(p, s, false) + kTile - 1) / kTile;
-  const uint32_t n = min((tiles + sp.chunk - 1) / sp.chunk, sp.splits);  // splits that wrote
-  const float *part = static_cast<const float *>(p.workspace) + row * sp.splits * kDim;
-  const float2 *ml = reinterpret_cast<const float2 *>(
-                         static_cast<const float *>(p.workspace) +
-                         static_cast<int64_t>(p.n_seq) * p.q_heads * sp.splits * kDim) + row * sp.splits;
+  const Partials w = partials_of(p, pl);
+  const uint64_t per = stretch_of(w.starts[p.n_seq], pl.grid);
+  const uint64_t tiles = (w.starts[s + 1] - w.starts[s]) / pl.head_blocks;
+  const uint64_t from = w.starts[s] + hb * tiles, to = from + tiles;
+  const uint32_t c0 = static_cast<uint32_t>(from / per);
+  const uint32_t n = tiles ? static_cast<uint32_t>((to - 1) / per) - c0 + 1 : 0;
+  if (n == 1) return;  // one CTA's: written
+  auto slot_of = [&](uint32_t i) {  // the unit is the first of that CTA's stretch, or its last
+    return (static_cast<size_t>(c0 + i) * 2 + (per * (c0 + i) >= from ? 0 : 1)) * pl.rows + r;
+  };
   float top = -INFINITY;
-  for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, ml[i].x);
+  for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, w.ml[slot_of(i)].x);
 #pragma unroll
   for (int i = 16; i > 0; i /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
   float sum = 0.f, acc[kLane] = {};
 #pragma unroll 4
-  for (uint32_t i = warp; i < n; i += kWarps) {
-    const float2 x = ml[i];
+  for (uint32_t i = warp; i < n; i += 4) {
+    const size_t at = slot_of(i);
+    const float2 x = w.ml[at];
     const float f = top == -INFINITY ? 1.f : ex2_approx(x.x - top);
     sum = fmaf(x.y, f, sum);
 #pragma unroll
     for (int e = 0; e < kLane; e += 2) {
-      const float2 v = *reinterpret_cast<const float2 *>(part + static_cast<int64_t>(i) * kDim + lane * kLane + e);
+      const float2 v = *reinterpret_cast<const float2 *>(w.o + at * kDim + lane * kLane + e);
       acc[e] = fmaf(v.x, f, acc[e]);
       acc[e + 1] = fmaf(v.y, f, acc[e + 1]);
     }
   }
 #pragma unroll
   for (int e = 0; e < kLane; ++e) po[warp][lane * kLane + e] = acc[e];
-  if (lane == 0) pml[warp] = make_float2(top, sum);
+  if (lane == 0) pl4[warp] = sum;
   __syncthreads();
   if (threadIdx.x < kDim / 2) {
     const uint32_t d = threadIdx.x * 2;
-    float a = 0.f, b = 0.f;
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      a += po[w][d];
-      b += po[w][d + 1];
-      sum += pml[w].y;
-    }
+    sum = (pl4[0] + pl4[1]) + (pl4[2] + pl4[3]);
+    const float a = (po[0][d] + po[1][d]) + (po[2][d] + po[3][d]);
+    const float b = (po[0][d + 1] + po[1][d + 1]) + (po[2][d + 1] + po[3][d + 1]);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     *reinterpret_cast<uint32_t *>(p.out + static_cast<int64_t>(s) * p.out_seq + h * p.out_head + d) =
         Elem<kBf16>::pack(a * inv, b * inv);
@@ -396,9 +511,10 @@ __global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedAt
 }
 
 size_t attention_paged_workspace(const PagedAttention &p) {
-  const Split s = split_of(p);
-  if (s.splits <= 1) return 0;
-  return static_cast<size_t>(p.n_seq) * p.q_heads * s.splits * (p.head_dim + 2) * sizeof(float);
+  const Plan pl = plan_of(p);
+  if (pl.units) return 0;
+  const size_t n = (static_cast<size_t>(pl.grid) * 2 * pl.rows + 1) / 2 * 2;
+  return starts_bytes(p.n_seq) + n * (p.head_dim + 2) * sizeof(float);
 }
 
 namespace {
@@ -415,16 +531,14 @@ cudaError_t launch(const PagedAttention &p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
-  const Split s = split_of(p);
-  const uint64_t grid = static_cast<uint64_t>(p.n_seq) * s.head_blocks * s.splits;
+  const Plan pl = plan_of(p);
   const uint64_t join = static_cast<uint64_t>(p.n_seq) * p.q_heads;
-  if (grid > 0x7fffffffull || join > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  attention_paged_kernel<kBf16, kDim>
-      <<<dim3(static_cast<uint32_t>(grid)), dim3(kThreads), smem_bytes<kDim>(), stream>>>(p, s);
+  if (join > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+  attention_paged_kernel<kBf16, kDim><<<dim3(pl.grid), dim3(kThreads), smem_bytes<kDim>(), stream>>>(p, pl);
   const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || s.splits == 1) return e;
+  if (e != cudaSuccess || pl.units) return e;
   return launch_pdl(attention_paged_join_kernel<kBf16, kDim>, dim3(static_cast<uint32_t>(join)),
-                    dim3(256), 0, stream, p, s);
+                    dim3(128), 0, stream, p, pl);
 }
 }  // namespace
 
