@@ -207,15 +207,17 @@ struct PackedAttention {
 cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,
                                     std::string *err);
 
-// A page size and its shift (32 where it is no power of two).
+// A page size, and its division of a position below 2^31 as a product: with s = ceil(log2 size) and
+// magic = ceil(2^(31 + s) / size), magic size - 2^(31 + s) < size <= 2^s, so the quotient of
+// position magic by 2^(31 + s) is exact.
 struct PageDiv {
-  uint32_t size, shift;
+  uint32_t size, magic, shift;  // shift = 31 + s
 };
 inline PageDiv page_div(uint32_t size) {
-  PageDiv d{size, 32};
-  for (uint32_t s = 0; s < 32; ++s)
-    if (size == 1u << s) d.shift = s;
-  return d;
+  uint32_t s = 0;
+  while ((uint64_t{1} << s) < size) ++s;
+  const uint64_t power = uint64_t{1} << (31 + s);
+  return {size, static_cast<uint32_t>((power + size - 1) / size), 31 + s};
 }
 
 struct RopeAppend {

@@ -61,9 +61,9 @@ __device__ __forceinline__ int warp_find_sequence(const int32_t *cu, uint32_t n,
   }
 }
 
-// The page that holds position pos: a shift where the page size is a power of two.
+// The page that holds position pos < 2^31.
 __device__ __forceinline__ uint32_t page_of(PageDiv d, uint32_t pos) {
-  return d.shift < 32 ? pos >> d.shift : pos / d.size;
+  return static_cast<uint32_t>(static_cast<uint64_t>(pos) * d.magic >> d.shift);
 }
 
 }  // namespace dv3

@@ -419,7 +419,7 @@ def test_paged_capture_streams_and_workspace():
     torch.cuda.synchronize()
     for h in held:
         check_paged(q, k, v, table, [2999, 1, 64], h, None, 128 ** -0.5)
-    given = dv.attention_paged(q, k, v, table, n, workspace=torch.full((1 << 22,), 255, dtype=torch.uint8, device=DEV))
+    given = dv.attention_paged(q, k, v, table, n, workspace=torch.full((1 << 24,), 255, dtype=torch.uint8, device=DEV))
     assert torch.equal(given, held[0])
     assert dv.attention_paged(q[:0], k, v, table[:0], n[:0]).shape == (0, 8, 128)
 
