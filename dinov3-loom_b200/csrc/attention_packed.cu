@@ -19,8 +19,9 @@
 //              the element type) back to TMEM over the consumed scores. The reference m only moves
 //              when the maximum has grown by more than 2^8 over it: any m gives the same quotient,
 //              and sums and weights up to 2^8 too large lose nothing in f32, f16 or bf16; the row's
-//              output is then rescaled in TMEM. At an item's end O / sum is written, 32 bytes a
-//              store.
+//              output is then rescaled in TMEM. At an item's end O / sum goes through a staging
+//              tile to global memory. Of a last, partly visible step only the blocks of 32 keys
+//              that some row sees are computed.
 //   warp 8     TMA producer: Q tiles, then K and V tiles in turn through one ring of stages.
 //   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = N = 128), and O_t += P_t V with P
 //              from TMEM and V as the MN-major B operand, one tile at a time.
@@ -45,14 +46,14 @@ constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;  // TMEM allocator; issues tile 0's MMAs, warp 10 tile 1's
 constexpr int kGuardWarp = 11;
 constexpr int kKeys = 128;      // keys per step
-constexpr int kBuckets = 128;   // of the scheduler's order
+constexpr int kBuckets = 64;    // of the scheduler's order
 constexpr int kTmemCols = 512;
 constexpr int kTmemO = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;   // log2 units by which a row's maximum may pass its reference
 
-// One work item as the scheduler publishes it.
-struct Item {
+// One work item as the scheduler publishes it (two 16-byte words).
+struct __align__(16) Item {
   int32_t q_row;    // first query row
   int32_t q_count;  // its tokens (0: nothing to do)
   int32_t k_row;    // first key row of the sequence
@@ -63,22 +64,37 @@ struct Item {
   int32_t fix;      // set by the guard: V held something that is not finite
 };
 
+__device__ __forceinline__ Item read_item(const Item *slot) {
+  Item it;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(it.q_row), "=r"(it.q_count), "=r"(it.k_row), "=r"(it.k_len)
+               : "r"(smem_u32(slot))
+               : "memory");
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(it.visible), "=r"(it.head), "=r"(it.last), "=r"(it.fix)
+               : "r"(smem_u32(slot) + 16)
+               : "memory");
+  return it;
+}
+
 template <int kDim>
 struct Layout {
   static constexpr int kHalves = kDim / 64;         // 64-channel (128-byte) columns of a tile
   static constexpr int kHalfBytes = 128 * 128;      // 128 rows of one
   static constexpr int kTileBytes = kHalves * kHalfBytes;
-  static constexpr int kStages = kDim == 128 ? 5 : 8;
-  static constexpr int kRingOff = 2 * kTileBytes;   // Q_0 | Q_1 | stages
-  static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
+  static constexpr int kStages = kDim == 128 ? 4 : 6;
+  static constexpr int kRingOff = 2 * kTileBytes;   // Q_0 | Q_1 | stages | output staging
+  static constexpr int kOutOff = kRingOff + kStages * kTileBytes;
+  static constexpr int kOutBytes = 32 * 128;        // a softmax warp's: 32 rows of 64 channels
+  static constexpr int kBarOff = kOutOff + 8 * kOutBytes;
   // barriers: q_full[2] q_empty[2] s_full[2] p_full[4] (first halves, second halves) o_full[2]
   // drain[2] sched_full[3] sched_empty[3] kv_full[stages] kv_empty[stages] v_ok[stages] (by V tile, not by stage: a stage
   // of an odd ring holds K and V in turn)
   static constexpr int kBars = 20 + 3 * kStages;
-  static constexpr int kItemOff = kBarOff + kBars * 8;
+  static constexpr int kItemOff = (kBarOff + kBars * 8 + 15) / 16 * 16;
   static constexpr int kMiscOff = kItemOff + 3 * static_cast<int>(sizeof(Item));  // TMEM slot, abort, turn
   static constexpr int kOrderOff = kMiscOff + 16;
-  static constexpr int kBytes = 1024 + kOrderOff + 2 * kBuckets * 4;
+  static constexpr int kBytes = 1024 + kOrderOff + (kBuckets + 1) * 4;
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -128,13 +144,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// Items in an order that ends evenly: with two tiles of `tokens` query tokens an item, sequence s has
-// n_s = ceil(len / tokens) of them, and the later ones of a causal sequence see the most keys. They
-// are ordered by level (index within the sequence) downwards over all sequences, levels taken `width`
-// at a time as one of 128 buckets, and by sequence within a bucket.
+// The items stand in an order that ends evenly: most visible keys first, in kBuckets classes of
+// `width` keys; by sequence within a class, later items of a sequence first.
 struct Order {
-  uint32_t *starts;  // first tile of each bucket, top bucket first; [kBuckets]
-  uint32_t total;    // tiles
+  uint32_t *starts;  // first item of each class, top class first; [kBuckets]
+  uint32_t total;    // items
   uint32_t width;
   // where the last search stood
   int bucket;
@@ -151,29 +165,51 @@ struct PackedArgs {
   uint32_t *status;
   uint32_t n_seq, total_q, total_k, q_heads, kv_heads, group;
   uint32_t tokens;  // per tile
-  uint32_t width;   // levels per bucket
-  uint32_t wide;    // out rows are 32-byte aligned
+  PageDiv item;     // division by an item's 2 tokens
+  uint32_t boxed;   // 32 rows of a tile are whole tokens: one TMA box of the output
   bool causal;
   float scale_log2;
 };
 
 namespace {
-__device__ __forceinline__ uint32_t tiles_of(const PackedArgs &p, uint32_t s) {
-  uint32_t a, b;
-  sequence_rows(p.cu_q, s, p.total_q, &a, &b);
-  return (b - a + 2 * p.tokens - 1) / (2 * p.tokens);
+// A sequence as the scheduler sees it: `n` items of 2 p.tokens query tokens for one key-value head.
+struct Sequence {
+  uint32_t q0, a, k0, b, n;  // first rows, lengths
+};
+__device__ __forceinline__ Sequence sequence_of(const PackedArgs &p, uint32_t s) {
+  Sequence x;
+  uint32_t q1, k1;
+  sequence_rows(p.cu_q, s, p.total_q, &x.q0, &q1);
+  sequence_rows(p.cu_k, s, p.total_k, &x.k0, &k1);
+  x.a = q1 - x.q0;
+  x.b = k1 - x.k0;
+  x.n = page_of(p.item, x.a + 2 * p.tokens - 1);
+  return x;
+}
+// Items of the sequence whose last token sees more than `keys` keys: the last so many.
+__device__ __forceinline__ uint32_t items_above(const PackedArgs &p, const Sequence &x, uint32_t keys) {
+  if (x.n == 0 || x.b <= keys) return 0;
+  if (!p.causal) return x.n;
+  // item l's last token sees b - a + min(a, (l + 1) 2 tokens) of them
+  const int32_t beyond = static_cast<int32_t>(keys - x.b + x.a);
+  const uint32_t first = beyond < 0 ? 0u : page_of(p.item, static_cast<uint32_t>(beyond));
+  return x.n - min(first, x.n - 1);
+}
+// Items of the sequence in class c (`width` keys each; the lowest also holds those that see none).
+__device__ __forceinline__ uint32_t items_in(const PackedArgs &p, const Sequence &x, uint32_t c, uint32_t width) {
+  return (c == 0 ? x.n : items_above(p, x, c * width)) - items_above(p, x, (c + 1) * width);
 }
 
-// The item of tile `tile` and key-value head `head`; whole warp.
-__device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_t tile, uint32_t head) {
+// Item `index` in the order, for key-value head `head`; whole warp.
+__device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_t index, uint32_t head) {
   const uint32_t lane = threadIdx.x & 31u;
   Item it = {};
   it.head = static_cast<int32_t>(head);
   uint32_t mine = 0;
 #pragma unroll
-  for (int i = 0; i < kBuckets / 32; ++i) mine += o.starts[lane * (kBuckets / 32) + i] <= tile;
+  for (int i = 0; i < kBuckets / 32; ++i) mine += o.starts[lane * (kBuckets / 32) + i] <= index;
   const int at = static_cast<int>(__reduce_add_sync(0xffffffffu, mine)) - 1;
-  const uint32_t rest = tile - o.starts[at], base = (kBuckets - 1 - at) * o.width;
+  const uint32_t rest = index - o.starts[at], c = kBuckets - 1 - at;
   if (at != o.bucket || rest < o.before) {
     o.bucket = at;
     o.seq = 0;
@@ -181,31 +217,25 @@ __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_
   }
   for (; o.seq < p.n_seq; o.seq += 32) {
     const uint32_t s = o.seq + lane;
-    const uint32_t n = s < p.n_seq ? tiles_of(p, s) : 0u;
-    const uint32_t c = n > base ? min(n - base, at == 0 ? n : o.width) : 0u;
-    uint32_t sum = c;
+    Sequence x = {};
+    if (s < p.n_seq) x = sequence_of(p, s);
+    const uint32_t count = items_in(p, x, c, o.width);
+    uint32_t sum = count;
 #pragma unroll
     for (int i = 1; i < 32; i *= 2) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, sum, i);
-      if (lane >= static_cast<uint32_t>(i)) sum += x;
+      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, i);
+      if (lane >= static_cast<uint32_t>(i)) sum += y;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, rest < o.before + sum);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const uint32_t first = o.before + __shfl_sync(0xffffffffu, sum - c, src);
-      const uint32_t level = base + __shfl_sync(0xffffffffu, c, src) - 1 - (rest - first);
-      uint32_t q0, q1, k0, k1;
-      const uint32_t seq = o.seq + src;
-      sequence_rows(p.cu_q, seq, p.total_q, &q0, &q1);
-      sequence_rows(p.cu_k, seq, p.total_k, &k0, &k1);
-      const uint32_t t0 = level * 2 * p.tokens;
-      it.q_row = static_cast<int32_t>(q0 + t0);
-      it.q_count = static_cast<int32_t>(min(q1 - q0 - t0, 2 * p.tokens));
-      it.k_row = static_cast<int32_t>(k0);
-      it.k_len = static_cast<int32_t>(k1 - k0);
-      it.visible = p.causal ? static_cast<int32_t>(k1 - k0) - static_cast<int32_t>(q1 - q0) +
-                                  static_cast<int32_t>(t0) + 1
-                            : it.k_len;
+      const uint32_t within = rest - (o.before + sum - count);  // of this lane's sequence
+      const uint32_t t0 = (x.n - items_above(p, x, (c + 1) * o.width) - 1 - within) * 2 * p.tokens;
+      it.q_row = static_cast<int32_t>(__shfl_sync(0xffffffffu, x.q0 + t0, src));
+      it.q_count = static_cast<int32_t>(__shfl_sync(0xffffffffu, min(x.a - t0, 2 * p.tokens), src));
+      it.k_row = static_cast<int32_t>(__shfl_sync(0xffffffffu, x.k0, src));
+      it.k_len = static_cast<int32_t>(__shfl_sync(0xffffffffu, x.b, src));
+      it.visible = static_cast<int32_t>(__shfl_sync(0xffffffffu, p.causal ? x.b - x.a + t0 + 1 : x.b, src));
       return it;
     }
     o.before += __shfl_sync(0xffffffffu, sum, 31);
@@ -213,18 +243,23 @@ __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_
   return it;  // not reached while cu is ascending
 }
 
-// What a tile's rows see: steps of 128 keys, and the keys of its first token.
+// What a tile's rows see.
 struct Reach {
-  int steps;  // of this tile
+  int steps;  // of 128 keys
   int first;  // keys that its first token sees (at least 0)
+  int most;   // keys that its last token sees
 };
+// Blocks of 32 keys in step j that some row of the tile sees.
+__device__ __forceinline__ int blocks_of(const Reach &r, int j) {
+  return min(kKeys / 32, (r.most - j * kKeys + 31) / 32);
+}
 __device__ __forceinline__ Reach reach_of(const Item &it, int tile, int tokens, bool causal) {
   const int begin = tile * tokens, end = min(it.q_count, begin + tokens);
-  Reach r = {0, 0};
+  Reach r = {0, 0, 0};
   if (begin >= end) return r;
-  const int most = causal ? min(it.k_len, it.visible + end - 1) : it.k_len;
+  r.most = causal ? min(it.k_len, it.visible + end - 1) : it.k_len;
   r.first = max(0, causal ? min(it.k_len, it.visible + begin) : it.k_len);
-  r.steps = most > 0 ? (most + kKeys - 1) / kKeys : 0;
+  r.steps = r.most > 0 ? (r.most + kKeys - 1) / kKeys : 0;
   return r;
 }
 
@@ -243,82 +278,94 @@ __device__ __forceinline__ bool finite16(uint32_t half) {
   return (half & e) != e;
 }
 
-// Scores, weights and sums of one step for this thread's row. `vis`: keys of this step that the row
-// sees (used where kMasked). Returns through m (reference, log2 units), sum. The weights are handed
-// over in two halves (p_full[0], p_full[2]), so that the product with V starts under the second.
+// A row's reference, moved to the step's maximum `now` (log2 units) where that passes it by more than
+// kSlack; the row's sum and output so far follow. The previous product is done: the thread that
+// issued it issued these scores after it.
+__device__ __forceinline__ void move_reference(uint32_t to, int dim, float now, bool first, float &m,
+                                               float &sum) {
+  if (first) {
+    m = now;
+    return;
+  }
+  const bool grown = now > m + kSlack;
+  if (!__any_sync(0xffffffffu, grown)) return;
+  const float next = grown ? now : m;
+  const float f = grown ? ex2_approx(m - next) : 1.f;
+  sum *= f;
+  m = next;
+#pragma unroll 1
+  for (int d = 0; d < dim; d += 16) {
+    uint32_t x[16];
+    tmem_ld16(to + d, x);
+    tmem_ld_wait();
+    tmem_regs_ready16(x);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+    tmem_st16(to + d, x);
+  }
+}
+
+// The weights of 32 scores, 2^(s c - base), stored over consumed scores and added to (s0, s1).
+template <bool kBf16>
+__device__ __forceinline__ void weigh(uint32_t to, const uint32_t (&v)[32], uint64_t c2,
+                                      uint64_t base2, uint64_t &s0, uint64_t &s1) {
+  uint32_t w[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float2 x = unpair(fma2(pair(v[2 * e], v[2 * e + 1]), c2, base2));
+    const uint64_t w2 = pair(ex2_approx(x.x), ex2_approx(x.y));
+    if (e & 1)
+      s1 = add2(s1, w2);
+    else
+      s0 = add2(s0, w2);
+    const float2 f = unpair(w2);
+    w[e] = Elem<kBf16>::pack(f.x, f.y);
+  }
+  tmem_st16(to, w);
+}
+
+__device__ __forceinline__ void hand_over_weights(uint64_t *p_full) {
+  tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) mbar_arrive(p_full);
+}
+
+// Scores, weights and sums of one step for this thread's row, through m (reference, log2 units) and
+// sum. Where some row sees the step in part (kMasked), this one sees `vis` keys of it and the tile
+// `blocks` blocks of 32; the products skip the others. The weights are handed over in two halves
+// (p_full[0], p_full[2]), so that the product with V starts under the second.
 template <bool kBf16, bool kMasked>
 __device__ __forceinline__ void softmax_step(uint32_t tl, uint32_t to, int dim, float c, int vis,
-                                             bool first, float &m, float &sum, uint64_t *p_full) {
+                                             int blocks, bool first, float &m, float &sum,
+                                             uint64_t *p_full) {
   uint32_t v[4][32];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_ld32(tl + 32 * i, v[i]);
+  for (int i = 0; i < 4; ++i) tmem_ld32(tl + 32 * i, v[i]);  // past `blocks`: old values, not used
   tmem_wait_ld(v[0]);
 #pragma unroll
   for (int i = 1; i < 4; ++i) tmem_regs_ready(v[i]);
-  if constexpr (kMasked) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    if (kMasked && i >= blocks) break;
+    if constexpr (kMasked) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if (32 * i + e >= vis) v[i][e] = 0xff800000u;  // -inf
-  }
-  float top[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    top[i] = __uint_as_float(v[i][0]);
-#pragma unroll
-    for (int e = 1; e + 1 < 32; e += 2)
-      top[i] = max3(top[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
-    top[i] = fmaxf(top[i], __uint_as_float(v[i][31]));
-  }
-  const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-  if (first) {
-    m = now;
-  } else {
-    const bool grown = now > m + kSlack;
-    if (__any_sync(0xffffffffu, grown)) {
-      // rescale this row's output (factor 1 for rows that stay); the previous product is done: the
-      // same thread issued it before these scores
-      const float next = grown ? now : m;
-      const float f = grown ? ex2_approx(m - next) : 1.f;
-      sum *= f;
-      m = next;
-      for (int d = 0; d < dim; d += 16) {
-        uint32_t x[16];
-        tmem_ld16(to + d, x);
-        tmem_ld_wait();
-        tmem_regs_ready16(x);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-        tmem_st16(to + d, x);
-      }
     }
+#pragma unroll
+    for (int e = 0; e < 32; e += 2)
+      top[i] = max3(top[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
   }
+  move_reference(to, dim, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c, first, m, sum);
   const float base = m == -INFINITY ? 0.f : m;
   const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
   uint64_t s0 = 0, s1 = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t w[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint64_t x2 = fma2(pair(v[i][2 * e], v[i][2 * e + 1]), c2, base2);
-      const float2 x = unpair(x2);
-      const uint64_t w2 = pair(ex2_approx(x.x), ex2_approx(x.y));
-      if (e & 1)
-        s1 = add2(s1, w2);
-      else
-        s0 = add2(s0, w2);
-      const float2 f = unpair(w2);
-      w[e] = Elem<kBf16>::pack(f.x, f.y);
-    }
-    tmem_st16(tl + 16 * i, w);
-    if (i == 1 || i == 3) {
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (threadIdx.x % 32 == 0) mbar_arrive(p_full + (i == 1 ? 0 : 2));
-    }
+    if (!kMasked || i < blocks) weigh<kBf16>(tl + 16 * i, v[i], c2, base2, s0, s1);
+    if (i & 1) hand_over_weights(p_full + i - 1);
   }
   const float2 part = unpair(add2(s0, s1));
   sum += part.x + part.y;
@@ -330,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_packed_kernel(const __grid_constant__ CUtensorMap tmq,
                             const __grid_constant__ CUtensorMap tmk,
                             const __grid_constant__ CUtensorMap tmv,
+                            const __grid_constant__ CUtensorMap tmo,
                             const __grid_constant__ PackedArgs p) {
   using L = Layout<kDim>;
   constexpr int kStages = L::kStages;
@@ -339,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *q_empty = q_full + 2, *s_full = q_full + 4, *p_full = q_full + 6, *o_full = q_full + 10;
   uint64_t *drain = q_full + 12, *sched_full = q_full + 14, *sched_empty = q_full + 17;
   uint64_t *kv_full = q_full + 20, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages;
-  volatile Item *items = reinterpret_cast<volatile Item *>(smem + L::kItemOff);
+  Item *items = reinterpret_cast<Item *>(smem + L::kItemOff);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kMiscOff);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   uint32_t *turn = tmem_slot + 2;
@@ -378,14 +426,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
-  for (int i = threadIdx.x; i < 2 * kBuckets; i += kThreads) order[i] = 0;
+  for (int i = threadIdx.x; i <= kBuckets; i += kThreads) order[i] = 0;
   __syncthreads();
-  // Per bucket: sequences that end in it, and their levels there.
+  // The longest sequence sets the classes' width; then each sequence's items in them.
+  uint32_t longest = 0;
   for (uint32_t s = threadIdx.x; s < p.n_seq; s += kThreads) {
-    const uint32_t n = tiles_of(p, s);
-    const uint32_t b = min(n / p.width, kBuckets - 1u);
-    atomicAdd(&order[kBuckets - 1 - b], 1u);
-    atomicAdd(&order[kBuckets + kBuckets - 1 - b], n - b * p.width);
+    const Sequence x = sequence_of(p, s);
+    if (x.n) longest = max(longest, x.b);
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0) atomicMax(&order[kBuckets], longest);
+  __syncthreads();
+  const uint32_t width = max(1u, (order[kBuckets] + kBuckets - 1) / kBuckets);
+  // Few sequences: a warp for each, the classes over its lanes; else a thread, over its own classes.
+  if (p.n_seq <= 96) {
+    for (uint32_t s = warp; s < p.n_seq; s += kThreads / 32) {
+      const Sequence x = sequence_of(p, s);
+#pragma unroll
+      for (int i = lane; i < kBuckets; i += 32)
+        if (const uint32_t n = items_in(p, x, i, width)) atomicAdd(&order[kBuckets - 1 - i], n);
+    }
+  } else {
+    for (uint32_t s = threadIdx.x; s < p.n_seq; s += kThreads) {
+      const Sequence x = sequence_of(p, s);
+      uint32_t left = x.n;
+      for (int i = min(kBuckets - 1, static_cast<int>(x.b ? (x.b - 1) / width : 0)); left > 0; --i) {
+        const uint32_t n = items_in(p, x, i, width);
+        if (n) atomicAdd(&order[kBuckets - 1 - i], n);
+        left = i > 0 ? left - n : 0;
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -395,44 +465,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kGuardWarp) {
     fewer_registers();
-    // Starts of the buckets, top first: levels of a bucket = those of sequences ending in it, and
-    // `width` for each sequence that ends in a higher one.
-    Order o = {order, 0, p.width, -1, 0, 0};
-    {
-      constexpr int kPer = kBuckets / 32;
-      uint32_t ends[kPer], levels[kPer], higher = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        ends[i] = order[lane * kPer + i];
-        levels[i] = order[kBuckets + lane * kPer + i];
-        higher += ends[i];
-      }
-      const uint32_t own = higher;
+    Order o = {order, 0, width, -1, 0, 0};
+    {  // counts to starts
+      const uint32_t n0 = order[2 * lane], n1 = order[2 * lane + 1];
+      static_assert(kBuckets == 64, "two classes a lane");
+      uint32_t sum = n0 + n1;
 #pragma unroll
       for (int i = 1; i < 32; i *= 2) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, higher, i);
-        if (lane >= i) higher += x;
+        const uint32_t x = __shfl_up_sync(0xffffffffu, sum, i);
+        if (lane >= i) sum += x;
       }
-      higher -= own;
-      uint32_t sum = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const uint32_t n = levels[i] + higher * p.width;
-        higher += ends[i];
-        ends[i] = sum;  // start within this lane
-        sum += n;
-      }
-      uint32_t before = sum;
-#pragma unroll
-      for (int i = 1; i < 32; i *= 2) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, before, i);
-        if (lane >= i) before += x;
-      }
-      o.total = __shfl_sync(0xffffffffu, before, 31);
-      before -= sum;
+      o.total = __shfl_sync(0xffffffffu, sum, 31);
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) order[lane * kPer + i] = before + ends[i];
+      order[2 * lane] = sum - n0 - n1;
+      order[2 * lane + 1] = sum - n1;
       __syncwarp();
     }
     const uint64_t n_items = static_cast<uint64_t>(o.total) * p.kv_heads;
@@ -499,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               x[i] = w;
             }
-            items[k % 3].fix = 1;
+            *reinterpret_cast<volatile int32_t *>(&items[k % 3].fix) = 1;
             fence_proxy_async_smem();
           }
         }
@@ -519,9 +565,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       uint32_t ring = 0, phase = 0, armed = 0, parity = 0;
       uint32_t q_phase[2] = {0, 0};
-      bool q_armed[2] = {false, false}, ok = true;
+      bool q_armed[2] = {false, false}, q_due[2] = {false, false}, ok = true;
+      Item it = {};
+      // Q tiles go out as soon as the item before has used them up, between the K and V loads.
+      auto load_q = [&] {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!q_due[t] || !mbar_test(&q_empty[t], q_phase[t] ^ 1u)) continue;
+          mbar_arrive_expect_tx(&q_full[t], p.tokens * p.group * 128u * L::kHalves);
+#pragma unroll
+          for (int h = 0; h < L::kHalves; ++h)
+            tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &tmq, &q_full[t], 64 * h,
+                        it.head * static_cast<int>(p.group), it.q_row + t * tokens);
+          q_armed[t] = true;
+          q_due[t] = false;
+          q_phase[t] ^= 1;
+        }
+      };
+      auto wait = [&](auto &&done) {
+        if (done()) return true;
+        const uint64_t t0 = globaltimer();
+        while (true) {
+#pragma unroll 1
+          for (int i = 0; i < 64; ++i) {
+            load_q();
+            if (done()) return true;
+          }
+          if (*abort_flag || globaltimer() - t0 > kWaitTimeoutNs) return false;
+        }
+      };
       auto load_kv = [&](const CUtensorMap *map, int row, int head) {
-        if (!mbar_wait(&kv_empty[ring], phase ^ 1u, abort_flag)) return false;
+        if (!wait([&] { return mbar_test(&kv_empty[ring], phase ^ 1u); })) return false;
         uint8_t *dst = smem + L::kRingOff + ring * L::kTileBytes;
         mbar_arrive_expect_tx(&kv_full[ring], L::kTileBytes);
 #pragma unroll
@@ -535,36 +609,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t k = 0; ok; ++k) {
         ok = mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag);
         if (!ok) break;
-        Item it;
-        it.q_row = items[k % 3].q_row;
-        it.q_count = items[k % 3].q_count;
-        it.k_row = items[k % 3].k_row;
-        it.k_len = items[k % 3].k_len;
-        it.visible = items[k % 3].visible;
-        it.head = items[k % 3].head;
-        it.last = items[k % 3].last;
+        it = read_item(&items[k % 3]);
         mbar_arrive(&sched_empty[k % 3]);
         if (it.last) break;
         const Reach r[2] = {reach_of(it, 0, tokens, p.causal), reach_of(it, 1, tokens, p.causal)};
         const int steps = max(r[0].steps, r[1].steps);
+        q_due[0] = r[0].steps > 0;
+        q_due[1] = r[1].steps > 0;
         for (int j = 0; ok && j < steps; ++j) {
           ok = load_kv(&tmk, it.k_row + j * kKeys, it.head);
-          if (j == 0) {
-            for (int t = 0; ok && t < 2; ++t) {
-              if (r[t].steps == 0) continue;
-              ok = mbar_wait(&q_empty[t], q_phase[t] ^ 1u, abort_flag);
-              if (!ok) break;
-              mbar_arrive_expect_tx(&q_full[t], p.tokens * p.group * 128u * L::kHalves);
-#pragma unroll
-              for (int h = 0; h < L::kHalves; ++h)
-                tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &tmq, &q_full[t], 64 * h,
-                            it.head * static_cast<int>(p.group), it.q_row + t * tokens);
-              q_armed[t] = true;
-              q_phase[t] ^= 1;
-            }
-          }
+          load_q();
           ok = ok && load_kv(&tmv, it.k_row + j * kKeys, it.head);
         }
+        ok = ok && wait([&] { return !q_due[0] && !q_due[1]; });
       }
       if (!ok) {
         report(p.status, kErrAttentionWait);
@@ -580,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fewer_registers();
     if (lane == 0) {
       const int t = warp - kMmaWarp;
-      constexpr uint32_t idesc_s = idesc_f32(kBf16, 128, kKeys, false);
+      constexpr uint32_t idesc_s = idesc_f32(kBf16, 128, 0, false);  // N to come: 32 a block
       constexpr uint32_t idesc_o = idesc_f32(kBf16, 128, kDim, true);
       const uint32_t d_s = tmem + t * 128, d_o = tmem + kTmemO + t * 128;
       const uint32_t q_at = smem_u32(smem + t * L::kTileBytes);
@@ -602,12 +659,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto give = [&] { *reinterpret_cast<volatile uint32_t *>(turn) = 0u; };
       // S = Q K^T of stage `stage`, the last of a turn.
-      auto scores = [&](uint32_t stage) {
+      auto scores = [&](uint32_t stage, int blocks) {
+        const uint32_t idesc = idesc_s | static_cast<uint32_t>(blocks * 32 / 8) << 17;
+        tc_fence_after();
         const uint32_t k_at = smem_u32(smem + L::kRingOff + stage * L::kTileBytes);
 #pragma unroll
         for (int kk = 0; kk < kDim / 16; ++kk) {
           const uint32_t off = (kk / 4) * L::kHalfBytes + (kk % 4) * 32;
-          umma_f16(d_s, sw128_desc(q_at + off), sw128_desc(k_at + off), idesc_s, kk > 0);
+          umma_f16(d_s, sw128_desc(q_at + off), sw128_desc(k_at + off), idesc, kk > 0);
         }
         give();
       };
@@ -617,26 +676,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit(&s_full[t]);
         if (last) umma_commit(&q_empty[t]);
       };
-      // Half of O += P V.
-      auto product = [&](uint32_t v_at, int half, bool first) {
+      // Half of O += P V; of a step with fewer than four blocks of 32 keys only theirs.
+      auto product = [&](uint32_t v_at, int half, bool first, int blocks) {
+        tc_fence_after();
+        if (blocks == 4) {
 #pragma unroll
-        for (int i = 0; i < kKeys / 32; ++i) {
-          const int kk = half * (kKeys / 32) + i;
-          umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
-                      !first || kk > 0);
+          for (int i = 0; i < 4; ++i) {
+            const int kk = half * 4 + i;
+            umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
+                        !first || kk > 0);
+          }
+        } else {
+#pragma unroll 1
+          for (int kk = half * 4; kk < min(2 * blocks, half * 4 + 4); ++kk)
+            umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
+                        !first || kk > 0);
         }
       };
       for (uint32_t k = 0; ok; ++k) {
         ok = mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag);
         if (!ok) break;
-        Item it;
-        it.q_count = items[k % 3].q_count;
-        it.k_len = items[k % 3].k_len;
-        it.visible = items[k % 3].visible;
-        it.last = items[k % 3].last;
+        const Item it = read_item(&items[k % 3]);
         mbar_arrive(&sched_empty[k % 3]);
         if (it.last) break;
-        const int mine = reach_of(it, t, tokens, p.causal).steps;
+        const Reach reach = reach_of(it, t, tokens, p.causal);
+        const int mine = reach.steps;
         const int steps = max(mine, reach_of(it, 1 - t, tokens, p.causal).steps);
         if (steps == 0) continue;
         uint32_t k_stage = ring;
@@ -647,8 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = mbar_wait(&q_full[t], q_phase, abort_flag) && take();
           if (!ok) break;
           q_phase ^= 1;
-          tc_fence_after();
-          scores(k_stage);
+          scores(k_stage, blocks_of(reach, 0));
           hand_over(mine == 1);
         } else {
           mbar_arrive(&kv_empty[k_stage]);
@@ -675,8 +738,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t v_at = smem_u32(smem + L::kRingOff + v_stage * L::kTileBytes);
           ok = mbar_wait(&p_full[t], p_phase, abort_flag) && take();
           if (!ok) break;
-          tc_fence_after();
-          product(v_at, 0, j == 0);
+          const int blocks = blocks_of(reach, j);
+          product(v_at, 0, j == 0, blocks);
           // where the second half is there by now, the turn is kept
           if (!mbar_test(&p_full[2 + t], p_phase)) {
             give();
@@ -684,10 +747,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
           }
           p_phase ^= 1;
-          tc_fence_after();
-          product(v_at, 1, j == 0);
+          product(v_at, 1, j == 0, blocks);
           if (j + 1 < mine) {
-            scores(k_stage);
+            scores(k_stage, blocks_of(reach, j + 1));
             hand_over(j + 2 == mine);
           } else {
             give();
@@ -711,6 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tl = tmem + lanes + t * 128, to = tmem + lanes + kTmemO + t * 128;
     const float c = p.scale_log2;
+    uint8_t *stage = smem + L::kOutOff + warp * L::kOutBytes;
     uint32_t s_phase = 0, o_phase = 0, ring = 0;
     // Release the stage at `ring`, for this tile, once its last product with it is known to be done.
     auto release = [&] {
@@ -721,14 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t k = 0; ok; ++k) {
       ok = __all_sync(0xffffffffu, mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag));
       if (!ok) break;
-      Item it;
-      it.q_row = items[k % 3].q_row;
-      it.q_count = items[k % 3].q_count;
-      it.k_row = items[k % 3].k_row;
-      it.k_len = items[k % 3].k_len;
-      it.visible = items[k % 3].visible;
-      it.head = items[k % 3].head;
-      it.last = items[k % 3].last;
+      const Item it = read_item(&items[k % 3]);
       __syncwarp();
       const Reach r = reach_of(it, t, tokens, p.causal);
       const int whole = r.first / kKeys;  // steps that every row of the tile sees in full
@@ -743,11 +799,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j > 0) release();  // the previous step's V
         release();             // this step's K
         if (j < whole)
-          softmax_step<kBf16, false>(tl, to, kDim, c, kKeys, j == 0, m, sum, &p_full[t]);
+          softmax_step<kBf16, false>(tl, to, kDim, c, kKeys, 4, j == 0, m, sum, &p_full[t]);
         else
-          softmax_step<kBf16, true>(tl, to, kDim, c, sees - j * kKeys, j == 0, m, sum, &p_full[t]);
+          softmax_step<kBf16, true>(tl, to, kDim, c, sees - j * kKeys, blocks_of(r, j), j == 0, m, sum,
+                                    &p_full[t]);
       }
       if (!ok) break;
+      // Where the row goes, worked out under the last product.
+      const bool live = token < tokens && mine < it.q_count;
+      const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
+      const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
+      uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
+      if (live && p.lse) p.lse[out_row * p.q_heads + head] = (m + log2f(sum)) * kLn2;
       if (r.steps > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag));
         if (!ok) break;
@@ -757,49 +822,72 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // the issuer releases the stages of steps that only the other tile has
       ring = (ring + 2 * (max(r.steps, reach_of(it, 1 - t, tokens, p.causal).steps) - r.steps)) % kStages;
-      const int fix = r.steps > 0 ? items[k % 3].fix : 0;
+      const int fix = r.steps > 0 ? *reinterpret_cast<volatile int32_t *>(&items[k % 3].fix) : 0;
       __syncwarp();
-      // From here on the slot is not read again; the next item but one may be written into it.
+      // From here on the slot is not read again; the next item but two may be written into it.
       if (lane == 0) mbar_arrive(&sched_empty[k % 3]);
       if (it.last) break;
-      const bool live = token < tokens && mine < it.q_count;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
-      const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
-      uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
-      if (live && p.lse) p.lse[out_row * p.q_heads + head] = (m + log2f(sum)) * kLn2;
+      // 64 channels at a time through this warp's staging (16-byte chunk c of row r at c ^ (r & 7)):
+      // by one TMA store where all 32 rows are of the sequence and whole tokens, else 8 lanes to a
+      // row of 128 bytes.
+      const bool boxed = p.boxed && rows_live == 0xffffffffu;
+#pragma unroll 1
+      for (int d = 0; d < kDim; d += 64) {
+        if (lane == 0) bulk_wait_read<0>();  // the store before has read the staging
+        __syncwarp();
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t x[32];
+          if (r.steps > 0) {
+            tmem_load32(to + d + 32 * half, x);
+          } else {
 #pragma unroll
-      for (int d = 0; d < kDim; d += 32) {
-        uint32_t x[32];
-        if (r.steps > 0) {
-          tmem_load32(to + d, x);
-        } else {
+            for (int e = 0; e < 32; ++e) x[e] = 0;
+          }
+          if (fix && live) {
+            // what the guard took out of the steps that are seen in part
+            const int from = reach_of(it, 0, tokens, p.causal).first / kKeys * kKeys;
+#pragma unroll 1
+            for (int kk = from; kk < sees; ++kk) {
+              const uint32_t *v = reinterpret_cast<const uint32_t *>(
+                  p.v + (static_cast<int64_t>(it.k_row) + kk) * p.v_token + it.head * p.v_head + d + 32 * half);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = 0;
-        }
-        if (fix && live) {
-          // what the guard took out of the steps that are seen in part
-          const int from = reach_of(it, 0, tokens, p.causal).first / kKeys * kKeys;
-          for (int kk = from; kk < sees; ++kk) {
-            const uint32_t *v = reinterpret_cast<const uint32_t *>(
-                p.v + (static_cast<int64_t>(it.k_row) + kk) * p.v_token + it.head * p.v_head + d);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint32_t w = v[e];
-              const float2 f = Elem<kBf16>::unpack(w);
-              if (!finite16<kBf16>(w & 0xffffu)) x[2 * e] = __float_as_uint(__uint_as_float(x[2 * e]) + f.x);
-              if (!finite16<kBf16>(w >> 16)) x[2 * e + 1] = __float_as_uint(__uint_as_float(x[2 * e + 1]) + f.y);
+              for (int e = 0; e < 16; ++e) {
+                const uint32_t w = v[e];
+                const float2 f = Elem<kBf16>::unpack(w);
+                if (!finite16<kBf16>(w & 0xffffu)) x[2 * e] = __float_as_uint(__uint_as_float(x[2 * e]) + f.x);
+                if (!finite16<kBf16>(w >> 16)) x[2 * e + 1] = __float_as_uint(__uint_as_float(x[2 * e + 1]) + f.y);
+              }
             }
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = Elem<kBf16>::pack(__uint_as_float(x[8 * e + 2 * i]) * inv, __uint_as_float(x[8 * e + 2 * i + 1]) * inv);
+            *reinterpret_cast<uint4 *>(stage + lane * 128 + (((4 * half + e) ^ (lane & 7)) * 16)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          w[e] = Elem<kBf16>::pack(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv);
-        if (live) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<uint4 *>(dst + d + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+        if (boxed) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&tmo, stage, d, it.head * static_cast<int>(p.group), it.q_row + t * tokens + q * (32 / static_cast<int>(p.group)));
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const int from = 4 * i + lane / 8;  // row of this warp
+            const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), from);
+            if (rows_live >> from & 1)
+              *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(at) + d + 8 * (lane % 8)) =
+                  *reinterpret_cast<const uint4 *>(stage + from * 128 + (((lane % 8) ^ (from & 7)) * 16));
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -808,6 +896,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       report(p.status, kErrAttentionWait);
       *abort_flag = 1;
     }
+    if (lane == 0) bulk_wait<0>();  // output stores complete before the CTA retires
   }
 
   __syncwarp();
@@ -822,7 +911,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 namespace {
 template <bool kBf16, int kDim>
 cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v,
-                   const PackedArgs &a, int dev, uint32_t grid, cudaStream_t stream) {
+                   const CUtensorMap &o, const PackedArgs &a, int dev, uint32_t grid, cudaStream_t stream) {
   static std::atomic<bool> configured[64] = {};
   if (dev >= 0 && dev < 64 && !configured[dev].load(std::memory_order_acquire)) {
     // setting the attribute twice (two threads racing here) is harmless
@@ -833,7 +922,7 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
     configured[dev].store(true, std::memory_order_release);
   }
   attention_packed_kernel<kBf16, kDim>
-      <<<dim3(grid), dim3(kThreads), Layout<kDim>::kBytes, stream>>>(q, k, v, a);
+      <<<dim3(grid), dim3(kThreads), Layout<kDim>::kBytes, stream>>>(q, k, v, o, a);
   return cudaGetLastError();
 }
 }  // namespace
@@ -842,14 +931,17 @@ cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStr
                                     std::string *err) {
   if (p.total_q == 0 || p.n_seq == 0) return cudaSuccess;
   const uint32_t group = p.q_heads / p.kv_heads, tokens = 128 / group;
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, o;
+  const bool boxed = 32 % group == 0;
   const bool maps =
       encode_map_rows(&q, p.q, bf16, p.head_dim, p.q_heads, p.total_q, p.q_head, p.q_token, group, tokens, err) &&
       // without keys the maps stand on q: no load reads through them
       encode_map_rows(&k, p.total_k ? p.k : p.q, bf16, p.head_dim, p.kv_heads, p.total_k ? p.total_k : 1, p.k_head,
                       p.k_token, 1, kKeys, err) &&
       encode_map_rows(&v, p.total_k ? p.v : p.q, bf16, p.head_dim, p.kv_heads, p.total_k ? p.total_k : 1, p.v_head,
-                      p.v_token, 1, kKeys, err);
+                      p.v_token, 1, kKeys, err) &&
+      encode_map_rows(&o, p.out, bf16, p.head_dim, p.q_heads, p.total_q, p.out_head, p.out_token,
+                      boxed ? group : 1, boxed ? 32 / group : 1, err);
   if (!maps) return cudaErrorInvalidValue;
   PackedArgs a = {};
   a.v = p.v;
@@ -869,10 +961,11 @@ cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStr
   a.kv_heads = p.kv_heads;
   a.group = group;
   a.tokens = tokens;
+  a.item = page_div(2 * tokens);
+  a.boxed = boxed;
   a.causal = p.causal;
   a.scale_log2 = p.scale * kLog2e;
   const uint64_t levels = (static_cast<uint64_t>(p.total_q) + 2 * tokens - 1) / (2 * tokens);
-  a.width = static_cast<uint32_t>((levels + kBuckets - 1) / kBuckets);
   int dev = 0;
   cudaGetDevice(&dev);
   // at most one partly filled item per sequence
@@ -880,8 +973,8 @@ cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStr
   const uint32_t sms = static_cast<uint32_t>(sm_count(dev));
   const uint32_t grid = most < sms ? static_cast<uint32_t>(most) : sms;
   if (p.head_dim == 64)
-    return bf16 ? launch<true, 64>(q, k, v, a, dev, grid, stream) : launch<false, 64>(q, k, v, a, dev, grid, stream);
-  return bf16 ? launch<true, 128>(q, k, v, a, dev, grid, stream) : launch<false, 128>(q, k, v, a, dev, grid, stream);
+    return bf16 ? launch<true, 64>(q, k, v, o, a, dev, grid, stream) : launch<false, 64>(q, k, v, o, a, dev, grid, stream);
+  return bf16 ? launch<true, 128>(q, k, v, o, a, dev, grid, stream) : launch<false, 128>(q, k, v, o, a, dev, grid, stream);
 }
 
 }  // namespace dv3
