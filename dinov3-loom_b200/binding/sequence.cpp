@@ -26,7 +26,8 @@ namespace {
 int (*packed_fn)(const dv3k_packed_attention *, void *);
 int (*append_fn)(const dv3k_rope_append_args *, void *);
 int (*paged_fn)(const dv3k_paged_attention *, void *);
-size_t (*workspace_fn)(const dv3k_paged_attention *);
+size_t (*packed_workspace_fn)(const dv3k_packed_attention *);
+size_t (*paged_workspace_fn)(const dv3k_paged_attention *);
 PyObject *refuse_cb;  // refuse_cb(message) raises
 PyObject *check_cb;   // check_cb(status) raises the library's message
 
@@ -142,6 +143,25 @@ PyObject *result(PyObject *given, at::Tensor &&t) {
   return THPVariable_Wrap(std::move(t));
 }
 
+// The call's scratch: the given tensor, or a new one of the size it needs, which the caller holds until
+// the launch is out (torch's allocator then hands it on in stream order only).
+template <class Args>
+at::Tensor scratch_of(PyObject *given, Args &p, size_t (*need_of)(const Args *), const at::Tensor &q) {
+  at::Tensor w;
+  if (given != Py_None) {
+    w = tensor(given, "workspace");
+    if (w.scalar_type() != at::kByte || w.device() != q.device() || !w.is_contiguous())
+      refuse("workspace must be a contiguous uint8 tensor on ", q.device());
+  } else if (const size_t need = need_of(&p)) {
+    w = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte).requires_grad(false));
+  } else {
+    return w;
+  }
+  p.workspace = w.data_ptr();
+  p.workspace_bytes = static_cast<uint64_t>(w.numel());
+  return w;
+}
+
 // Runs `f` on the tensors' device and its current stream; a nonzero status raises.
 template <class F>
 void on_device(const at::Tensor &t, F &&f) {
@@ -175,9 +195,9 @@ PyObject *guarded(Py_ssize_t got, Py_ssize_t want, F &&f) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, k, v, cu_q, cu_k, causal, scale, out, lse, status)
+// (q, k, v, cu_q, cu_k, causal, scale, out, lse, workspace, status)
 PyObject *attention_packed(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  return guarded(n, 10, [&] {
+  return guarded(n, 11, [&] {
     const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
     const at::Tensor &cu_q = tensor(a[3], "cu_q"), &cu_k = a[4] == Py_None ? cu_q : tensor(a[4], "cu_k");
     dv3k_packed_attention p = {};
@@ -195,7 +215,7 @@ PyObject *attention_packed(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (causal < 0) throw Raised{};
     p.scale = scale_of(a[6], q.size(2));
     p.lse = static_cast<float *>(optional(a[8], "lse", q, at::kFloat, {q.size(0), q.size(1)}));
-    p.status = status_of(a[9], q);
+    p.status = status_of(a[10], q);
     at::Tensor out = output(a[7], "out", q, q);
     p.q = q.data_ptr();
     p.k = k.data_ptr();
@@ -218,7 +238,11 @@ PyObject *attention_packed(PyObject *, PyObject *const *a, Py_ssize_t n) {
     p.kv_heads = static_cast<uint32_t>(k.size(1));
     p.head_dim = size32(q.size(2), "dim");
     p.causal = static_cast<uint32_t>(causal);
-    on_device(q, [&](void *stream) { return packed_fn(&p, stream); });
+    at::Tensor scratch;
+    on_device(q, [&](void *stream) {
+      scratch = scratch_of(a[9], p, packed_workspace_fn, q);
+      return packed_fn(&p, stream);
+    });
     return result(a[7], std::move(out));
   });
 }
@@ -342,33 +366,24 @@ PyObject *attention_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
     p.head_dim = size32(q.size(2), "dim");
     at::Tensor scratch;
     on_device(q, [&](void *stream) {
-      if (a[9] != Py_None) {
-        const at::Tensor &w = tensor(a[9], "workspace");
-        if (w.scalar_type() != at::kByte || w.device() != q.device() || !w.is_contiguous())
-          refuse("workspace must be a contiguous uint8 tensor on ", q.device());
-        p.workspace = w.data_ptr();
-        p.workspace_bytes = static_cast<uint64_t>(w.numel());
-      } else if (const size_t need = workspace_fn(&p)) {
-        // freed on return: torch's allocator hands it on in stream order only
-        scratch = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte).requires_grad(false));
-        p.workspace = scratch.data_ptr();
-        p.workspace_bytes = need;
-      }
+      scratch = scratch_of(a[9], p, paged_workspace_fn, q);
       return paged_fn(&p, stream);
     });
     return result(a[7], std::move(out));
   });
 }
 
-// bind(packed, append, paged, workspace, refuse, check): the entry points' addresses, and what raises.
+// bind(packed, its workspace, append, paged, its workspace, refuse, check): the entry points' addresses,
+// and what raises.
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long f[4];
+  unsigned long long f[5];
   PyObject *refuse_to, *check_to;
-  if (!PyArg_ParseTuple(args, "KKKKOO", &f[0], &f[1], &f[2], &f[3], &refuse_to, &check_to)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKOO", &f[0], &f[1], &f[2], &f[3], &f[4], &refuse_to, &check_to)) return nullptr;
   packed_fn = reinterpret_cast<decltype(packed_fn)>(f[0]);
-  append_fn = reinterpret_cast<decltype(append_fn)>(f[1]);
-  paged_fn = reinterpret_cast<decltype(paged_fn)>(f[2]);
-  workspace_fn = reinterpret_cast<decltype(workspace_fn)>(f[3]);
+  packed_workspace_fn = reinterpret_cast<decltype(packed_workspace_fn)>(f[1]);
+  append_fn = reinterpret_cast<decltype(append_fn)>(f[2]);
+  paged_fn = reinterpret_cast<decltype(paged_fn)>(f[3]);
+  paged_workspace_fn = reinterpret_cast<decltype(paged_workspace_fn)>(f[4]);
   Py_INCREF(refuse_to);
   Py_INCREF(check_to);
   Py_XSETREF(refuse_cb, refuse_to);

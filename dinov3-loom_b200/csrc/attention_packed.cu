@@ -14,7 +14,7 @@
 //
 // Roles (384 threads):
 //   warps 0-3  softmax and output of tile 0, warps 4-7 of tile 1: one query row per thread (its
-//              TMEM lane). All 128 scores of a step are held in registers: running maximum, w =
+//              TMEM lane). All scores of a step are held in registers: running maximum, w =
 //              2^(s c - m c) with c = scale log2(e), f32 sum of the unrounded weights, P (rounded to
 //              the element type) back to TMEM over the consumed scores. The reference m only moves
 //              when the maximum has grown by more than 2^8 over it: any m gives the same quotient,
@@ -23,14 +23,13 @@
 //              tile to global memory. Of a last, partly visible step only the blocks of 32 keys
 //              that some row sees are computed.
 //   warp 8     TMA producer: Q tiles, then K and V tiles in turn through one ring of stages.
-//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = N = 128), and O_t += P_t V with P
+//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = 128, N = a step's keys), and O_t += P_t V with P
 //              from TMEM and V as the MN-major B operand, one tile at a time.
 //   warp 11    scheduler (publishes items one ahead), and guard of V: a key that a row does not see has weight 0, but 0 times
 //              an infinity or NaN is NaN. Only the tiles at an item's end (from the first that some
 //              row sees in part) can hold such keys; there it tests V in shared memory, sets what
 //              is not finite to 0 and leaves a note, and the rows that do see those keys add them
 //              at the end from global memory.
-// TMEM: S_0 | S_1 | O_0 | O_1, 128 columns each.
 //
 // Every wait is bounded; on a timeout the kernel records kErrAttentionWait, raises the CTA's
 // abort flag, lets its own copies and MMAs in flight land, frees TMEM and returns.
@@ -45,10 +44,7 @@ constexpr int kThreads = 384;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;  // TMEM allocator; issues tile 0's MMAs, warp 10 tile 1's
 constexpr int kGuardWarp = 11;
-constexpr int kKeys = 128;      // keys per step
 constexpr int kBuckets = 64;    // of the scheduler's order
-constexpr int kTmemCols = 512;
-constexpr int kTmemO = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;   // log2 units by which a row's maximum may pass its reference
 
@@ -60,7 +56,7 @@ struct __align__(16) Item {
   int32_t k_len;
   int32_t visible;  // keys the first token sees, less than 1 if none; a later one sees one more if causal
   int32_t head;     // key-value head
-  int32_t last;     // 1: no more items
+  int32_t part;     // -1: no more items; 0: the whole of it; else 1 + the place of its partial result
   int32_t fix;      // set by the guard: V held something that is not finite
 };
 
@@ -71,26 +67,35 @@ __device__ __forceinline__ Item read_item(const Item *slot) {
                : "r"(smem_u32(slot))
                : "memory");
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(it.visible), "=r"(it.head), "=r"(it.last), "=r"(it.fix)
+               : "=r"(it.visible), "=r"(it.head), "=r"(it.part), "=r"(it.fix)
                : "r"(smem_u32(slot) + 16)
                : "memory");
   return it;
 }
 
+// At 64 channels the outputs leave TMEM columns for P, so that a step's scores need not wait for the
+// step before to be done with its weights: they are issued when the softmax has the previous ones in
+// registers, and the next softmax starts at once.
 template <int kDim>
 struct Layout {
-  static constexpr int kHalves = kDim / 64;         // 64-channel (128-byte) columns of a tile
-  static constexpr int kHalfBytes = 128 * 128;      // 128 rows of one
-  static constexpr int kTileBytes = kHalves * kHalfBytes;
+  static constexpr int kKeys = 128;  // a step
+  static constexpr int kBlocks = kKeys / 32;
+  static constexpr bool kOwnP = kDim == 64;
+  static constexpr int kTmemO = 2 * kKeys;              // S_0 | S_1 | O_0 | O_1 | P_0 | P_1
+  static constexpr int kTmemP = kOwnP ? kTmemO + 2 * kDim : 0;
+  static constexpr int kTmemPStep = kOwnP ? kKeys / 2 : kKeys;  // from P_0 to P_1
+  static constexpr int kHalves = kDim / 64;             // 64-channel (128-byte) columns of a tile
+  static constexpr int kQHalf = 128 * 128, kQBytes = kHalves * kQHalf;
+  static constexpr int kTileHalf = kKeys * 128, kTileBytes = kHalves * kTileHalf;  // of K or V
   static constexpr int kStages = kDim == 128 ? 4 : 6;
-  static constexpr int kRingOff = 2 * kTileBytes;   // Q_0 | Q_1 | stages | output staging
+  static constexpr int kRingOff = 2 * kQBytes;          // Q_0 | Q_1 | stages | output staging
   static constexpr int kOutOff = kRingOff + kStages * kTileBytes;
-  static constexpr int kOutBytes = 32 * 128;        // a softmax warp's: 32 rows of 64 channels
+  static constexpr int kOutBytes = 32 * 128;            // a softmax warp's: 32 rows of 64 channels
   static constexpr int kBarOff = kOutOff + 8 * kOutBytes;
-  // barriers: q_full[2] q_empty[2] s_full[2] p_full[4] (first halves, second halves) o_full[2]
+  // barriers: q_full[2] q_empty[2] s_full[2] s_free[2] p_full[4] (first halves, second halves) o_full[2]
   // drain[2] sched_full[3] sched_empty[3] kv_full[stages] kv_empty[stages] v_ok[stages] (by V tile, not by stage: a stage
   // of an odd ring holds K and V in turn)
-  static constexpr int kBars = 20 + 3 * kStages;
+  static constexpr int kBars = 22 + 3 * kStages;
   static constexpr int kItemOff = (kBarOff + kBars * 8 + 15) / 16 * 16;
   static constexpr int kMiscOff = kItemOff + 3 * static_cast<int>(sizeof(Item));  // TMEM slot, abort, turn
   static constexpr int kOrderOff = kMiscOff + 16;
@@ -145,11 +150,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // The items stand in an order that ends evenly: most visible keys first, in kBuckets classes of
-// `width` keys; by sequence within a class, later items of a sequence first.
+// `width` keys; by sequence within a class, later items of a sequence first. Where there are few items
+// and some have more steps than 1.5 times what the average CTA has in all, those are cut into parts of
+// at most so many (`part`), by class, that other CTAs take (300 queries behind 16000 keys: 253 us uncut,
+// 148 cut at the average, where the parts' starts and joins weigh more, 106 so); a part leaves (max, sum, unnormalised output) in
+// the workspace and a second launch joins them. The classes that are cut are the first in the order,
+// so that a part's place in it is also its place in the workspace.
 struct Order {
-  uint32_t *starts;  // first item of each class, top class first; [kBuckets]
-  uint32_t total;    // items
+  uint32_t *starts;  // first entry (item, or part) of each class, top class first; [kBuckets]
+  uint32_t total;    // entries
   uint32_t width;
+  uint32_t part;     // steps; 0: nothing is cut
   // where the last search stood
   int bucket;
   uint32_t seq, before;
@@ -168,7 +179,36 @@ struct PackedArgs {
   PageDiv item;     // division by an item's 2 tokens
   uint32_t boxed;   // 32 rows of a tile are whole tokens: one TMA box of the output
   bool causal;
+  bool flat;           // no CTA gets more than one item: their order does not matter
+  uint32_t parts_max;  // partial results that the workspace holds; 0: nothing is cut
+  void *workspace;
   float scale_log2;
+};
+
+// Workspace of the cut items: the parts' number, then for each part what it is, (max, sum) of its
+// 2 x 128 rows, and their outputs, four channels of 128 rows after another.
+struct Part {
+  int32_t q_row, q_count, head, index, parts;
+  int32_t unused[3];
+};
+template <int kDim>
+struct Parts {
+  uint32_t *count;
+  Part *what;
+  float2 *ml;   // [part][2][128]
+  float4 *o;    // [part][2][kDim / 4][128]
+  __host__ __device__ static size_t bytes(uint32_t n) {
+    return 16 + static_cast<size_t>(n) * (sizeof(Part) + 256 * sizeof(float2) + 256 * kDim * sizeof(float));
+  }
+  __device__ static Parts of(void *workspace, uint32_t n) {
+    Parts p;
+    uint8_t *at = static_cast<uint8_t *>(workspace);
+    p.count = reinterpret_cast<uint32_t *>(at);
+    p.what = reinterpret_cast<Part *>(at + 16);
+    p.ml = reinterpret_cast<float2 *>(p.what + n);
+    p.o = reinterpret_cast<float4 *>(p.ml + static_cast<size_t>(n) * 256);
+    return p;
+  }
 };
 
 namespace {
@@ -200,7 +240,15 @@ __device__ __forceinline__ uint32_t items_in(const PackedArgs &p, const Sequence
   return (c == 0 ? x.n : items_above(p, x, c * width)) - items_above(p, x, (c + 1) * width);
 }
 
-// Item `index` in the order, for key-value head `head`; whole warp.
+// Steps of 128 keys in the items of a class, and the parts that each is cut into.
+__device__ __forceinline__ uint32_t steps_of(uint32_t c, uint32_t width) {
+  return ((c + 1) * width + 127) / 128;
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t c, uint32_t width, uint32_t part) {
+  return part ? (steps_of(c, width) + part - 1) / part : 1;
+}
+
+// Entry `index` of the order, for key-value head `head`; whole warp.
 __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_t index, uint32_t head) {
   const uint32_t lane = threadIdx.x & 31u;
   Item it = {};
@@ -209,7 +257,8 @@ __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_
 #pragma unroll
   for (int i = 0; i < kBuckets / 32; ++i) mine += o.starts[lane * (kBuckets / 32) + i] <= index;
   const int at = static_cast<int>(__reduce_add_sync(0xffffffffu, mine)) - 1;
-  const uint32_t rest = index - o.starts[at], c = kBuckets - 1 - at;
+  const uint32_t c = kBuckets - 1 - at, parts = parts_of(c, o.width, o.part);
+  const uint32_t entry = index - o.starts[at], rest = parts > 1 ? entry / parts : entry;
   if (at != o.bucket || rest < o.before) {
     o.bucket = at;
     o.seq = 0;
@@ -236,6 +285,26 @@ __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_
       it.k_row = static_cast<int32_t>(__shfl_sync(0xffffffffu, x.k0, src));
       it.k_len = static_cast<int32_t>(__shfl_sync(0xffffffffu, x.b, src));
       it.visible = static_cast<int32_t>(__shfl_sync(0xffffffffu, p.causal ? x.b - x.a + t0 + 1 : x.b, src));
+      if (parts > 1) {
+        // this part's steps, as an item of its own over their keys
+        const int which = static_cast<int>(entry % parts), n = static_cast<int>(parts);
+        const int most = p.causal ? min(it.k_len, it.visible + it.q_count - 1) : it.k_len;
+        const int steps = (max(most, 0) + 127) / 128, from = steps * which / n * 128;
+        const int to = which + 1 == n ? it.k_len : min(it.k_len, steps * (which + 1) / n * 128);
+        it.k_row += from;
+        it.k_len = to - from;
+        it.visible -= from;
+        const uint32_t place = index * p.kv_heads + head;
+        it.part = static_cast<int32_t>(place) + 1;
+        if (lane == 0) {
+          Part *w = reinterpret_cast<Part *>(static_cast<uint8_t *>(p.workspace) + 16) + place;
+          w->q_row = it.q_row;
+          w->q_count = it.q_count;
+          w->head = it.head;
+          w->index = which;
+          w->parts = n;
+        }
+      }
       return it;
     }
     o.before += __shfl_sync(0xffffffffu, sum, 31);
@@ -244,18 +313,21 @@ __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_
 }
 
 // What a tile's rows see.
+template <int kKeys>
 struct Reach {
-  int steps;  // of 128 keys
+  int steps;  // of kKeys keys
   int first;  // keys that its first token sees (at least 0)
   int most;   // keys that its last token sees
 };
 // Blocks of 32 keys in step j that some row of the tile sees.
-__device__ __forceinline__ int blocks_of(const Reach &r, int j) {
+template <int kKeys>
+__device__ __forceinline__ int blocks_of(const Reach<kKeys> &r, int j) {
   return min(kKeys / 32, (r.most - j * kKeys + 31) / 32);
 }
-__device__ __forceinline__ Reach reach_of(const Item &it, int tile, int tokens, bool causal) {
+template <int kKeys>
+__device__ __forceinline__ Reach<kKeys> reach_of(const Item &it, int tile, int tokens, bool causal) {
   const int begin = tile * tokens, end = min(it.q_count, begin + tokens);
-  Reach r = {0, 0, 0};
+  Reach<kKeys> r = {0, 0, 0};
   if (begin >= end) return r;
   r.most = causal ? min(it.k_len, it.visible + end - 1) : it.k_len;
   r.first = max(0, causal ? min(it.k_len, it.visible + begin) : it.k_len);
@@ -332,43 +404,59 @@ __device__ __forceinline__ void hand_over_weights(uint64_t *p_full) {
 }
 
 // Scores, weights and sums of one step for this thread's row, through m (reference, log2 units) and
-// sum. Where some row sees the step in part (kMasked), this one sees `vis` keys of it and the tile
-// `blocks` blocks of 32; the products skip the others. The weights are handed over in two halves
-// (p_full[0], p_full[2]), so that the product with V starts under the second.
-template <bool kBf16, bool kMasked>
-__device__ __forceinline__ void softmax_step(uint32_t tl, uint32_t to, int dim, float c, int vis,
-                                             int blocks, bool first, float &m, float &sum,
-                                             uint64_t *p_full) {
-  uint32_t v[4][32];
+// sum. Where some row of the tile sees the step in part (`masked`), this one sees `vis` keys of it
+// and the tile `blocks` blocks of 32; the products skip the others. The weights are handed over in
+// two halves (p_full[0], p_full[2]), so that the product with V starts under the second. One form for
+// both kinds of step: two thrashed the instruction cache. loaded() is called when the scores are in
+// registers, before() before the output or the weights' columns (at tp) are touched.
+template <bool kBf16, int kBlocks, class Loaded, class Before>
+__device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, float c, bool masked,
+                                             int vis, int blocks, bool first, float &m, float &sum,
+                                             uint32_t tp, uint64_t *p_full, Loaded &&loaded,
+                                             Before &&before) {
+  uint32_t v[kBlocks][32];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_ld32(tl + 32 * i, v[i]);  // past `blocks`: old values, not used
+  for (int i = 0; i < kBlocks; ++i) tmem_ld32(tl + 32 * i, v[i]);  // past `blocks`: old values, not used
   tmem_wait_ld(v[0]);
 #pragma unroll
-  for (int i = 1; i < 4; ++i) tmem_regs_ready(v[i]);
-  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  for (int i = 1; i < kBlocks; ++i) tmem_regs_ready(v[i]);
+  loaded();
+  if (masked) {
+    const int least = __reduce_min_sync(0xffffffffu, vis);  // of the warp's rows
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (kMasked && i >= blocks) break;
-    if constexpr (kMasked) {
+    for (int i = 0; i < kBlocks; ++i) {
+      if (least >= 32 * (i + 1)) continue;
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if (32 * i + e >= vis) v[i][e] = 0xff800000u;  // -inf
     }
-#pragma unroll
-    for (int e = 0; e < 32; e += 2)
-      top[i] = max3(top[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
   }
-  move_reference(to, dim, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c, first, m, sum);
+  float tops[kBlocks];
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i) {
+    tops[i] = max3(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]), __uint_as_float(v[i][2]));
+#pragma unroll
+    for (int e = 3; e + 1 < 32; e += 2)
+      tops[i] = max3(tops[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
+    tops[i] = fmaxf(tops[i], __uint_as_float(v[i][31]));
+  }
+  float top = tops[0];
+#pragma unroll
+  for (int i = 1; i < kBlocks; ++i) top = fmaxf(top, tops[i]);
+  if (!before()) return false;
+  move_reference(to, dim, top * c, first, m, sum);
   const float base = m == -INFINITY ? 0.f : m;
   const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
   uint64_t s0 = 0, s1 = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (!kMasked || i < blocks) weigh<kBf16>(tl + 16 * i, v[i], c2, base2, s0, s1);
-    if (i & 1) hand_over_weights(p_full + i - 1);
+  for (int i = 0; i < kBlocks; ++i) {
+    if (i < blocks) weigh<kBf16>(tp + 16 * i, v[i], c2, base2, s0, s1);
+    if (i == kBlocks / 2 - 1) hand_over_weights(p_full);
+    if (i == kBlocks - 1) hand_over_weights(p_full + 2);
   }
   const float2 part = unpair(add2(s0, s1));
   sum += part.x + part.y;
+  return true;
 }
 }  // namespace
 
@@ -380,13 +468,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const __grid_constant__ CUtensorMap tmo,
                             const __grid_constant__ PackedArgs p) {
   using L = Layout<kDim>;
-  constexpr int kStages = L::kStages;
+  constexpr int kStages = L::kStages, kKeys = L::kKeys, kTmemO = L::kTmemO, kTmemCols = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
-  uint64_t *q_empty = q_full + 2, *s_full = q_full + 4, *p_full = q_full + 6, *o_full = q_full + 10;
-  uint64_t *drain = q_full + 12, *sched_full = q_full + 14, *sched_empty = q_full + 17;
-  uint64_t *kv_full = q_full + 20, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages;
+  uint64_t *q_empty = q_full + 2, *s_full = q_full + 4, *s_free = q_full + 6, *p_full = q_full + 8;
+  uint64_t *o_full = q_full + 12, *drain = q_full + 14, *sched_full = q_full + 16, *sched_empty = q_full + 19;
+  uint64_t *kv_full = q_full + 22, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages;
   Item *items = reinterpret_cast<Item *>(smem + L::kItemOff);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kMiscOff);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -399,6 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);  // the tile's softmax warps
       mbar_init(&p_full[i], 4);  // the tile's softmax warps
       mbar_init(&p_full[2 + i], 4);
       mbar_init(&o_full[i], 1);
@@ -427,33 +516,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   for (int i = threadIdx.x; i <= kBuckets; i += kThreads) order[i] = 0;
-  __syncthreads();
-  // The longest sequence sets the classes' width; then each sequence's items in them.
-  uint32_t longest = 0;
-  for (uint32_t s = threadIdx.x; s < p.n_seq; s += kThreads) {
-    const Sequence x = sequence_of(p, s);
-    if (x.n) longest = max(longest, x.b);
-  }
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  if (lane == 0) atomicMax(&order[kBuckets], longest);
-  __syncthreads();
-  const uint32_t width = max(1u, (order[kBuckets] + kBuckets - 1) / kBuckets);
-  // Few sequences: a warp for each, the classes over its lanes; else a thread, over its own classes.
-  if (p.n_seq <= 96) {
-    for (uint32_t s = warp; s < p.n_seq; s += kThreads / 32) {
-      const Sequence x = sequence_of(p, s);
-#pragma unroll
-      for (int i = lane; i < kBuckets; i += 32)
-        if (const uint32_t n = items_in(p, x, i, width)) atomicAdd(&order[kBuckets - 1 - i], n);
-    }
-  } else {
+  uint32_t width = 0x7fffff00u;  // one class
+  if (!p.flat) {
+    __syncthreads();
+    // The longest sequence sets the classes' width; then each sequence's items in them.
+    uint32_t longest = 0;
     for (uint32_t s = threadIdx.x; s < p.n_seq; s += kThreads) {
       const Sequence x = sequence_of(p, s);
-      uint32_t left = x.n;
-      for (int i = min(kBuckets - 1, static_cast<int>(x.b ? (x.b - 1) / width : 0)); left > 0; --i) {
-        const uint32_t n = items_in(p, x, i, width);
-        if (n) atomicAdd(&order[kBuckets - 1 - i], n);
-        left = i > 0 ? left - n : 0;
+      if (x.n) longest = max(longest, x.b);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) atomicMax(&order[kBuckets], longest);
+    __syncthreads();
+    width = max(1u, (order[kBuckets] + kBuckets - 1) / kBuckets);
+    // Few sequences: a warp for each, the classes over its lanes; else a thread, over its own classes.
+    if (p.n_seq <= 96) {
+      for (uint32_t s = warp; s < p.n_seq; s += kThreads / 32) {
+        const Sequence x = sequence_of(p, s);
+#pragma unroll
+        for (int i = lane; i < kBuckets; i += 32)
+          if (const uint32_t n = items_in(p, x, i, width)) atomicAdd(&order[kBuckets - 1 - i], n);
+      }
+    } else {
+      for (uint32_t s = threadIdx.x; s < p.n_seq; s += kThreads) {
+        const Sequence x = sequence_of(p, s);
+        uint32_t left = x.n;
+        for (int i = min(kBuckets - 1, static_cast<int>(x.b ? (x.b - 1) / width : 0)); left > 0; --i) {
+          const uint32_t n = items_in(p, x, i, width);
+          if (n) atomicAdd(&order[kBuckets - 1 - i], n);
+          left = i > 0 ? left - n : 0;
+        }
       }
     }
   }
@@ -465,10 +557,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kGuardWarp) {
     fewer_registers();
-    Order o = {order, 0, width, -1, 0, 0};
-    {  // counts to starts
-      const uint32_t n0 = order[2 * lane], n1 = order[2 * lane + 1];
+    Order o = {order, 0, width, 0, -1, 0, 0};
+    if (!p.flat) {  // counts to starts
       static_assert(kBuckets == 64, "two classes a lane");
+      uint32_t n0 = order[2 * lane], n1 = order[2 * lane + 1];
+      const uint32_t c0 = kBuckets - 1 - 2 * lane, c1 = c0 - 1;
+      auto sum_of = [](uint64_t x) {
+#pragma unroll
+        for (int i = 16; i > 0; i /= 2) x += __shfl_xor_sync(0xffffffffu, x, i);
+        return x;
+      };
+      if (p.parts_max) {
+        const uint64_t steps = sum_of(static_cast<uint64_t>(n0) * steps_of(c0, width) +
+                                      static_cast<uint64_t>(n1) * steps_of(c1, width)) * p.kv_heads;
+        uint64_t cut;
+        o.part = max(4u, static_cast<uint32_t>((steps * 3 / 2 + gridDim.x - 1) / gridDim.x));
+        while (true) {  // until the parts fit the workspace
+          const uint32_t p0 = parts_of(c0, width, o.part), p1 = parts_of(c1, width, o.part);
+          cut = sum_of((p0 > 1 ? static_cast<uint64_t>(n0) * p0 : 0) + (p1 > 1 ? static_cast<uint64_t>(n1) * p1 : 0)) * p.kv_heads;
+          if (cut <= p.parts_max) break;
+          o.part += o.part / 4 + 1;
+        }
+        if (blockIdx.x == 0 && lane == 0) *Parts<kDim>::of(p.workspace, p.parts_max).count = static_cast<uint32_t>(cut);
+        n0 *= parts_of(c0, width, o.part);
+        n1 *= parts_of(c1, width, o.part);
+      }
       uint32_t sum = n0 + n1;
 #pragma unroll
       for (int i = 1; i < 32; i *= 2) {
@@ -481,7 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       order[2 * lane + 1] = sum - n1;
       __syncwarp();
     }
-    const uint64_t n_items = static_cast<uint64_t>(o.total) * p.kv_heads;
+    // flat: as many items as CTAs at most, whatever their number
+    const uint64_t n_items = p.flat ? gridDim.x : static_cast<uint64_t>(o.total) * p.kv_heads;
     bool ok = true;
     // Publish item k of this CTA: up the order and down again in turn, so that no CTA always gets
     // the longest of each round.
@@ -492,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (at < n_items)
         it = find_item(p, o, static_cast<uint32_t>(at / p.kv_heads), static_cast<uint32_t>(at % p.kv_heads));
       // the up-and-down order may leave one CTA an item in a round in which others have none
-      it.last = static_cast<uint64_t>(k) * gridDim.x >= n_items;
+      if (static_cast<uint64_t>(k) * gridDim.x >= n_items) it.part = -1;
       ok = __all_sync(0xffffffffu, mbar_wait(&sched_empty[k % 3], ((k / 3) & 1) ^ 1u, abort_flag));
       if (ok && lane == 0) {
         volatile Item *d = &items[k % 3];
@@ -502,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         d->k_len = it.k_len;
         d->visible = it.visible;
         d->head = it.head;
-        d->last = it.last;
+        d->part = it.part;
         d->fix = 0;
         mbar_arrive(&sched_full[k % 3]);
       }
@@ -513,11 +627,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       *abort_flag = 1;
     }
     uint32_t ring = 0, phase = 0, v_ring = 0;
-    Item it = publish(0);
-    for (uint32_t k = 0; ok && !it.last; ++k) {
-      const Item next = publish(k + 1);
+    Item it = {};  // nothing before the first
+    for (uint32_t k = 0; ok && it.part >= 0; ++k) {
+      const Item next = publish(k);
       if (!ok) break;
-      const Reach r0 = reach_of(it, 0, tokens, p.causal), r1 = reach_of(it, 1, tokens, p.causal);
+      const Reach<kKeys> r0 = reach_of<kKeys>(it, 0, tokens, p.causal), r1 = reach_of<kKeys>(it, 1, tokens, p.causal);
       const int steps = max(r0.steps, r1.steps), partial = r0.first / kKeys;
       for (int j = 0; j < steps; ++j) {
         if (++ring == kStages) ring = 0, phase ^= 1;  // the step's K stage
@@ -526,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j >= partial) {
           uint4 *x = reinterpret_cast<uint4 *>(smem + L::kRingOff + ring * L::kTileBytes);
           uint32_t acc = 0;
-#pragma unroll 8
+#pragma unroll 4
           for (int i = lane; i < L::kTileBytes / 16; i += 32) {
             const uint4 w = x[i];
             acc = times_zero<kBf16>(w.x, acc);
@@ -545,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               x[i] = w;
             }
-            *reinterpret_cast<volatile int32_t *>(&items[k % 3].fix) = 1;
+            *reinterpret_cast<volatile int32_t *>(&items[(k - 1) % 3].fix) = 1;
             fence_proxy_async_smem();
           }
         }
@@ -575,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(&q_full[t], p.tokens * p.group * 128u * L::kHalves);
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
-            tma_load_3d(smem + t * L::kTileBytes + h * L::kHalfBytes, &tmq, &q_full[t], 64 * h,
+            tma_load_3d(smem + t * L::kQBytes + h * L::kQHalf, &tmq, &q_full[t], 64 * h,
                         it.head * static_cast<int>(p.group), it.q_row + t * tokens);
           q_armed[t] = true;
           q_due[t] = false;
@@ -600,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive_expect_tx(&kv_full[ring], L::kTileBytes);
 #pragma unroll
         for (int h = 0; h < L::kHalves; ++h)
-          tma_load_3d(dst + h * L::kHalfBytes, map, &kv_full[ring], 64 * h, head, row);
+          tma_load_3d(dst + h * L::kTileHalf, map, &kv_full[ring], 64 * h, head, row);
         armed |= 1u << ring;
         parity = (parity & ~(1u << ring)) | (phase << ring);
         if (++ring == kStages) ring = 0, phase ^= 1;
@@ -611,8 +725,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         it = read_item(&items[k % 3]);
         mbar_arrive(&sched_empty[k % 3]);
-        if (it.last) break;
-        const Reach r[2] = {reach_of(it, 0, tokens, p.causal), reach_of(it, 1, tokens, p.causal)};
+        if (it.part < 0) break;
+        const Reach<kKeys> r[2] = {reach_of<kKeys>(it, 0, tokens, p.causal), reach_of<kKeys>(it, 1, tokens, p.causal)};
         const int steps = max(r[0].steps, r[1].steps);
         q_due[0] = r[0].steps > 0;
         q_due[1] = r[1].steps > 0;
@@ -639,8 +753,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = warp - kMmaWarp;
       constexpr uint32_t idesc_s = idesc_f32(kBf16, 128, 0, false);  // N to come: 32 a block
       constexpr uint32_t idesc_o = idesc_f32(kBf16, 128, kDim, true);
-      const uint32_t d_s = tmem + t * 128, d_o = tmem + kTmemO + t * 128;
-      const uint32_t q_at = smem_u32(smem + t * L::kTileBytes);
+      const uint32_t d_s = tmem + t * kKeys, d_o = tmem + kTmemO + t * kDim, p_at = tmem + L::kTmemP + t * L::kTmemPStep;
+      const uint32_t q_at = smem_u32(smem + t * L::kQBytes);
       uint32_t ring = 0, phase = 0, v_ring = 0, v_phase = 0, p_phase = 0, q_phase = 0;
       bool ok = true;
       // One tile at a time puts its products on the tensor cores. Left to interleave, both tiles'
@@ -658,17 +772,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto give = [&] { *reinterpret_cast<volatile uint32_t *>(turn) = 0u; };
-      // S = Q K^T of stage `stage`, the last of a turn.
+      // S = Q K^T of stage `stage`.
       auto scores = [&](uint32_t stage, int blocks) {
         const uint32_t idesc = idesc_s | static_cast<uint32_t>(blocks * 32 / 8) << 17;
         tc_fence_after();
         const uint32_t k_at = smem_u32(smem + L::kRingOff + stage * L::kTileBytes);
 #pragma unroll
         for (int kk = 0; kk < kDim / 16; ++kk) {
-          const uint32_t off = (kk / 4) * L::kHalfBytes + (kk % 4) * 32;
-          umma_f16(d_s, sw128_desc(q_at + off), sw128_desc(k_at + off), idesc, kk > 0);
+          const uint32_t in = (kk % 4) * 32;
+          umma_f16(d_s, sw128_desc(q_at + (kk / 4) * L::kQHalf + in),
+                   sw128_desc(k_at + (kk / 4) * L::kTileHalf + in), idesc, kk > 0);
         }
-        give();
       };
       // One commit, for the softmax, covers the scores and all before: the softmax releases the
       // stages when it sees it (a commit holds the issuing thread about 100 cycles).
@@ -676,20 +790,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit(&s_full[t]);
         if (last) umma_commit(&q_empty[t]);
       };
-      // Half of O += P V; of a step with fewer than four blocks of 32 keys only theirs.
+      // Half of O += P V; of a step that is seen in part only the blocks of 32 keys that are.
       auto product = [&](uint32_t v_at, int half, bool first, int blocks) {
         tc_fence_after();
-        if (blocks == 4) {
+        constexpr int kHalf = kKeys / 32;  // products of 16 keys in half a step
+        if (blocks == L::kBlocks) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int kk = half * 4 + i;
-            umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
+          for (int i = 0; i < kHalf; ++i) {
+            const int kk = half * kHalf + i;
+            umma_f16_ts(d_o, p_at + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kTileHalf), idesc_o,
                         !first || kk > 0);
           }
         } else {
 #pragma unroll 1
-          for (int kk = half * 4; kk < min(2 * blocks, half * 4 + 4); ++kk)
-            umma_f16_ts(d_o, d_s + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kHalfBytes), idesc_o,
+          for (int kk = half * kHalf; kk < min(2 * blocks, half * kHalf + kHalf); ++kk)
+            umma_f16_ts(d_o, p_at + 8 * kk, sw128_mn_desc(v_at + kk * 2048, L::kTileHalf), idesc_o,
                         !first || kk > 0);
         }
       };
@@ -698,63 +813,113 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const Item it = read_item(&items[k % 3]);
         mbar_arrive(&sched_empty[k % 3]);
-        if (it.last) break;
-        const Reach reach = reach_of(it, t, tokens, p.causal);
+        if (it.part < 0) break;
+        const Reach<kKeys> reach = reach_of<kKeys>(it, t, tokens, p.causal);
         const int mine = reach.steps;
-        const int steps = max(mine, reach_of(it, 1 - t, tokens, p.causal).steps);
+        const int steps = max(mine, reach_of<kKeys>(it, 1 - t, tokens, p.causal).steps);
         if (steps == 0) continue;
-        uint32_t k_stage = ring;
-        ok = mbar_wait(&kv_full[ring], phase, abort_flag);
-        if (!ok) break;
-        if (++ring == kStages) ring = 0, phase ^= 1;
-        if (mine > 0) {
-          ok = mbar_wait(&q_full[t], q_phase, abort_flag) && take();
-          if (!ok) break;
-          q_phase ^= 1;
-          scores(k_stage, blocks_of(reach, 0));
-          hand_over(mine == 1);
-        } else {
-          mbar_arrive(&kv_empty[k_stage]);
-        }
-        for (int j = 0; j < steps; ++j) {
-          // this step's V, and the next step's K behind it
-          const uint32_t v_stage = ring;
-          ok = mbar_wait(&kv_full[ring], phase, abort_flag) && mbar_wait(&v_ok[v_ring], v_phase, abort_flag);
-          if (!ok) break;
-          if (++v_ring == kStages) v_ring = 0, v_phase ^= 1;
-          if (++ring == kStages) ring = 0, phase ^= 1;
-          const bool more = j + 1 < steps;
-          if (more) {
-            k_stage = ring;
-            ok = mbar_wait(&kv_full[ring], phase, abort_flag);
+        if constexpr (L::kOwnP) {
+          // The item's nth stage, K and V in turn, counted over all items.
+          auto wait_stage = [&](uint32_t n) {
+            return mbar_wait(&kv_full[n % kStages], n / kStages & 1, abort_flag);
+          };
+          for (int j = -1; j < steps; ++j) {
+            // the next step's scores, once the softmax has this one's in registers
+            if (j + 1 < steps) {
+              const uint32_t n = ring + 2 * (j + 1);
+              ok = wait_stage(n);
+              if (!ok) break;
+              if (j + 1 < mine) {
+                if (j < 0) {
+                  ok = mbar_wait(&q_full[t], q_phase, abort_flag);
+                  q_phase ^= 1;
+                }
+                ok = ok && mbar_wait(&s_free[t], phase ^ 1u, abort_flag);
+                if (!ok) break;
+                phase ^= 1;
+                scores(n % kStages, blocks_of(reach, j + 1));
+                hand_over(j + 2 == mine);
+              } else {
+                mbar_arrive(&kv_empty[n % kStages]);
+              }
+            }
+            if (j < 0) continue;
+            const uint32_t n = ring + 2 * j + 1;
+            ok = wait_stage(n) && mbar_wait(&v_ok[v_ring], v_phase, abort_flag);
             if (!ok) break;
-            if (++ring == kStages) ring = 0, phase ^= 1;
-          }
-          if (j >= mine) {
-            mbar_arrive(&kv_empty[v_stage]);
-            if (more) mbar_arrive(&kv_empty[k_stage]);
-            continue;
-          }
-          const uint32_t v_at = smem_u32(smem + L::kRingOff + v_stage * L::kTileBytes);
-          ok = mbar_wait(&p_full[t], p_phase, abort_flag) && take();
-          if (!ok) break;
-          const int blocks = blocks_of(reach, j);
-          product(v_at, 0, j == 0, blocks);
-          // where the second half is there by now, the turn is kept
-          if (!mbar_test(&p_full[2 + t], p_phase)) {
-            give();
-            ok = mbar_wait(&p_full[2 + t], p_phase, abort_flag) && take();
+            if (++v_ring == kStages) v_ring = 0, v_phase ^= 1;
+            if (j >= mine) {
+              mbar_arrive(&kv_empty[n % kStages]);
+              continue;
+            }
+            const uint32_t v_at = smem_u32(smem + L::kRingOff + n % kStages * L::kTileBytes);
+            const int blocks = blocks_of(reach, j);
+            ok = mbar_wait(&p_full[t], p_phase, abort_flag);
             if (!ok) break;
-          }
-          p_phase ^= 1;
-          product(v_at, 1, j == 0, blocks);
-          if (j + 1 < mine) {
-            scores(k_stage, blocks_of(reach, j + 1));
-            hand_over(j + 2 == mine);
-          } else {
-            give();
+            product(v_at, 0, j == 0, blocks);
+            ok = mbar_wait(&p_full[2 + t], p_phase, abort_flag);
+            if (!ok) break;
+            p_phase ^= 1;
+            product(v_at, 1, j == 0, blocks);
             umma_commit(&o_full[t]);
-            if (more) mbar_arrive(&kv_empty[k_stage]);
+          }
+          ring += 2 * steps;
+        } else {
+          uint32_t k_stage = ring;
+          ok = mbar_wait(&kv_full[ring], phase, abort_flag);
+          if (!ok) break;
+          if (++ring == kStages) ring = 0, phase ^= 1;
+          if (mine > 0) {
+            ok = mbar_wait(&q_full[t], q_phase, abort_flag) && take();
+            if (!ok) break;
+            q_phase ^= 1;
+            scores(k_stage, blocks_of(reach, 0));
+            give();
+            hand_over(mine == 1);
+          } else {
+            mbar_arrive(&kv_empty[k_stage]);
+          }
+          for (int j = 0; j < steps; ++j) {
+            // this step's V, and the next step's K behind it
+            const uint32_t v_stage = ring;
+            ok = mbar_wait(&kv_full[ring], phase, abort_flag) && mbar_wait(&v_ok[v_ring], v_phase, abort_flag);
+            if (!ok) break;
+            if (++v_ring == kStages) v_ring = 0, v_phase ^= 1;
+            if (++ring == kStages) ring = 0, phase ^= 1;
+            const bool more = j + 1 < steps;
+            if (more) {
+              k_stage = ring;
+              ok = mbar_wait(&kv_full[ring], phase, abort_flag);
+              if (!ok) break;
+              if (++ring == kStages) ring = 0, phase ^= 1;
+            }
+            if (j >= mine) {
+              mbar_arrive(&kv_empty[v_stage]);
+              if (more) mbar_arrive(&kv_empty[k_stage]);
+              continue;
+            }
+            const uint32_t v_at = smem_u32(smem + L::kRingOff + v_stage * L::kTileBytes);
+            ok = mbar_wait(&p_full[t], p_phase, abort_flag) && take();
+            if (!ok) break;
+            const int blocks = blocks_of(reach, j);
+            product(v_at, 0, j == 0, blocks);
+            // where the second half is there by now, the turn is kept
+            if (!mbar_test(&p_full[2 + t], p_phase)) {
+              give();
+              ok = mbar_wait(&p_full[2 + t], p_phase, abort_flag) && take();
+              if (!ok) break;
+            }
+            p_phase ^= 1;
+            product(v_at, 1, j == 0, blocks);
+            if (j + 1 < mine) {
+              scores(k_stage, blocks_of(reach, j + 1));
+              give();
+              hand_over(j + 2 == mine);
+            } else {
+              give();
+              umma_commit(&o_full[t]);
+              if (more) mbar_arrive(&kv_empty[k_stage]);
+            }
           }
         }
       }
@@ -771,62 +936,87 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row = q * 32 + lane;
     const int token = row / static_cast<int>(p.group), sub = row % static_cast<int>(p.group);
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t tl = tmem + lanes + t * 128, to = tmem + lanes + kTmemO + t * 128;
+    const uint32_t tl = tmem + lanes + t * kKeys, to = tmem + lanes + kTmemO + t * kDim;
     const float c = p.scale_log2;
     uint8_t *stage = smem + L::kOutOff + warp * L::kOutBytes;
+    const uint32_t tp = L::kOwnP ? tmem + lanes + L::kTmemP + t * L::kTmemPStep : tl;
     uint32_t s_phase = 0, o_phase = 0, ring = 0;
-    // Release the stage at `ring`, for this tile, once its last product with it is known to be done.
-    auto release = [&] {
-      if (q == 0 && lane == 0) mbar_arrive(&kv_empty[ring]);
-      if (++ring == kStages) ring = 0;
+    // Release the item's nth stage (K and V in turn), for this tile, when its last product with it is
+    // known to be done.
+    auto release = [&](int n) {
+      if (q == 0 && lane == 0) mbar_arrive(&kv_empty[(ring + n) % kStages]);
     };
     bool ok = true;
     for (uint32_t k = 0; ok; ++k) {
       ok = __all_sync(0xffffffffu, mbar_wait(&sched_full[k % 3], (k / 3) & 1, abort_flag));
       if (!ok) break;
-      const Item it = read_item(&items[k % 3]);
+      const Item seen = read_item(&items[k % 3]);
       __syncwarp();
-      const Reach r = reach_of(it, t, tokens, p.causal);
+      const Reach<kKeys> r = reach_of<kKeys>(seen, t, tokens, p.causal);
       const int whole = r.first / kKeys;  // steps that every row of the tile sees in full
       const int mine = t * tokens + token;  // token within the item
-      const int sees = p.causal ? min(it.k_len, it.visible + mine) : it.k_len;
+      const int sees = p.causal ? min(seen.k_len, seen.visible + mine) : seen.k_len;
       float m = -INFINITY, sum = 0.f;
       for (int j = 0; j < r.steps; ++j) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], s_phase, abort_flag));
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after();
-        if (j > 0) release();  // the previous step's V
-        release();             // this step's K
-        if (j < whole)
-          softmax_step<kBf16, false>(tl, to, kDim, c, kKeys, 4, j == 0, m, sum, &p_full[t]);
-        else
-          softmax_step<kBf16, true>(tl, to, kDim, c, sees - j * kKeys, blocks_of(r, j), j == 0, m, sum,
-                                    &p_full[t]);
+        const bool masked = j >= whole;
+        auto step = [&](auto &&loaded, auto &&before) {
+          return softmax_step<kBf16, L::kBlocks>(tl, to, kDim, c, masked, sees - j * kKeys,
+                                                 masked ? blocks_of(r, j) : L::kBlocks, j == 0, m, sum,
+                                                 tp, &p_full[t], loaded, before);
+        };
+        if constexpr (L::kOwnP) {
+          release(2 * j);  // this step's K
+          ok = step(
+              [&] {  // S may be overwritten
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[t]);
+              },
+              [&] {  // the product of the step before is done: its V, P and O are free
+                if (j == 0) return true;
+                if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag))) return false;
+                o_phase ^= 1;
+                tc_fence_after();
+                release(2 * j - 1);
+                return true;
+              });
+          if (!ok) break;
+        } else {
+          if (j > 0) release(2 * j - 1);  // the previous step's V
+          release(2 * j);                 // this step's K
+          step([] {}, [] { return true; });
+        }
       }
       if (!ok) break;
-      // Where the row goes, worked out under the last product.
+      // Where the row goes, worked out under the last product (the item read again: its registers are
+      // the scores' meanwhile).
+      const Item it = read_item(&items[k % 3]);
       const bool live = token < tokens && mine < it.q_count;
       const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
       const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
       uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
-      if (live && p.lse) p.lse[out_row * p.q_heads + head] = (m + log2f(sum)) * kLn2;
+      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = (m + log2f(sum)) * kLn2;
       if (r.steps > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag));
         if (!ok) break;
         o_phase ^= 1;
         tc_fence_after();
-        release();
+        release(2 * r.steps - 1);
       }
       // the issuer releases the stages of steps that only the other tile has
-      ring = (ring + 2 * (max(r.steps, reach_of(it, 1 - t, tokens, p.causal).steps) - r.steps)) % kStages;
+      ring = (ring + 2 * max(r.steps, reach_of<kKeys>(it, 1 - t, tokens, p.causal).steps)) % kStages;
       const int fix = r.steps > 0 ? *reinterpret_cast<volatile int32_t *>(&items[k % 3].fix) : 0;
       __syncwarp();
       // From here on the slot is not read again; the next item but two may be written into it.
       if (lane == 0) mbar_arrive(&sched_empty[k % 3]);
-      if (it.last) break;
+      if (it.part < 0) break;
+      if (rows_live == 0) continue;
       // 64 channels at a time through this warp's staging (16-byte chunk c of row r at c ^ (r & 7)):
       // by one TMA store where all 32 rows are of the sequence and whole tokens, else 8 lanes to a
       // row of 128 bytes.
@@ -846,7 +1036,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (fix && live) {
             // what the guard took out of the steps that are seen in part
-            const int from = reach_of(it, 0, tokens, p.causal).first / kKeys * kKeys;
+            const int from = reach_of<kKeys>(it, 0, tokens, p.causal).first / kKeys * kKeys;
 #pragma unroll 1
             for (int kk = from; kk < sees; ++kk) {
               const uint32_t *v = reinterpret_cast<const uint32_t *>(
@@ -860,6 +1050,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
+          if (it.part > 0) {  // a part: as it is
+            const Parts<kDim> to_join = Parts<kDim>::of(p.workspace, p.parts_max);
+            const size_t tile = static_cast<size_t>(it.part - 1) * 2 + t;
+            if (live) {
+              if (d + half == 0) to_join.ml[tile * 128 + row] = make_float2(m, sum);
+              float4 *o = to_join.o + (tile * (kDim / 4) + (d + 32 * half) / 4) * 128 + row;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                o[e * 128] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
+                                         __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+            }
+            continue;
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t w[4];
@@ -870,7 +1073,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        if (boxed) {
+        if (it.part > 0) {
+        } else if (boxed) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -908,6 +1112,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Joins the parts of the cut items: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the parts in
+// order. The CTAs of a part take its share of the item's rows, 16 channels each: a thread for a row and
+// four channels, rows next to one another.
+template <bool kBf16, int kDim>
+__global__ void __launch_bounds__(256) attention_packed_join_kernel(const PackedArgs p) {
+  pdl_wait();
+  const Parts<kDim> w = Parts<kDim>::of(p.workspace, p.parts_max);
+  if (blockIdx.x >= *w.count) return;
+  const Part part = w.what[blockIdx.x];
+  // the item's parts stand kv_heads apart
+  const uint32_t first = blockIdx.x - part.index * p.kv_heads;
+  const int from = 256 * part.index / part.parts, rows = 256 * (part.index + 1) / part.parts - from;
+  for (int x = threadIdx.x; x < rows * 4; x += 256) {
+    const int row = from + x % rows, d4 = blockIdx.y * 4 + x / rows;
+    const int t = row / 128, in = row % 128, token = in / static_cast<int>(p.group);
+    const int mine = t * static_cast<int>(p.tokens) + token;
+    if (token >= static_cast<int>(p.tokens) || mine >= part.q_count) continue;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < part.parts; ++i)
+      top = fmaxf(top, w.ml[(static_cast<size_t>(first) + i * p.kv_heads) * 256 + row].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < part.parts; ++i) {
+      const size_t at = static_cast<size_t>(first) + i * p.kv_heads;
+      const float2 ml = w.ml[at * 256 + row];
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // sees none of the part's keys
+      const float f = top == -INFINITY ? 1.f : ex2_approx(ml.x - top);
+      const float4 v = w.o[((at * 2 + t) * (kDim / 4) + d4) * 128 + in];
+      sum = fmaf(ml.y, f, sum);
+      acc.x = fmaf(v.x, f, acc.x);
+      acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z);
+      acc.w = fmaf(v.w, f, acc.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t out_row = static_cast<int64_t>(part.q_row) + mine;
+    const uint32_t head = part.head * p.group + in % p.group;
+    *reinterpret_cast<uint2 *>(p.out + out_row * p.out_token + head * p.out_head + 4 * d4) =
+        make_uint2(Elem<kBf16>::pack(acc.x * inv, acc.y * inv), Elem<kBf16>::pack(acc.z * inv, acc.w * inv));
+    if (p.lse && d4 == 0) p.lse[out_row * p.q_heads + head] = (top + log2f(sum)) * kLn2;
+  }
+}
+
 namespace {
 template <bool kBf16, int kDim>
 cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v,
@@ -923,23 +1171,58 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
   }
   attention_packed_kernel<kBf16, kDim>
       <<<dim3(grid), dim3(kThreads), Layout<kDim>::kBytes, stream>>>(q, k, v, o, a);
-  return cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.parts_max == 0) return e;
+  return launch_pdl(attention_packed_join_kernel<kBf16, kDim>, dim3(a.parts_max, kDim / 16), dim3(256), 0, stream, a);
+}
+
+// What the host can tell of a call's items.
+struct Items {
+  uint32_t tokens;     // of a tile
+  uint64_t most;       // items at most: one partly filled one per sequence
+  uint32_t parts_max;  // see PackedArgs
+};
+Items items_of(const PackedAttention &p, uint32_t sms) {
+  Items x;
+  x.tokens = 128 / (p.q_heads / p.kv_heads);
+  x.most = ((static_cast<uint64_t>(p.total_q) + 2 * x.tokens - 1) / (2 * x.tokens) + p.n_seq) * p.kv_heads;
+  // Items are cut where they may be few (fewer than four a CTA: beyond, an uneven end is short beside
+  // the whole) and long (more than 8 steps, and sequences of more than 4 on average: a join that has
+  // nothing to do costs a short call 2.5 us). A part costs its own start and end and 133 KB of partial
+  // results at 128 channels, so there are two for each CTA at most.
+  x.parts_max = x.most < 4ull * sms && p.total_k > 8 * 128 && p.total_k / p.n_seq > 4 * 128 ? 2 * sms : 0;
+  return x;
 }
 }  // namespace
+
+size_t attention_packed_workspace(const PackedAttention &p) {
+  if (p.total_q == 0 || p.n_seq == 0) return 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint32_t parts = items_of(p, static_cast<uint32_t>(sm_count(dev))).parts_max;
+  if (parts == 0) return 0;
+  return p.head_dim == 64 ? Parts<64>::bytes(parts) : Parts<128>::bytes(parts);
+}
 
 cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,
                                     std::string *err) {
   if (p.total_q == 0 || p.n_seq == 0) return cudaSuccess;
-  const uint32_t group = p.q_heads / p.kv_heads, tokens = 128 / group;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint32_t sms = static_cast<uint32_t>(sm_count(dev));
+  const Items items = items_of(p, sms);
+  const uint32_t group = p.q_heads / p.kv_heads, tokens = items.tokens;
   CUtensorMap q, k, v, o;
   const bool boxed = 32 % group == 0;
+  constexpr uint32_t keys = Layout<64>::kKeys;
+  static_assert(Layout<64>::kKeys == Layout<128>::kKeys, "one box");
   const bool maps =
       encode_map_rows(&q, p.q, bf16, p.head_dim, p.q_heads, p.total_q, p.q_head, p.q_token, group, tokens, err) &&
       // without keys the maps stand on q: no load reads through them
       encode_map_rows(&k, p.total_k ? p.k : p.q, bf16, p.head_dim, p.kv_heads, p.total_k ? p.total_k : 1, p.k_head,
-                      p.k_token, 1, kKeys, err) &&
+                      p.k_token, 1, keys, err) &&
       encode_map_rows(&v, p.total_k ? p.v : p.q, bf16, p.head_dim, p.kv_heads, p.total_k ? p.total_k : 1, p.v_head,
-                      p.v_token, 1, kKeys, err) &&
+                      p.v_token, 1, keys, err) &&
       encode_map_rows(&o, p.out, bf16, p.head_dim, p.q_heads, p.total_q, p.out_head, p.out_token,
                       boxed ? group : 1, boxed ? 32 / group : 1, err);
   if (!maps) return cudaErrorInvalidValue;
@@ -965,13 +1248,10 @@ cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStr
   a.boxed = boxed;
   a.causal = p.causal;
   a.scale_log2 = p.scale * kLog2e;
-  const uint64_t levels = (static_cast<uint64_t>(p.total_q) + 2 * tokens - 1) / (2 * tokens);
-  int dev = 0;
-  cudaGetDevice(&dev);
-  // at most one partly filled item per sequence
-  const uint64_t most = (levels + p.n_seq) * p.kv_heads;
-  const uint32_t sms = static_cast<uint32_t>(sm_count(dev));
-  const uint32_t grid = most < sms ? static_cast<uint32_t>(most) : sms;
+  a.parts_max = items.parts_max;
+  a.workspace = p.workspace;
+  a.flat = !items.parts_max && items.most <= sms;
+  const uint32_t grid = items.parts_max || items.most > sms ? sms : static_cast<uint32_t>(items.most);
   if (p.head_dim == 64)
     return bf16 ? launch<true, 64>(q, k, v, o, a, dev, grid, stream) : launch<false, 64>(q, k, v, o, a, dev, grid, stream);
   return bf16 ? launch<true, 128>(q, k, v, o, a, dev, grid, stream) : launch<false, 128>(q, k, v, o, a, dev, grid, stream);

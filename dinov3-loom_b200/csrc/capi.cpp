@@ -607,7 +607,8 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
   if (a->total_q == 0 || a->n_seq == 0) return DV3_OK;
   if (!a->q || !a->out || !a->cu_q || !a->cu_k || (a->total_k > 0 && (!a->k || !a->v)))
     return bad_args("null tensor");
-  if (!all_aligned(a->q, a->k, a->v, a->out)) return bad_args("pointers must be 16-byte aligned");
+  if (!all_aligned(a->q, a->k, a->v, a->out, a->workspace))
+    return bad_args("pointers must be 16-byte aligned");
   dv3::PackedAttention p = {};
   p.q = static_cast<const uint16_t *>(a->q);
   p.k = static_cast<const uint16_t *>(a->k);
@@ -633,11 +634,27 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
   p.scale = a->scale;
+  p.workspace = a->workspace;
+  if (const size_t need = dv3::attention_packed_workspace(p);
+      need > 0 && (!a->workspace || a->workspace_bytes < need))
+    return bad_args("workspace must hold dv3k_attention_packed_workspace bytes");
   std::string err;
   const cudaError_t e = dv3::launch_attention_packed(p, a->dtype == DV3K_BF16,
                                                      static_cast<cudaStream_t>(stream), &err);
   if (!err.empty()) return bad_args(err.c_str());
   return launch_status(e, "attention_packed");
+}
+
+size_t dv3k_attention_packed_workspace(const dv3k_packed_attention *a) {
+  if (!a || check_heads(a->q_heads, a->kv_heads, a->head_dim, DV3K_F16) || a->q_heads == 0) return 0;
+  dv3::PackedAttention p = {};
+  p.n_seq = a->n_seq;
+  p.total_q = a->total_q;
+  p.total_k = a->total_k;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  return dv3::attention_packed_workspace(p);
 }
 
 int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {

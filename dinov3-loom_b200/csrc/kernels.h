@@ -202,7 +202,9 @@ struct PackedAttention {
   uint32_t n_seq, total_q, total_k, q_heads, kv_heads, head_dim;
   bool causal;
   float scale;
+  void *workspace;
 };
+size_t attention_packed_workspace(const PackedAttention &p);  // bytes, on the current device
 // cudaErrorInvalidValue with *err set where a tensor map cannot be built.
 cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,
                                     std::string *err);

@@ -96,6 +96,7 @@ SIGNATURES = {
     "dv3k_attention_packed": ([ctypes.c_char_p, _P], _I),
     "dv3k_rope_append": ([ctypes.c_char_p, _P], _I),
     "dv3k_attention_paged": ([ctypes.c_char_p, _P], _I),
+    "dv3k_attention_packed_workspace": ([ctypes.c_char_p], _SZ),
     "dv3k_attention_paged_workspace": ([ctypes.c_char_p], _SZ),
     "dv3k_gateup_source_row": ([_U32], _U32),
     "dv3k_bounded_wait_selftest": ([ctypes.c_uint64, _P, _P], _I),

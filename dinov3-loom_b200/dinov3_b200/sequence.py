@@ -8,8 +8,8 @@ face of dv3k_attention_packed, dv3k_rope_append and dv3k_attention_paged
     out = attention_paged(q, k_cache, v_cache, page_table, lens)   # one new token per sequence
 
 The calls are asynchronous on torch's current stream of the tensors' device (which need not be the
-current device), can be captured into a CUDA graph, and allocate only what they return (and
-attention_paged its scratch, unless it is given) through torch's allocator. They compute no
+current device), can be captured into a CUDA graph, and allocate only what they return (and the
+attentions their scratch, unless it is given) through torch's allocator. They compute no
 gradients: a tensor that wants one is refused. What does not fit raises DINOv3Error
 (INVALID_ARGUMENT) before anything is launched. `status` is an optional int32 CUDA tensor of two
 words, cleared and read by the caller, that collects what only the device sees (bad pages and
@@ -33,17 +33,19 @@ def _refuse(message: str):
     raise DINOv3Error(INVALID_ARGUMENT, message)
 
 
-_names = ("dv3k_attention_packed", "dv3k_rope_append", "dv3k_attention_paged", "dv3k_attention_paged_workspace")
+_names = ("dv3k_attention_packed", "dv3k_attention_packed_workspace", "dv3k_rope_append", "dv3k_attention_paged",
+          "dv3k_attention_paged_workspace")
 _sequence.bind(*(ctypes.cast(getattr(_lib.load(), n), ctypes.c_void_p).value for n in _names), _refuse, _check)
 
 
-def attention_packed(q, k, v, cu_q, cu_k=None, *, causal=False, scale=None, out=None, lse=None, status=None):
+def attention_packed(q, k, v, cu_q, cu_k=None, *, causal=False, scale=None, out=None, lse=None, workspace=None, status=None):
     """Attention of packed sequences (dv3k_attention_packed) -> out [total_q, q_heads, dim].
 
     q [total_q, q_heads, dim]; k, v [total_k, kv_heads, dim]; cu_q, cu_k int32 [n_seq + 1] (cu_k None:
     cu_q). scale defaults to dim ** -0.5. `out` may be given; rows outside the sequences are left as
-    they were. `lse`, float32 [total_q, q_heads], is filled where given."""
-    return _sequence.attention_packed(q, k, v, cu_q, cu_k, causal, scale, out, lse, status)
+    they were. `lse`, float32 [total_q, q_heads], is filled where given. `workspace`: a uint8 tensor of
+    dv3k_attention_packed_workspace's size to use instead of a new one."""
+    return _sequence.attention_packed(q, k, v, cu_q, cu_k, causal, scale, out, lse, workspace, status)
 
 
 def rope_append(q, k, v, k_cache, v_cache, page_table, lens, cos=None, sin=None, *, cu_new=None, q_out=None, status=None):

@@ -225,19 +225,26 @@ enum { DV3K_F16 = 0, DV3K_BF16 = 1 };
  *   out[i][h] = sum_j w_ij v[j][g] / sum_j w_ij,  w_ij = exp(scale (q[i][h] . k[j][g] - max_j)),
  * over the sequence's keys j < b, where causal over j <= i + b - a of them (a queries, b keys: the
  * last query sees the last key). A row that sees no key gets 0, and -inf in lse. lse (f32
- * [total_q][q_heads], optional) gets log sum_j exp(scale q . k_j). scale > 0. */
+ * [total_q][q_heads], optional) gets log sum_j exp(scale q . k_j). scale > 0.
+ *   - workspace: dv3k_attention_packed_workspace(args) bytes on the current device (0 unless few
+ *     queries may see many keys; NULL will do then), 16-byte aligned, scratch of this call. Calls that
+ *     may overlap on the GPU (on two streams, or in two graphs) need one each. It reads n_seq, total_q,
+ *     total_k, q_heads, kv_heads and head_dim. */
 typedef struct {
   const void *q, *k, *v;
   void *out;
   float *lse;
   const int32_t *cu_q, *cu_k;
+  void *workspace;
   uint32_t *status;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  uint64_t workspace_bytes;
   uint32_t n_seq, total_q, total_k, q_heads, kv_heads, head_dim, dtype, causal;
   float scale;
   uint32_t reserved; /* 0 */
 } dv3k_packed_attention;
 int dv3k_attention_packed(const dv3k_packed_attention *args, void *stream);
+size_t dv3k_attention_packed_workspace(const dv3k_packed_attention *args);
 
 /* Rotate new queries and keys by their positions and append the keys and values to the cache.
  * Row t of sequence s (cu_new; NULL: row t is sequence t's only one and total == n_seq) stands at

@@ -145,6 +145,32 @@ def test_packed_long(causal, dim):
     check_packed(q, k, v, out, None, len_q, len_k, causal, dim ** -0.5)
 
 
+@pytest.mark.parametrize("len_q,len_k", [([1], [5000]), ([70, 3], [3000, 1500]), ([300, 0, 10, 64], [2500, 700, 5, 2048]), ([1030], [1030]), ([600, 1], [20, 4000])])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (6, 6), (5, 1)])
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@both
+def test_packed_few_queries_many_keys(len_q, len_k, hq, hkv, causal, dtype):
+    """Long items are cut into parts for several CTAs and joined."""
+    for dim in (64, 128):
+        q, k, v = packed_case(12, len_q, len_k, hq, hkv, dim, dtype, 2.0)
+        lse = torch.empty(q.shape[0], hq, device=DEV)
+        status = torch.zeros(2, dtype=torch.int32, device=DEV)
+        scratch = torch.full((1 << 26,), 255, dtype=torch.uint8, device=DEV)  # NaN wherever it is not written
+        out = dv.attention_packed(q, k, v, cu_of(len_q), cu_of(len_k), causal=causal, lse=lse, workspace=scratch, status=status)
+        check_packed(q, k, v, out, lse, len_q, len_k, causal, dim ** -0.5)
+        assert torch.equal(out, dv.attention_packed(q, k, v, cu_of(len_q), cu_of(len_k), causal=causal)) and status.tolist() == [0, 0]
+
+
+def test_packed_cut_items_and_values_that_are_not_finite():
+    """A part at the diagonal keeps later keys' infinities from the rows that do not see them."""
+    q, k, v = packed_case(13, [100], [3000], 4, 2, 64, torch.float16)
+    want = dv.attention_packed(q, k, v, ints([0, 100]), ints([0, 3000]), causal=True)
+    v2 = v.clone()
+    v2[2950:] = math.inf
+    got = dv.attention_packed(q, k, v2, ints([0, 100]), ints([0, 3000]), causal=True)
+    assert torch.equal(got[:50], want[:50]) and (got[50:] == math.inf).all()
+
+
 @both
 def test_packed_many_sequences(dtype):
     rng = torch.Generator().manual_seed(5)

@@ -15,10 +15,10 @@ BUF = ctypes.create_string_buffer(4096)
 BASE = (ctypes.addressof(BUF) + 63) & ~63
 
 # The argument structs of dinov3_kernels.h: pointers and 8-byte integers first, then 4-byte ones.
-PACKED_STRUCT, APPEND_STRUCT, PAGED_STRUCT = struct.Struct("8Q8q8IfI"), struct.Struct("12Q11q12I"), struct.Struct("9Q7qQ9If")
+PACKED_STRUCT, APPEND_STRUCT, PAGED_STRUCT = struct.Struct("9Q8qQ8IfI"), struct.Struct("12Q11q12I"), struct.Struct("9Q7qQ9If")
 
-PACKED = ["q", "k", "v", "out", "lse", "cu_q", "cu_k", "status", "q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token",
-          "out_head", "n_seq", "total_q", "total_k", "q_heads", "kv_heads", "head_dim", "dtype", "causal", "scale", "reserved"]
+PACKED = ["q", "k", "v", "out", "lse", "cu_q", "cu_k", "workspace", "status", "q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token",
+          "out_head", "workspace_bytes", "n_seq", "total_q", "total_k", "q_heads", "kv_heads", "head_dim", "dtype", "causal", "scale", "reserved"]
 APPEND = ["q", "k", "v", "q_out", "k_cache", "v_cache", "cu_new", "lens", "page_table", "cos", "sin", "status", "q_token", "q_head", "k_token",
           "k_head", "v_token", "v_head", "q_out_token", "q_out_head", "k_page", "v_page", "table_stride", "n_seq", "total", "max_pages", "n_pages",
           "page_size", "positions", "rot_dim", "q_heads", "kv_heads", "head_dim", "dtype", "reserved"]
@@ -57,6 +57,7 @@ HEADS = [("dtype", dict(dtype=2)), ("head_dim", dict(head_dim=80)), ("kv_heads",
     ("strides", dict(v_token=-128)), ("strides", dict(out_head=1 << 40)), ("overlap", dict(out_token=64)), ("overlap", dict(out_head=8)),
     ("overlap", dict(out_token=128, out_head=200)), ("null", dict(q=0)), ("null", dict(cu_k=0)), ("null", dict(v=0)), ("aligned", dict(k=BASE + 2)),
     ("aligned", dict(out=BASE + 8)), ("too many", dict(total_q=1 << 31)),
+    ("workspace", dict(total_k=4096)), ("workspace", dict(total_k=4096, workspace=BASE, workspace_bytes=1000)), ("aligned", dict(workspace=BASE + 8)),
 ])
 def test_packed_refusals(text, changes):
     refused("dv3k_attention_packed", PACKED_STRUCT, PACKED, packed_ok, text, **changes)
@@ -88,7 +89,9 @@ def test_null_arguments_and_nothing_to_do():
     lib = _lib.load()
     for name in ("dv3k_attention_packed", "dv3k_rope_append", "dv3k_attention_paged"):
         assert getattr(lib, name)(None, None) == dv.INVALID_ARGUMENT and "null" in _lib.last_error()
-    assert lib.dv3k_attention_paged_workspace(None) == 0
+    assert lib.dv3k_attention_paged_workspace(None) == 0 and lib.dv3k_attention_packed_workspace(None) == 0
+    few = dict(packed_ok, total_k=1024)
+    assert lib.dv3k_attention_packed_workspace(PACKED_STRUCT.pack(*(few[f] for f in PACKED))) == 0  # nothing long to cut
     for changes in (dict(n_seq=0), dict(total_q=0, q=0, out=0)):
         assert call("dv3k_attention_packed", PACKED_STRUCT, PACKED, dict(packed_ok, **changes))[0] == 0
     for changes in (dict(n_seq=0), dict(total=0, q=0, k=0)):
