@@ -42,26 +42,8 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const RopeA
   const uint64_t base = static_cast<uint64_t>(blockIdx.x) * kAppendThreads;
   const uint64_t warp_first = base + (threadIdx.x & ~31u);
   if (warp_first >= total_units) return;
-  const uint32_t t_first = static_cast<uint32_t>(warp_first / units);
-  int s = p.cu_new ? warp_find_sequence(p.cu_new, p.n_seq, t_first) : static_cast<int>(t_first);
-  const uint64_t at = base + threadIdx.x;
-  if (at >= total_units) return;
+  const uint64_t at = base + threadIdx.x < total_units ? base + threadIdx.x : total_units - 1;
   const uint32_t t = static_cast<uint32_t>(at / units), u = static_cast<uint32_t>(at % units);
-  if (p.cu_new) {
-    // a later row of the warp may belong to a later sequence
-    while (s + 1 < static_cast<int>(p.n_seq) && static_cast<int64_t>(p.cu_new[s + 1]) <= t) ++s;
-  } else {
-    s = static_cast<int>(t);
-  }
-  if (s < 0 || s >= static_cast<int>(p.n_seq)) return;
-  uint32_t first, end;
-  sequence_rows(p.cu_new, s, p.total, &first, &end);
-  if (t < first || t >= end) return;  // before the first or behind the last sequence
-  const int64_t pos = static_cast<int64_t>(p.lens[s]) - (end - first) + (t - first);
-  if (pos < 0 || (p.rot_dim && pos >= p.positions)) {
-    report(p.status, kErrPosition);
-    return;
-  }
   const uint32_t head = u / per_head, w = u % per_head;
   const bool is_q = head < p.q_heads;
   const bool is_k = !is_q && head < p.q_heads + p.kv_heads;
@@ -73,6 +55,23 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const RopeA
   const uint16_t *src = is_q ? p.q + t * p.q_token + h * p.q_head
                         : is_k ? p.k + t * p.k_token + h * p.k_head
                                : p.v + t * p.v_token + h * p.v_head;
+  // The data first: where it goes takes a chain of loads (sequence, length, page) that they overlap.
+  uint4 a = *reinterpret_cast<const uint4 *>(src + ca), b = *reinterpret_cast<const uint4 *>(src + cb);
+  int s = static_cast<int>(t);
+  if (p.cu_new) {
+    s = warp_find_sequence(p.cu_new, p.n_seq, static_cast<uint32_t>(warp_first / units));
+    // a later row of the warp may belong to a later sequence
+    while (s + 1 < static_cast<int>(p.n_seq) && static_cast<int64_t>(p.cu_new[s + 1]) <= t) ++s;
+  }
+  if (base + threadIdx.x >= total_units || s < 0 || s >= static_cast<int>(p.n_seq)) return;
+  uint32_t first, end;
+  sequence_rows(p.cu_new, s, p.total, &first, &end);
+  if (t < first || t >= end) return;  // before the first or behind the last sequence
+  const int64_t pos = static_cast<int64_t>(p.lens[s]) - (end - first) + (t - first);
+  if (pos < 0 || (p.rot_dim && pos >= p.positions)) {
+    report(p.status, kErrPosition);
+    return;
+  }
   uint16_t *dst;
   if (is_q) {
     dst = p.q_out + t * p.qo_token + h * p.qo_head;
@@ -87,7 +86,6 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const RopeA
     dst = (is_k ? p.k_cache + id * p.k_page : p.v_cache + id * p.v_page) +
           (static_cast<int64_t>(h) * p.page.size + slot) * p.head_dim;
   }
-  uint4 a = *reinterpret_cast<const uint4 *>(src + ca), b = *reinterpret_cast<const uint4 *>(src + cb);
   if (w < turned) {
     const int64_t row = pos * (p.rot_dim / 2) + ca;
     rotate<kBf16>(a, b, p.cos + row, p.sin + row);

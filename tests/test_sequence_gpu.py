@@ -12,6 +12,9 @@ The log-sum differs by d + n 2^-24 + 2^-20 + 2^-23 |lse|. A rotation differs by 
 |b|) (+ 2^-25 in float16).
 """
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -238,6 +241,19 @@ def test_packed_unseen_rows_do_not_reach_a_result(dtype, dim, bad):
     assert (hit.isnan() if math.isnan(bad) else hit == bad).all()
 
 
+@dims
+def test_packed_bad_queries_stay_in_their_rows(dim):
+    q, k, v = packed_case(14, [150, 60], [150, 60], 6, 2, dim, torch.bfloat16)
+    cu = cu_of([150, 60])
+    want = dv.attention_packed(q, k, v, cu, causal=True)
+    q2 = q.clone()
+    q2[77, 4], q2[160, 0] = math.nan, math.inf
+    got = dv.attention_packed(q2, k, v, cu, causal=True)
+    assert got[77, 4].isnan().all() and got[160, 0].isnan().all()
+    got[77, 4], got[160, 0] = want[77, 4], want[160, 0]
+    assert torch.equal(got, want)
+
+
 @both
 def test_packed_extreme_scores(dtype):
     """Scores far apart and of one sign, and equal ones: the maximum moves with almost every key."""
@@ -448,6 +464,39 @@ def test_paged_capture_streams_and_workspace():
     given = dv.attention_paged(q, k, v, table, n, workspace=torch.full((1 << 24,), 255, dtype=torch.uint8, device=DEV))
     assert torch.equal(given, held[0])
     assert dv.attention_paged(q[:0], k, v, table[:0], n[:0]).shape == (0, 8, 128)
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, dinov3_b200 as dv
+d = "cuda:0"
+q = torch.randn(40, 8, 64, device=d).half()
+cache, table = torch.zeros(80, 8, 16, 64, device=d).half(), torch.arange(80, dtype=torch.int32, device=d).view(1, 80)
+cu, n = torch.tensor([0, 40], dtype=torch.int32, device=d), torch.tensor([1200], dtype=torch.int32, device=d)
+cos = torch.ones(1300, 32, device=d)
+big = torch.randn(4096, 8, 64, device=d).half()
+big_cu = torch.tensor([0, 4096], dtype=torch.int32, device=d)
+def step():
+    a = dv.attention_packed(q, q, q, cu)
+    b = dv.attention_packed(q, big, big, cu, big_cu, causal=True)
+    r = dv.rope_append(q, q, q, cache, cache.clone(), table, n, cos, cos, cu_new=cu)
+    return a, b, r, dv.attention_paged(q[:1], cache, cache, table, n)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    held = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(held, step()))
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    here = os.path.dirname(os.path.abspath(__file__))
+    got = subprocess.run([sys.executable, "-c", FIRST_CALL, os.path.join(os.path.dirname(here), "dinov3-loom_b200")], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip() == "same", got.stderr[-2000:]
 
 
 # ---- append ----------------------------------------------------------------------------------

@@ -80,6 +80,7 @@ def test_append_refusals(text, changes):
 @pytest.mark.parametrize("text,changes", HEADS + CACHE + [
     ("q_heads", dict(q_heads=0)), ("scale", dict(scale=float("nan"))), ("strides", dict(q_seq=12)), ("overlap", dict(out_seq=128)),
     ("null", dict(out=0)), ("null", dict(lens=0)), ("aligned", dict(q=BASE + 8)), ("aligned", dict(workspace=BASE + 8)),
+    ("workspace", dict(max_pages=64, table_stride=64, max_len=1024)),
 ])
 def test_paged_refusals(text, changes):
     refused("dv3k_attention_paged", PAGED_STRUCT, PAGED, paged_ok, text, **changes)
