@@ -903,12 +903,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             const int blocks = blocks_of(reach, j);
             product(v_at, 0, j == 0, blocks);
-            // where the second half is there by now, the turn is kept
-            if (!mbar_test(&p_full[2 + t], p_phase)) {
-              give();
-              ok = mbar_wait(&p_full[2 + t], p_phase, abort_flag) && take();
-              if (!ok) break;
-            }
+            ok = mbar_wait(&p_full[2 + t], p_phase, abort_flag);
+            if (!ok) break;
             p_phase ^= 1;
             product(v_at, 1, j == 0, blocks);
             if (j + 1 < mine) {
