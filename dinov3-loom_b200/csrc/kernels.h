@@ -230,7 +230,7 @@ struct RopeAppend {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head, k_page, v_page,
       table_stride;
   uint32_t *status;
-  PageDiv page;
+  PageDiv page, units;  // units: of a row, set by the launch
   uint32_t n_seq, total, max_pages, n_pages, positions, rot_dim, q_heads, kv_heads, head_dim;
 };
 cudaError_t launch_rope_append(const RopeAppend &p, bool bf16, cudaStream_t stream);
