@@ -26,7 +26,7 @@
 //   - Where no sequence passes 256 keys, stretches are whole units and there is nothing to join; with
 //     no more units than CTAs, the four warps of a CTA share one and join in shared memory.
 // Four warps on one 64-key tile, meeting at barriers, took 24.8 us for 256 images of 201 tokens and
-// 51.5 us for 64 sequences of 1..4096 (32/8 heads of 128); these take 17.8 and 41.
+// 51.5 us for 64 sequences of 1..4096 (32/8 heads of 128); these take 18 and 40.
 #include <atomic>
 #include <type_traits>
 
@@ -129,21 +129,26 @@ Plan plan_of(const PagedAttention &p) {
   return s;
 }
 
-// Workspace: the start of each sequence in the row of all tiles [n_seq + 1] (u64, written by
-// CTA 0), then (max, sum) and the output of [warps][2][rows] partial results.
-__host__ __device__ inline size_t starts_bytes(uint32_t n_seq) {
-  return ((static_cast<size_t>(n_seq) + 1) * 8 + 15) / 16 * 16;
+// Workspace: for each unit with tokens the first warp that has part of it, and how many have (the top
+// bit: it is that warp's last unit, not its first), written by that warp; then (max, sum) and the
+// output of [warps][2][rows] partial results.
+struct Share {
+  uint32_t first, parts;
+};
+constexpr uint32_t kLastUnit = 0x80000000u;
+__host__ __device__ inline size_t shares_bytes(const PagedAttention &p, const Plan &pl) {
+  return (static_cast<size_t>(p.n_seq) * pl.head_blocks * sizeof(Share) + 15) / 16 * 16;
 }
 struct Partials {
-  uint64_t *starts;
+  Share *shares;
   float2 *ml;
   float *o;
 };
 __device__ __forceinline__ Partials partials_of(const PagedAttention &p, const Plan &pl) {
   Partials w;
   uint8_t *at = static_cast<uint8_t *>(p.workspace);
-  w.starts = reinterpret_cast<uint64_t *>(at);
-  w.ml = reinterpret_cast<float2 *>(at + starts_bytes(p.n_seq));
+  w.shares = reinterpret_cast<Share *>(at);
+  w.ml = reinterpret_cast<float2 *>(at + shares_bytes(p, pl));
   const size_t n = (static_cast<size_t>(pl.grid) * kWarps * 2 * pl.rows + 1) / 2 * 2;
   w.o = reinterpret_cast<float *>(w.ml + n);
   return w;
@@ -186,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
   pdl_trigger();  // the joining launch waits for this one's end by itself
   auto tiles_of = [&](uint32_t s) { return (cached_tokens(p, s, false) + kTile - 1) / kTile; };
 
+  uint64_t per = 0;  // tiles of a stretch
   // The stretches of this CTA's warps: each from (s, hb, t) up to but without the next one's.
   const uint64_t warp0 = static_cast<uint64_t>(blockIdx.x) * kWarps;
   if (pl.units) {
@@ -216,14 +222,12 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
       if (w < warp) at += scan[w];
       total += scan[w];
     }
-    const uint64_t per = stretch_of(total, pl.grid);
+    per = stretch_of(total, pl.grid);
     if (tid <= kWarps && per * (warp0 + tid) >= total) {
       found[tid][0] = p.n_seq;
       found[tid][1] = found[tid][2] = 0;
     }
-    uint64_t *starts = static_cast<uint64_t *>(p.workspace);
     for (uint32_t s = from; s < to; ++s) {
-      if (blockIdx.x == 0) starts[s] = at;
       const uint64_t n = cost_of(tiles_of(s)), next = at + n * pl.head_blocks;
 #pragma unroll 1
       for (int e = 0; e <= kWarps; ++e) {
@@ -237,7 +241,6 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
       }
       at = next;
     }
-    if (blockIdx.x == 0 && tid == 0) starts[p.n_seq] = total;
   }
   __syncthreads();
   const uint32_t to = pl.team ? kWarps : warp + 1, step = pl.team ? kWarps : 1;
@@ -376,6 +379,13 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
     const uint32_t heads = min(16u, (at.head + 1) * group - h0);
     const bool whole = at.t == 0 && at.end == at.tiles;
     const uint32_t slot = i == 0 ? 0 : 1;                      // the stretch's first unit, or its last
+    if (!pl.units && lane == 0 && at.t == 0 && at.tiles > 0) {
+      // the warps after this one start within the unit and take `per` tiles of it each
+      const uint32_t after = at.tiles - at.end;
+      Share share = {static_cast<uint32_t>(warp0) + warp, 1 + static_cast<uint32_t>((after + per - 1) / per)};
+      if (slot) share.parts |= kLastUnit;
+      partials_of(p, pl).shares[static_cast<size_t>(at.s) * pl.head_blocks + at.hb] = share;
+    }
     if (lane == 0 && at.hb == 0) cached_tokens(p, at.s, true);  // tells of a length past the table
 
 #pragma unroll
@@ -573,7 +583,9 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
 // the stretches i in order; and writes the rows of empty sequences. kJoin warps take every kJoin-th
 // part of a (sequence, query head), then meet in shared memory: 4 where units have few parts, 32
 // where they have more than 16 (4 warps took 20 us for 148 parts; 32, or a single one, 2 to 4 us
-// more than 4 for the few parts of 64 sequences of 1..4096 tokens).
+// more than 4 for the few parts of 64 sequences of 1..4096 tokens). What a unit's parts are the first
+// launch has left in the workspace: summing the lengths before s again, as it was, kept the join's
+// loads waiting (42.0 us in all for those 64 sequences; 39.6 so).
 template <bool kBf16, int kDim, int kJoin>
 __global__ void __launch_bounds__(kJoin * 32)
     attention_paged_join_kernel(const PagedAttention p, const Plan pl) {
@@ -586,34 +598,48 @@ __global__ void __launch_bounds__(kJoin * 32)
   const uint32_t hb = h / group * blocks + h % group / 16, r = h % group % 16;
   pdl_wait();
   const Partials w = partials_of(p, pl);
-  const uint64_t total = w.starts[p.n_seq], start = w.starts[s], next = w.starts[s + 1];
-  const uint64_t per = stretch_of(total, pl.grid);
-  const uint64_t cost = (next - start) / pl.head_blocks, from = start + hb * cost;
-  const uint32_t c0 = static_cast<uint32_t>((from + kUnit) / per);
-  const uint32_t n = cost ? static_cast<uint32_t>((from + cost - 1) / per) - c0 + 1 : 0;
+  Share share = w.shares[static_cast<size_t>(s) * pl.head_blocks + hb];  // of an empty one: not read
+  if (cached_tokens(p, s, false) == 0) share = {0, 0};
+  const uint32_t n = share.parts & ~kLastUnit;
   if (n == 1) return;  // one warp's: written
-  // the unit is the first of a stretch, or its last
-  const uint32_t first_slot = per * c0 >= from ? 0 : 1;
   auto slot_of = [&](uint32_t i) {
-    return (static_cast<size_t>(c0 + i) * 2 + (i ? 0 : first_slot)) * pl.rows + r;
+    return ((static_cast<size_t>(share.first) + i) * 2 + (i == 0 && share.parts != n)) * pl.rows + r;
   };
+  // The first of this warp's parts on their way under the search for the largest maximum.
+  constexpr int kEarly = 4;
+  float2 ml[kEarly];
+  float v[kEarly][kLane];
+  auto load = [&](uint32_t i, float2 &x, float(&o)[kLane]) {
+    const size_t at = slot_of(i);
+    x = w.ml[at];
+#pragma unroll
+    for (int e = 0; e < kLane; e += 2) {
+      const float2 y = *reinterpret_cast<const float2 *>(w.o + at * kDim + lane * kLane + e);
+      o[e] = y.x;
+      o[e + 1] = y.y;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k)
+    if (warp + k * kJoin < n) load(warp + k * kJoin, ml[k], v[k]);
   float top = -INFINITY;
   for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, w.ml[slot_of(i)].x);
 #pragma unroll
   for (int i = 16; i > 0; i /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
   float sum = 0.f, acc[kLane] = {};
-#pragma unroll 4
-  for (uint32_t i = warp; i < n; i += kJoin) {
-    const size_t at = slot_of(i);
-    const float2 x = w.ml[at];
+  auto add = [&](const float2 &x, const float(&o)[kLane]) {
     const float f = top == -INFINITY ? 1.f : ex2_approx(x.x - top);
     sum = fmaf(x.y, f, sum);
 #pragma unroll
-    for (int e = 0; e < kLane; e += 2) {
-      const float2 v = *reinterpret_cast<const float2 *>(w.o + at * kDim + lane * kLane + e);
-      acc[e] = fmaf(v.x, f, acc[e]);
-      acc[e + 1] = fmaf(v.y, f, acc[e + 1]);
-    }
+    for (int e = 0; e < kLane; ++e) acc[e] = fmaf(o[e], f, acc[e]);
+  };
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k)
+    if (warp + k * kJoin < n) add(ml[k], v[k]);
+#pragma unroll 4
+  for (uint32_t i = warp + kEarly * kJoin; i < n; i += kJoin) {
+    load(i, ml[0], v[0]);
+    add(ml[0], v[0]);
   }
 #pragma unroll
   for (int e = 0; e < kLane; ++e) po[warp][lane * kLane + e] = acc[e];
@@ -641,7 +667,7 @@ size_t attention_paged_workspace(const PagedAttention &p) {
   const Plan pl = plan_of(p);
   if (pl.units) return 0;
   const size_t n = (static_cast<size_t>(pl.grid) * kWarps * 2 * pl.rows + 1) / 2 * 2;
-  return starts_bytes(p.n_seq) + n * (p.head_dim + 2) * sizeof(float);
+  return shares_bytes(p, pl) + n * (p.head_dim + 2) * sizeof(float);
 }
 
 namespace {
