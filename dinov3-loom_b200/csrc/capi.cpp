@@ -513,6 +513,11 @@ bool strides_ok(int64_t row, uint32_t rows, int64_t head, uint32_t heads) {
   return row > 0 && head > 0 && row % 8 == 0 && head % 8 == 0 && row < kMost && head < kMost;
 }
 
+template <typename... P>
+bool words_aligned(P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 3u) == 0;
+}
+
 // No two (row, head) vectors of `dim` elements share memory.
 bool rows_apart(int64_t row, uint32_t rows, int64_t head, uint32_t heads, uint32_t dim) {
   if (rows > 1 && row < dim) return false;
@@ -609,6 +614,8 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
     return bad_args("null tensor");
   if (!all_aligned(a->q, a->k, a->v, a->out, a->workspace))
     return bad_args("pointers must be 16-byte aligned");
+  if (!words_aligned(a->lse, a->cu_q, a->cu_k, a->status))
+    return bad_args("lse, cu_q, cu_k and status must be 4-byte aligned");
   dv3::PackedAttention p = {};
   p.q = static_cast<const uint16_t *>(a->q);
   p.k = static_cast<const uint16_t *>(a->k);
@@ -638,6 +645,8 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
   if (const size_t need = dv3::attention_packed_workspace(p);
       need > 0 && (!a->workspace || a->workspace_bytes < need))
     return bad_args("workspace must hold dv3k_attention_packed_workspace bytes");
+  if (a->out == a->q || a->out == a->k || a->out == a->v)
+    return bad_args("out overlaps an input");
   std::string err;
   const cudaError_t e = dv3::launch_attention_packed(p, a->dtype == DV3K_BF16,
                                                      static_cast<cudaStream_t>(stream), &err);
@@ -686,6 +695,8 @@ int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {
     return bad_args("null tensor");
   if (!all_aligned(a->q, a->k, a->v, a->q_out, a->cos, a->sin))
     return bad_args("pointers must be 16-byte aligned");
+  if (!words_aligned(a->cu_new, a->lens, a->status))
+    return bad_args("cu_new, lens and status must be 4-byte aligned");
   dv3::RopeAppend p = {};
   p.q = static_cast<const uint16_t *>(a->q);
   p.k = static_cast<const uint16_t *>(a->k);
@@ -720,6 +731,8 @@ int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {
   p.q_heads = a->q_heads;
   p.kv_heads = a->kv_heads;
   p.head_dim = a->head_dim;
+  if (p.q && p.q == p.q_out && (p.q_token != p.qo_token || p.q_head != p.qo_head))
+    return bad_args("q_out overlaps q: in place the strides are the same");
   return launch_status(
       dv3::launch_rope_append(p, a->dtype == DV3K_BF16, static_cast<cudaStream_t>(stream)),
       "rope_append");
@@ -737,7 +750,8 @@ int dv3k_attention_paged(const dv3k_paged_attention *a, void *stream) {
   if (const char *e = check_heads(a->q_heads, a->kv_heads, a->head_dim, a->dtype)) return bad_args(e);
   if (a->q_heads == 0) return bad_args("q_heads must be positive");
   if (!scale_ok(a->scale)) return bad_args("scale must be positive and finite");
-  if (a->n_seq > 0x7fffff00u) return bad_args("too many sequences");
+  if (static_cast<uint64_t>(a->n_seq) * a->q_heads > 0x7fffff00u)
+    return bad_args("too many sequences and heads");
   if (!strides_ok(a->q_seq, a->n_seq, a->q_head, a->q_heads) ||
       !strides_ok(a->out_seq, a->n_seq, a->out_head, a->q_heads))
     return bad_args("strides must be positive multiples of 8 elements");
@@ -750,10 +764,13 @@ int dv3k_attention_paged(const dv3k_paged_attention *a, void *stream) {
   if (a->n_seq == 0) return DV3_OK;
   if (!a->q || !a->out || !a->lens) return bad_args("null tensor");
   if (!all_aligned(a->q, a->out, a->workspace)) return bad_args("pointers must be 16-byte aligned");
+  if (!words_aligned(a->lse, a->lens, a->status))
+    return bad_args("lse, lens and status must be 4-byte aligned");
   const dv3::PagedAttention p = paged_args(*a);
   if (const size_t need = dv3::attention_paged_workspace(p);
       need > 0 && (!a->workspace || a->workspace_bytes < need))
     return bad_args("workspace must hold dv3k_attention_paged_workspace bytes");
+  if (a->out == a->q) return bad_args("out overlaps q");
   return launch_status(
       dv3::launch_attention_paged(p, a->dtype == DV3K_BF16, static_cast<cudaStream_t>(stream)),
       "attention_paged");

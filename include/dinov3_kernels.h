@@ -205,7 +205,8 @@ int dv3k_matmul_swiglu(const uint16_t *h, uint32_t rows, const uint16_t *gateup_
  *     product's sum are f32; the weights are rounded to `dtype` before the product with v.
  *   - A row tensor [rows][heads][head_dim] is given by its row (token) and head strides in
  *     elements, multiples of 8, with head_dim contiguous. Rows or heads of an output do not
- *     overlap, nor does an output overlap an input (but q_out of dv3k_rope_append may be q).
+ *     overlap, nor does an output overlap an input (but q_out of dv3k_rope_append may be q); arrays of
+ *     4-byte words are 4-byte aligned, all else 16-byte.
  *   - `cu` arrays [n_seq + 1] (i32, device) hold the first row of each sequence and the end of the
  *     last, ascending. Sequences may be empty. Rows before cu[0] or from cu[n_seq] on are left as
  *     they were. Values outside the tensor are clamped to it.
@@ -254,8 +255,9 @@ size_t dv3k_attention_packed_workspace(const dv3k_packed_attention *args);
  *   q_out[t][h][c + rot/2] = q[c + rot/2] cos[p][c] + q[c] sin[p][c]   for c < rot/2,
  * and as it is for c >= rot; k the same into slot p % page_size of page page_table[s][p /
  * page_size], v unchanged. cos, sin: f32 [positions][rot_dim / 2]; rot_dim is a multiple of 16 up
- * to head_dim, or 0 (no rotation, tables NULL). q NULL (with q_heads 0): append only. Two rows of
- * one call that name the same slot leave either's value there. */
+ * to head_dim, or 0 (no rotation, tables NULL). q NULL (with q_heads 0): append only. In
+ * place (q_out = q) both have the same strides. Rows of one call do not name the same slot; where
+ * they do all the same, it holds channels of each. */
 typedef struct {
   const void *q, *k, *v;
   void *q_out, *k_cache, *v_cache;

@@ -58,6 +58,8 @@ HEADS = [("dtype", dict(dtype=2)), ("head_dim", dict(head_dim=80)), ("kv_heads",
     ("overlap", dict(out_token=128, out_head=200)), ("null", dict(q=0)), ("null", dict(cu_k=0)), ("null", dict(v=0)), ("aligned", dict(k=BASE + 2)),
     ("aligned", dict(out=BASE + 8)), ("too many", dict(total_q=1 << 31)),
     ("workspace", dict(total_k=4096)), ("workspace", dict(total_k=4096, workspace=BASE, workspace_bytes=1000)), ("aligned", dict(workspace=BASE + 8)),
+    ("4-byte", dict(lse=BASE + 2)), ("4-byte", dict(cu_q=BASE + 1)), ("4-byte", dict(status=BASE + 2)), ("out overlaps", dict(out=BASE)),
+    ("out overlaps", dict(q=BASE + 1024, k=BASE + 2048)),
 ])
 def test_packed_refusals(text, changes):
     refused("dv3k_attention_packed", PACKED_STRUCT, PACKED, packed_ok, text, **changes)
@@ -72,15 +74,17 @@ CACHE = [("page_size", dict(page_size=0)), ("page_size", dict(page_size=1 << 17)
     ("reserved", dict(reserved=3)), ("go together", dict(q=0)), ("go together", dict(q_heads=0)), ("rot_dim", dict(rot_dim=24)),
     ("rot_dim", dict(rot_dim=80)), ("total", dict(cu_new=0)), ("strides", dict(k_token=4)), ("strides", dict(q_head=0)), ("overlap", dict(q_out_token=64)),
     ("null", dict(k=0)), ("null", dict(lens=0)), ("null", dict(q_out=0)), ("null", dict(sin=0)), ("aligned", dict(cos=BASE + 4)),
+    ("4-byte", dict(lens=BASE + 2)), ("4-byte", dict(cu_new=BASE + 3)), ("q_out overlaps", dict(q_out_token=512)), ("q_out overlaps", dict(q_head=8)),
 ])
 def test_append_refusals(text, changes):
     refused("dv3k_rope_append", APPEND_STRUCT, APPEND, append_ok, text, **changes)
 
 
 @pytest.mark.parametrize("text,changes", HEADS + CACHE + [
-    ("q_heads", dict(q_heads=0)), ("scale", dict(scale=float("nan"))), ("strides", dict(q_seq=12)), ("overlap", dict(out_seq=128)),
+    ("q_heads", dict(q_heads=0)), ("too many", dict(n_seq=1 << 29)), ("scale", dict(scale=float("nan"))), ("strides", dict(q_seq=12)), ("overlap", dict(out_seq=128)),
     ("null", dict(out=0)), ("null", dict(lens=0)), ("aligned", dict(q=BASE + 8)), ("aligned", dict(workspace=BASE + 8)),
-    ("workspace", dict(max_pages=64, table_stride=64, max_len=1024)),
+    ("workspace", dict(max_pages=64, table_stride=64, max_len=1024)), ("4-byte", dict(lens=BASE + 2)), ("4-byte", dict(status=BASE + 1)),
+    ("out overlaps", dict(out=BASE)),
 ])
 def test_paged_refusals(text, changes):
     refused("dv3k_attention_paged", PAGED_STRUCT, PAGED, paged_ok, text, **changes)
