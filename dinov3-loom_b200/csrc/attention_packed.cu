@@ -23,10 +23,10 @@
 //              tile to global memory. Of a last, partly visible step only the blocks of 32 keys
 //              that some row sees are computed.
 //   warp 8     TMA producer: Q tiles, then K and V tiles in turn through one ring of stages.
-//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = 128, N = a step's keys), and O_t += P_t V with P
-//              from TMEM and V as the MN-major B operand, one tile at a time.
-//   warp 11    scheduler (publishes items one ahead), and guard of V: a key that a row does not see has weight 0, but 0 times
-//              an infinity or NaN is NaN. Only the tiles at an item's end (from the first that some
+//   warps 9/10 MMA issuers of tile 0 / tile 1: S_t = Q_t K^T (M = 128, N = a step's keys), and
+//              O_t += P_t V with P from TMEM and V as the MN-major B operand, one tile at a time.
+//   warp 11    scheduler (publishes items one ahead), and guard of V: a key that a row does not see
+//              has weight 0, but 0 times an infinity or NaN is NaN. Only the tiles at an item's end (from the first that some
 //              row sees in part) can hold such keys; there it tests V in shared memory, sets what
 //              is not finite to 0 and leaves a note, and the rows that do see those keys add them
 //              at the end from global memory.
@@ -511,11 +511,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_map(&tmk);
     tma_prefetch_map(&tmv);
   }
+  for (int i = threadIdx.x; i <= kBuckets; i += kThreads) order[i] = 0;
+  // All before is under the end of the kernel before. TMEM after the wait: all its columns are taken, and
+  // a kernel that is not done may still want some on this SM. This kernel does not let the next one in
+  // early: its CTAs would take the SMs in the order they fall free, and 24 prompts of 1..2048 tokens, each
+  // call behind the last, then took 90 us and not 84.
+  pdl_wait();
   if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
-  for (int i = threadIdx.x; i <= kBuckets; i += kThreads) order[i] = 0;
   uint32_t width = 0x7fffff00u;  // one class
   if (!p.flat) {
     __syncthreads();
@@ -622,10 +627,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return it;
     };
-    if (!ok && lane == 0) {
-      report(p.status, kErrAttentionWait);
-      *abort_flag = 1;
-    }
     uint32_t ring = 0, phase = 0, v_ring = 0;
     Item it = {};  // nothing before the first
     for (uint32_t k = 0; ok && it.part >= 0; ++k) {
@@ -760,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // One tile at a time puts its products on the tensor cores. Left to interleave, both tiles'
       // would end together, both softmaxes would start together, and the tiles would stay in step,
       // the tensor cores idle under the softmax and the other way round (2.30 ms for 16384 causal
-      // tokens against 2.12); taken in turn, one falls half a step behind the other by itself.
+      // tokens of 32/8 heads of 128 against 2.07); taken in turn, one falls half a step behind the other by itself.
       auto take = [&] {
         if (atomicCAS(turn, 0u, 1u) == 0u) return true;
         const uint64_t t0 = globaltimer();
@@ -1165,9 +1166,8 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
-  attention_packed_kernel<kBf16, kDim>
-      <<<dim3(grid), dim3(kThreads), Layout<kDim>::kBytes, stream>>>(q, k, v, o, a);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_pdl(attention_packed_kernel<kBf16, kDim>, dim3(grid), dim3(kThreads), Layout<kDim>::kBytes,
+                                   stream, q, k, v, o, a);
   if (e != cudaSuccess || a.parts_max == 0) return e;
   return launch_pdl(attention_packed_join_kernel<kBf16, kDim>, dim3(a.parts_max, kDim / 16), dim3(256), 0, stream, a);
 }

@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
   __shared__ uint64_t scan[kWarps];
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t group = p.q_heads / p.kv_heads, blocks = pl.head_blocks / p.kv_heads;
-  pdl_trigger();  // the joining launch waits for this one's end by itself
+  pdl_wait();  // what the kernel before wrote is there from here on
+  pdl_trigger();
   auto tiles_of = [&](uint32_t s) { return (cached_tokens(p, s, false) + kTile - 1) / kTile; };
 
   uint64_t per = 0;  // tiles of a stretch
@@ -597,6 +598,7 @@ __global__ void __launch_bounds__(kJoin * 32)
   const uint32_t group = p.q_heads / p.kv_heads, blocks = pl.head_blocks / p.kv_heads;
   const uint32_t hb = h / group * blocks + h % group / 16, r = h % group % 16;
   pdl_wait();
+  pdl_trigger();
   const Partials w = partials_of(p, pl);
   Share share = w.shares[static_cast<size_t>(s) * pl.head_blocks + hb];  // of an empty one: not read
   if (cached_tokens(p, s, false) == 0) share = {0, 0};
@@ -684,12 +686,10 @@ cudaError_t launch(const PagedAttention &p, const Plan &pl, cudaStream_t stream)
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
-  const uint64_t join = static_cast<uint64_t>(p.n_seq) * p.q_heads;
-  if (join > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  attention_paged_kernel<kBf16, kDim, kHeads8><<<dim3(pl.grid), dim3(kThreads), kWarps * Ring<kDim>::kBytes, stream>>>(p, pl);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_pdl(attention_paged_kernel<kBf16, kDim, kHeads8>, dim3(pl.grid), dim3(kThreads),
+                                   kWarps * Ring<kDim>::kBytes, stream, p, pl);
   if (e != cudaSuccess || pl.units) return e;
-  const uint32_t rows = static_cast<uint32_t>(join);
+  const uint32_t rows = p.n_seq * p.q_heads;  // below 2^31
   return pl.crowd ? launch_pdl(attention_paged_join_kernel<kBf16, kDim, 32>, dim3(rows), dim3(1024), 0, stream, p, pl)
                   : launch_pdl(attention_paged_join_kernel<kBf16, kDim, 4>, dim3(rows), dim3(128), 0, stream, p, pl);
 }

@@ -39,6 +39,8 @@ __device__ __forceinline__ void rotate(uint4 &a, uint4 &b, const float *cs, cons
 template <bool kBf16>
 __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(
     const RopeAppend p, uint32_t row0, uint32_t rows) {
+  pdl_wait();  // what the kernel before wrote is there from here on
+  pdl_trigger();
   const uint32_t units = p.units.size;
   const uint32_t total_units = rows * units;  // below 2^31
   const uint32_t base = blockIdx.x * kAppendThreads;
@@ -101,15 +103,11 @@ cudaError_t launch_rope_append(const RopeAppend &args, bool bf16, cudaStream_t s
   p.units = page_div((p.q_heads + 2 * p.kv_heads) * (p.head_dim / 16));
   // one launch, but for more units than 31 bits count
   const uint32_t most = 0x7fffff00u / p.units.size;
-  if (most == 0) return cudaErrorInvalidConfiguration;
   for (uint32_t row0 = 0; row0 < p.total; row0 += most) {
     const uint32_t rows = p.total - row0 < most ? p.total - row0 : most;
     const dim3 g((rows * p.units.size + kAppendThreads - 1) / kAppendThreads), b(kAppendThreads);
-    if (bf16)
-      rope_append_kernel<true><<<g, b, 0, stream>>>(p, row0, rows);
-    else
-      rope_append_kernel<false><<<g, b, 0, stream>>>(p, row0, rows);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = bf16 ? launch_pdl(rope_append_kernel<true>, g, b, 0, stream, p, row0, rows)
+                               : launch_pdl(rope_append_kernel<false>, g, b, 0, stream, p, row0, rows);
     if (e != cudaSuccess || rows < most) return e;
   }
   return cudaSuccess;
