@@ -592,6 +592,43 @@ def test_append_skips_and_reports_bad_places():
 
 # ---- together --------------------------------------------------------------------------------
 @both
+@dims
+def test_calls_that_read_what_the_one_before_wrote(dtype, dim):
+    """A launch may be set up under the end of the one before. Layers whose every call reads the output
+    of the call before it, with one workspace for all: the same bits whether the host waits between
+    the calls, does not, or replays them from a graph."""
+    hq, hkv, page, lens = 8, 2, 16, [1, 900, 37, 2100, 0, 300]
+    g, rows = gen(60 + dim), sum(lens)
+    k_cache, v_cache, table = paged_cache(61, lens, hkv, page, dim, dtype)
+    first = randn(g, rows, hq, dim, dtype=dtype)
+    cos, sin = tables(4096, dim)
+    cu, n = cu_of(lens), ints(lens)
+    scratch = torch.empty(1 << 27, dtype=torch.uint8, device=DEV)
+
+    def layers(wait):
+        x, got = first, []
+        for _ in range(5):
+            q = dv.rope_append(x, x[:, :hkv], x[:, hkv:2 * hkv], k_cache, v_cache, table, n, cos, sin, cu_new=cu)
+            wait()
+            x = dv.attention_packed(q, q[:, :hkv], q[:, hkv:2 * hkv], cu, causal=True, workspace=scratch)
+            wait()
+            got += [q, x, dv.attention_paged(x[:len(lens)], k_cache, v_cache, table, n, workspace=scratch)]
+            wait()
+        return got
+
+    waited = [t.clone() for t in layers(torch.cuda.synchronize)]
+    assert waited[-1].abs().max() > 0 and not torch.equal(waited[1], waited[4])
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(waited, layers(lambda: None)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = layers(lambda: None)
+    for _ in range(2):
+        graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(waited, held))
+
+
+@both
 def test_prompt_then_tokens(dtype):
     """A decoder's attention: prompts packed, rotated, cached and attended, then tokens one at a
     time, against the whole sequences in float64. Captured decode steps give the eager bits."""
