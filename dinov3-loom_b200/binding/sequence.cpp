@@ -8,7 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -120,8 +120,13 @@ uint32_t *status_of(PyObject *o, const at::Tensor &like) {
   return static_cast<uint32_t *>(t.data_ptr());
 }
 
+// A new tensor from torch's allocator, without the dispatcher's way to it.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 at::Tensor output(PyObject *o, const char *name, const at::Tensor &like, const at::Tensor &q) {
-  if (o == Py_None) return at::empty(q.sizes(), q.options().requires_grad(false));
+  if (o == Py_None) return fresh(q.sizes(), q.scalar_type(), q);
   const at::Tensor &t = tensor(o, name);
   rows(t, name, like);
   if (t.sizes() != q.sizes()) refuse(name, " must have shape ", q.sizes(), ": ", t.sizes());
@@ -153,7 +158,7 @@ at::Tensor scratch_of(PyObject *given, Args &p, size_t (*need_of)(const Args *),
     if (w.scalar_type() != at::kByte || w.device() != q.device() || !w.is_contiguous())
       refuse("workspace must be a contiguous uint8 tensor on ", q.device());
   } else if (const size_t need = need_of(&p)) {
-    w = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte).requires_grad(false));
+    w = fresh({static_cast<int64_t>(need)}, at::kByte, q);
   } else {
     return w;
   }

@@ -69,7 +69,7 @@ def _build_binding(force: bool):
                sysconfig.get_paths()["include"]]
     cmd = [NVCC, "-O2", "-std=c++17", "-shared", "-cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden",
            *("-I" + d for d in include), BINDING, "-o", BINDING_LIB, "-L" + os.path.join(torch, "lib"),
-           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"binding failed:\n{r.stdout}")
