@@ -414,6 +414,20 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
                                              int vis, int blocks, bool first, float &m, float &sum,
                                              uint32_t tp, uint64_t *p_full, Loaded &&loaded,
                                              Before &&before) {
+  if (masked) {
+    // what a row does not see becomes -inf in TMEM, in the blocks that some row of the warp sees in part
+    const int least = __reduce_min_sync(0xffffffffu, vis);
+#pragma unroll 1
+    for (int i = max(least, 0) / 32; i < blocks; ++i) {
+      uint32_t x[32];
+      tmem_load32(tl + 32 * i, x);
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (e >= vis - 32 * i) x[e] = 0xff800000u;
+      tmem_st32(tl + 32 * i, x);
+    }
+    tmem_st_wait();
+  }
   uint32_t v[kBlocks][32];
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) tmem_ld32(tl + 32 * i, v[i]);  // past `blocks`: old values, not used
@@ -421,16 +435,6 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
 #pragma unroll
   for (int i = 1; i < kBlocks; ++i) tmem_regs_ready(v[i]);
   loaded();
-  if (masked) {
-    const int least = __reduce_min_sync(0xffffffffu, vis);  // of the warp's rows
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-      if (least >= 32 * (i + 1)) continue;
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (32 * i + e >= vis) v[i][e] = 0xff800000u;  // -inf
-    }
-  }
   float tops[kBlocks];
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) {
@@ -439,6 +443,7 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
     for (int e = 3; e + 1 < 32; e += 2)
       tops[i] = max3(tops[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
     tops[i] = fmaxf(tops[i], __uint_as_float(v[i][31]));
+    if (i >= blocks) tops[i] = -INFINITY;
   }
   float top = tops[0];
 #pragma unroll
@@ -1014,64 +1019,72 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&sched_empty[k % 3]);
       if (it.part < 0) break;
       if (rows_live == 0) continue;
+      if (fix) {
+        // what the guard took out of the steps that are seen in part
+        const int from = reach_of<kKeys>(it, 0, tokens, p.causal).first / kKeys * kKeys;
+#pragma unroll 1
+        for (int d = 0; d < kDim; d += 16) {
+          uint32_t x[16];
+          tmem_ld16(to + d, x);
+          tmem_ld_wait();
+          tmem_regs_ready16(x);
+#pragma unroll 1
+          for (int kk = from; live && kk < sees; ++kk) {
+            const uint32_t *v = reinterpret_cast<const uint32_t *>(
+                p.v + (static_cast<int64_t>(it.k_row) + kk) * p.v_token + it.head * p.v_head + d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t w = v[e];
+              const float2 f = Elem<kBf16>::unpack(w);
+              if (!finite16<kBf16>(w & 0xffffu)) x[2 * e] = __float_as_uint(__uint_as_float(x[2 * e]) + f.x);
+              if (!finite16<kBf16>(w >> 16)) x[2 * e + 1] = __float_as_uint(__uint_as_float(x[2 * e + 1]) + f.y);
+            }
+          }
+          __syncwarp();
+          tmem_st16(to + d, x);
+        }
+        tmem_st_wait();
+      }
       // 64 channels at a time through this warp's staging (16-byte chunk c of row r at c ^ (r & 7)):
       // by one TMA store where all 32 rows are of the sequence and whole tokens, else 8 lanes to a
-      // row of 128 bytes.
+      // row of 128 bytes. The next 64 are read and rounded while the store before reads the staging.
       const bool boxed = p.boxed && rows_live == 0xffffffffu;
 #pragma unroll 1
       for (int d = 0; d < kDim; d += 64) {
+        uint32_t x[2][32];
+        if (r.steps > 0) {
+          tmem_ld32(to + d, x[0]);
+          tmem_ld32(to + d + 32, x[1]);
+          tmem_wait_ld(x[0]);
+          tmem_regs_ready(x[1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) x[e / 32][e % 32] = 0;
+        }
+        if (it.part > 0) {  // a part: as it is
+          const Parts<kDim> to_join = Parts<kDim>::of(p.workspace, p.parts_max);
+          const size_t tile = static_cast<size_t>(it.part - 1) * 2 + t;
+          if (live) {
+            if (d == 0) to_join.ml[tile * 128 + row] = make_float2(m, sum);
+            float4 *o = to_join.o + (tile * (kDim / 4) + d / 4) * 128 + row;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e * 128] = make_float4(__uint_as_float(x[e / 8][4 * e % 32]), __uint_as_float(x[e / 8][4 * e % 32 + 1]),
+                                       __uint_as_float(x[e / 8][4 * e % 32 + 2]), __uint_as_float(x[e / 8][4 * e % 32 + 3]));
+          }
+          continue;
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          w[e] = Elem<kBf16>::pack(__uint_as_float(x[e / 16][2 * e % 32]) * inv, __uint_as_float(x[e / 16][2 * e % 32 + 1]) * inv);
         if (lane == 0) bulk_wait_read<0>();  // the store before has read the staging
         __syncwarp();
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t x[32];
-          if (r.steps > 0) {
-            tmem_load32(to + d + 32 * half, x);
-          } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = 0;
-          }
-          if (fix && live) {
-            // what the guard took out of the steps that are seen in part
-            const int from = reach_of<kKeys>(it, 0, tokens, p.causal).first / kKeys * kKeys;
-#pragma unroll 1
-            for (int kk = from; kk < sees; ++kk) {
-              const uint32_t *v = reinterpret_cast<const uint32_t *>(
-                  p.v + (static_cast<int64_t>(it.k_row) + kk) * p.v_token + it.head * p.v_head + d + 32 * half);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const uint32_t w = v[e];
-                const float2 f = Elem<kBf16>::unpack(w);
-                if (!finite16<kBf16>(w & 0xffffu)) x[2 * e] = __float_as_uint(__uint_as_float(x[2 * e]) + f.x);
-                if (!finite16<kBf16>(w >> 16)) x[2 * e + 1] = __float_as_uint(__uint_as_float(x[2 * e + 1]) + f.y);
-              }
-            }
-          }
-          if (it.part > 0) {  // a part: as it is
-            const Parts<kDim> to_join = Parts<kDim>::of(p.workspace, p.parts_max);
-            const size_t tile = static_cast<size_t>(it.part - 1) * 2 + t;
-            if (live) {
-              if (d + half == 0) to_join.ml[tile * 128 + row] = make_float2(m, sum);
-              float4 *o = to_join.o + (tile * (kDim / 4) + (d + 32 * half) / 4) * 128 + row;
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                o[e * 128] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
-                                         __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
-            }
-            continue;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = Elem<kBf16>::pack(__uint_as_float(x[8 * e + 2 * i]) * inv, __uint_as_float(x[8 * e + 2 * i + 1]) * inv);
-            *reinterpret_cast<uint4 *>(stage + lane * 128 + (((4 * half + e) ^ (lane & 7)) * 16)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        if (it.part > 0) {
-        } else if (boxed) {
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4 *>(stage + lane * 128 + ((e ^ (lane & 7)) * 16)) =
+              make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        if (boxed) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
