@@ -11,7 +11,7 @@
 // operations an element. One thread moves one unit of 16 channels as two 16-byte chunks: the two
 // halves of 8 rotated pairs, or 32 contiguous bytes where nothing turns; a unit's row and head come from
 // products by a precomputed reciprocal (64-bit divisions kept the kernel issue-bound: 66 us for 375 MB,
-// 59 without).
+// 58 without: 6.4 TB/s, 98 % of a plain copy's rate).
 #include "sequence.cuh"
 
 namespace dv3 {
