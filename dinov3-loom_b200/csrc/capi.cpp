@@ -508,6 +508,7 @@ int64_t used_stride(int64_t stride, uint32_t extent) { return extent > 1 ? strid
 
 bool strides_ok(int64_t row, uint32_t rows, int64_t head, uint32_t heads) {
   constexpr int64_t kMost = int64_t{1} << 38;  // a tensor map's strides stay below 2^40 bytes
+  if (rows == 0) return true;
   row = used_stride(row, rows);
   head = used_stride(head, heads);
   return row > 0 && head > 0 && row % 8 == 0 && head % 8 == 0 && row < kMost && head < kMost;
@@ -520,6 +521,7 @@ bool words_aligned(P... p) {
 
 // No two (row, head) vectors of `dim` elements share memory.
 bool rows_apart(int64_t row, uint32_t rows, int64_t head, uint32_t heads, uint32_t dim) {
+  if (rows == 0) return true;
   if (rows > 1 && row < dim) return false;
   if (heads > 1 && head < dim) return false;
   if (rows <= 1 || heads <= 1) return true;
@@ -627,9 +629,9 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
   p.q_token = used_stride(a->q_token, a->total_q);
   p.q_head = used_stride(a->q_head, a->q_heads);
   p.k_token = used_stride(a->k_token, a->total_k);
-  p.k_head = used_stride(a->k_head, a->kv_heads);
+  p.k_head = used_stride(a->k_head, a->total_k ? a->kv_heads : 0);
   p.v_token = used_stride(a->v_token, a->total_k);
-  p.v_head = used_stride(a->v_head, a->kv_heads);
+  p.v_head = used_stride(a->v_head, a->total_k ? a->kv_heads : 0);
   p.out_token = used_stride(a->out_token, a->total_q);
   p.out_head = used_stride(a->out_head, a->q_heads);
   p.status = a->status;

@@ -300,6 +300,16 @@ def test_packed_nothing_to_do():
 
 
 # ---- the cache -------------------------------------------------------------------------------
+@dims
+def test_packed_empty_tensors_with_strides_of_nothing(dim):
+    """[heads, 0, dim] seen as [0, heads, dim] has a head stride of 0."""
+    none = torch.empty(4, 0, dim, device=DEV, dtype=torch.float16).transpose(0, 1)
+    q, cu, some = randn(gen(16), 5, 4, dim, dtype=torch.float16), ints([0, 0, 0]), ints([0, 2, 5])
+    assert dv.attention_packed(none, q, q, cu, some).shape == (0, 4, dim)
+    assert (dv.attention_packed(q, none, none, some, cu) == 0).all()
+    assert dv.attention_packed(none, none, none, cu).shape == (0, 4, dim)
+
+
 def paged_cache(seed, lens, hkv, page, dim, dtype, wide=0, joined=False):
     """A shuffled table (unused entries -1) over random pages; `joined`: k and v in one pool."""
     g = gen(seed)
@@ -370,6 +380,19 @@ def test_paged_long_and_any_bound(max_len, dtype):
     check_paged(q, k, v, table, lens, out, lse, 128 ** -0.5)
     again = dv.attention_paged(q, k, v, table, ints(lens), max_len=max_len)
     assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("hq,hkv,longest", [(4, 2, 700), (33, 1, 400), (3, 3, 2000)])
+@dims
+def test_paged_many_sequences(hq, hkv, longest, dim):
+    """More sequences than a block has threads, empty ones among them, in a workspace that holds NaN."""
+    g = gen(26 + dim)
+    lens = torch.randint(0, longest, (300,), generator=g, device=DEV).tolist()
+    lens[:3], lens[100:104], lens[-2:] = [0, 0, longest], [0, 0, 0, 1], [longest, 0]
+    k, v, table = paged_cache(27, lens, hkv, 16, dim, torch.bfloat16)
+    q, lse = randn(g, len(lens), hq, dim, dtype=torch.bfloat16), torch.empty(len(lens), hq, device=DEV)
+    out = dv.attention_paged(q, k, v, table, ints(lens), lse=lse, workspace=torch.full((1 << 26,), 255, dtype=torch.uint8, device=DEV))
+    check_paged(q, k, v, table, lens, out, lse, dim ** -0.5)
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf])

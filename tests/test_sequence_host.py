@@ -97,11 +97,12 @@ def test_null_arguments_and_nothing_to_do():
     assert lib.dv3k_attention_paged_workspace(None) == 0 and lib.dv3k_attention_packed_workspace(None) == 0
     few = dict(packed_ok, total_k=1024)
     assert lib.dv3k_attention_packed_workspace(PACKED_STRUCT.pack(*(few[f] for f in PACKED))) == 0  # nothing long to cut
-    for changes in (dict(n_seq=0), dict(total_q=0, q=0, out=0)):
+    for changes in (dict(n_seq=0), dict(total_q=0, q=0, out=0), dict(total_q=0, q_head=0, out_token=0)):
         assert call("dv3k_attention_packed", PACKED_STRUCT, PACKED, dict(packed_ok, **changes))[0] == 0
-    for changes in (dict(n_seq=0), dict(total=0, q=0, k=0)):
+    for changes in (dict(n_seq=0), dict(total=0, q=0, k=0), dict(total=0, q_head=0, q_out_head=0, k_token=0)):
         assert call("dv3k_rope_append", APPEND_STRUCT, APPEND, dict(append_ok, **changes))[0] == 0
     assert call("dv3k_attention_paged", PAGED_STRUCT, PAGED, dict(paged_ok, n_seq=0, q=0))[0] == 0
+    assert call("dv3k_attention_paged", PAGED_STRUCT, PAGED, dict(paged_ok, n_seq=0, q_head=0, out_head=0))[0] == 0
 
 
 def test_structs_match_the_header(tmp_path):
