@@ -24,7 +24,10 @@
 //     output) in the workspace, at most two a warp, and a second launch joins them in order.
 //     Nothing depends on the order in which warps end.
 //   - Where no sequence passes 256 keys, stretches are whole units and there is nothing to join; with
-//     no more units than CTAs, the four warps of a CTA share one and join in shared memory.
+//     no more units than CTAs, the four warps of a CTA share one and join in shared memory. So do
+//     the warps of a cluster of 2 to 8 CTAs where units are few and not so long that the rest of the
+//     SMs is missed: that spares the second launch (one sequence of 1000 keys, 32/8 heads of 128: 7.7 us,
+//     10.7 with it; 2500 keys 10.6 and 11.2; 5000 keys would take 15.6 and not 12.7).
 // Four warps on one 64-key tile, meeting at barriers, took 24.8 us for 256 images of 201 tokens and
 // 51.5 us for 64 sequences of 1..4096 (32/8 heads of 128); these take 18 and 39. One sequence of 131072 tokens takes 96 us (5.6 TB/s with its join).
 #include <atomic>
@@ -41,6 +44,7 @@ constexpr int kTile = 16;  // keys
 constexpr uint32_t kLeast = 4;   // tiles that a warp takes at least
 constexpr uint32_t kShort = 16;  // tiles up to which a unit is not split
 constexpr uint32_t kUnit = 2;    // what a unit's start and end cost, in tiles
+constexpr uint32_t kJoinTiles = 4;  // what the joining launch costs, in a warp's tiles
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A warp's shared memory: stages of K and V, and the addresses of the rows of the tiles in flight
@@ -55,6 +59,21 @@ struct Ring {
   static constexpr int kPerSm = kDim == 64 ? 3 : 2;  // CTAs
 };
 
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared memory location in the cluster's CTA `rank`, and a load from there.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t to;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+  return to;
+}
+__device__ __forceinline__ float2 load_cta(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -104,7 +123,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 struct Plan {
   uint32_t grid, head_blocks, rows;  // rows: query heads of a unit at most
   bool units;                        // stretches are whole units
-  bool team;                         // a CTA's four warps share one unit, every fourth tile each
+  bool team;                         // the warps of a cluster of CTAs share one unit, a tile each in turn
+  uint32_t cluster, log;             // its CTAs, and their number's logarithm
   bool crowd;                        // many stretches share a unit
 };
 
@@ -119,11 +139,22 @@ Plan plan_of(const PagedAttention &p) {
   s.rows = group < 16 ? group : 16;
   const uint64_t units = static_cast<uint64_t>(p.n_seq) * s.head_blocks;
   const uint64_t tiles = (static_cast<uint64_t>(p.max_len) + kTile - 1) / kTile;
-  s.units = tiles <= kShort;
-  s.team = s.units && units <= slots;
+  // Few long units: a cluster each, whose warps take tiles in turn and meet in its shared memory, where
+  // that costs a warp less than kJoinTiles more than an equal share of all tiles.
+  s.cluster = 1;
+  s.log = 0;
+  if (tiles > kShort)
+    for (uint32_t log = 3, c = 8; c > 1; c /= 2, --log)
+      if (units * c <= slots && tiles / (c * kWarps) <= tiles * units / (slots * kWarps) + kJoinTiles) {
+        s.cluster = c;
+        s.log = log;
+        break;
+      }
+  s.units = tiles <= kShort || s.cluster > 1;
+  s.team = s.cluster > 1 || (s.units && units <= slots);
   // as many CTAs as run at once, but no warp for less than a unit or kLeast tiles
   const uint64_t warps = s.units ? units : units * ((tiles + kLeast - 1) / kLeast);
-  const uint64_t most = s.team ? units : (warps + kWarps - 1) / kWarps;
+  const uint64_t most = s.team ? units * s.cluster : (warps + kWarps - 1) / kWarps;
   s.grid = static_cast<uint32_t>(most < slots ? most : slots);
   s.crowd = !s.units && static_cast<uint64_t>(s.grid) * kWarps > 16 * units;
   return s;
@@ -198,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
   if (pl.units) {
     const uint64_t n = static_cast<uint64_t>(p.n_seq) * pl.head_blocks, warps = static_cast<uint64_t>(pl.grid) * kWarps;
     if (tid <= kWarps) {
-      const uint64_t u = pl.team ? blockIdx.x + (tid == kWarps) : n * (warp0 + tid) / warps;
+      const uint64_t u = pl.team ? (blockIdx.x >> pl.log) + (tid == kWarps) : n * (warp0 + tid) / warps;
       found[tid][0] = u / pl.head_blocks;
       found[tid][1] = u % pl.head_blocks;
       found[tid][2] = 0;
@@ -244,7 +275,8 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
     }
   }
   __syncthreads();
-  const uint32_t to = pl.team ? kWarps : warp + 1, step = pl.team ? kWarps : 1;
+  const uint32_t to = pl.team ? kWarps : warp + 1, step = pl.team ? kWarps * pl.cluster : 1;
+  const uint32_t rank = blockIdx.x & (pl.cluster - 1);  // in the cluster
   const uint32_t end_s = static_cast<uint32_t>(found[to][0]), end_hb = static_cast<uint32_t>(found[to][1]),
                  end_t = static_cast<uint32_t>(found[to][2]);
 
@@ -273,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
     enter(x);
   };
   Place ld = {static_cast<uint32_t>(found[warp][0]), static_cast<uint32_t>(found[warp][1]),
-              static_cast<uint32_t>(found[warp][2]) + (pl.team ? warp : 0), 0, 0, 0, 0};
+              static_cast<uint32_t>(found[warp][2]) + (pl.team ? rank * kWarps + warp : 0), 0, 0, 0, 0};
   enter(ld);
   Place at = ld;
   auto settle = [&] {  // to the next tile there is
@@ -516,25 +548,46 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
             to[r * kDim + 16 * n + ra + 8] = o[h][n][2 + e];
           }
         }
-      __syncthreads();
-      constexpr uint32_t kPairs = kDim / 2;
-      for (uint32_t x = tid; x < heads * kPairs; x += kThreads) {
-        const uint32_t r = x / kPairs, d = x % kPairs * 2;
-        float top = -INFINITY, sum = 0.f, a = 0.f, b = 0.f;
+      auto join = [&](auto many) {
+        // a partial result of the cluster's CTA c
+        auto part_of = [&](const void *here, uint32_t c) {
+          if constexpr (decltype(many)::value)
+            return load_cta(in_cta(smem_u32(here), c));
+          else
+            return *static_cast<const float2 *>(here);
+        };
+        const uint32_t ctas = decltype(many)::value ? pl.cluster : 1;
+        constexpr uint32_t kPairs = kDim / 2;
+        for (uint32_t x = rank * kThreads + tid; x < heads * kPairs; x += ctas * kThreads) {
+          const uint32_t r = x / kPairs, d = x % kPairs * 2;
+          float top = -INFINITY, sum = 0.f, a = 0.f, b = 0.f;
+#pragma unroll 2
+          for (uint32_t c = 0; c < ctas; ++c)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * 16 + r].x);
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_of(ml + w * 16 + r, c).x);
+#pragma unroll 2
+          for (uint32_t c = 0; c < ctas; ++c)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 part = ml[w * 16 + r], v = *reinterpret_cast<const float2 *>(to + (w * 16 + r) * kDim + d);
-          const float f = top == -INFINITY ? 1.f : ex2_approx(part.x - top);
-          sum = fmaf(part.y, f, sum);
-          a = fmaf(v.x, f, a);
-          b = fmaf(v.y, f, b);
+            for (int w = 0; w < kWarps; ++w) {
+              const float2 part = part_of(ml + w * 16 + r, c), v = part_of(to + (w * 16 + r) * kDim + d, c);
+              const float f = top == -INFINITY ? 1.f : ex2_approx(part.x - top);
+              sum = fmaf(part.y, f, sum);
+              a = fmaf(v.x, f, a);
+              b = fmaf(v.y, f, b);
+            }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint32_t *>(p.out + static_cast<int64_t>(at.s) * p.out_seq + (h0 + r) * p.out_head + d) =
+              Elem<kBf16>::pack(a * inv, b * inv);
+          if (p.lse && d == 0) p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = (top + log2f(sum)) * kLn2;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<uint32_t *>(p.out + static_cast<int64_t>(at.s) * p.out_seq + (h0 + r) * p.out_head + d) =
-            Elem<kBf16>::pack(a * inv, b * inv);
-        if (p.lse && d == 0) p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = (top + log2f(sum)) * kLn2;
+      };
+      if (pl.cluster > 1) {
+        cluster_sync();
+        join(std::true_type{});
+        cluster_sync();  // the others have read this CTA's shared memory
+      } else {
+        __syncthreads();
+        join(std::false_type{});
       }
       break;
     }
@@ -686,8 +739,19 @@ cudaError_t launch(const PagedAttention &p, const Plan &pl, cudaStream_t stream)
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
-  const cudaError_t e = launch_pdl(attention_paged_kernel<kBf16, kDim, kHeads8>, dim3(pl.grid), dim3(kThreads),
-                                   kWarps * Ring<kDim>::kBytes, stream, p, pl);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {pl.cluster, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kWarps * Ring<kDim>::kBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pl.cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attention_paged_kernel<kBf16, kDim, kHeads8>, p, pl);
   if (e != cudaSuccess || pl.units) return e;
   const uint32_t rows = p.n_seq * p.q_heads;  // below 2^31
   return pl.crowd ? launch_pdl(attention_paged_join_kernel<kBf16, kDim, 32>, dim3(rows), dim3(1024), 0, stream, p, pl)

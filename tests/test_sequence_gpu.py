@@ -382,6 +382,19 @@ def test_paged_long_and_any_bound(max_len, dtype):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (33, 1), (8, 8)])
+@pytest.mark.parametrize("lens", [[300], [257, 0], [1100, 300, 5], [700] * 9, [400, 1] * 12])
+@both
+@dims
+def test_paged_few_sequences(lens, hq, hkv, dtype, dim):
+    """Few units of medium length, whose blocks meet in a cluster; bounds below the lengths too."""
+    k, v, table = paged_cache(28, lens, hkv, 16, dim, dtype)
+    q, lse = randn(gen(29), len(lens), hq, dim, dtype=dtype) * 2, torch.empty(len(lens), hq, device=DEV)
+    for max_len in (None, 270):
+        out = dv.attention_paged(q, k, v, table, ints(lens), max_len=max_len, lse=lse.fill_(7.0))
+        check_paged(q, k, v, table, lens, out, lse, dim ** -0.5)
+
+
 @pytest.mark.parametrize("hq,hkv,longest", [(4, 2, 700), (33, 1, 400), (3, 3, 2000)])
 @dims
 def test_paged_many_sequences(hq, hkv, longest, dim):
