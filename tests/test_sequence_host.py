@@ -83,7 +83,7 @@ def test_append_refusals(text, changes):
 @pytest.mark.parametrize("text,changes", HEADS + CACHE + [
     ("q_heads", dict(q_heads=0)), ("too many", dict(n_seq=1 << 29)), ("scale", dict(scale=float("nan"))), ("strides", dict(q_seq=12)), ("overlap", dict(out_seq=128)),
     ("null", dict(out=0)), ("null", dict(lens=0)), ("aligned", dict(q=BASE + 8)), ("aligned", dict(workspace=BASE + 8)),
-    ("workspace", dict(max_pages=64, table_stride=64, max_len=1024)), ("4-byte", dict(lens=BASE + 2)), ("4-byte", dict(status=BASE + 1)),
+    ("workspace", dict(max_pages=4096, table_stride=4096, max_len=65536)), ("4-byte", dict(lens=BASE + 2)), ("4-byte", dict(status=BASE + 1)),
     ("out overlaps", dict(out=BASE)),
 ])
 def test_paged_refusals(text, changes):
