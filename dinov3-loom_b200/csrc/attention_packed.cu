@@ -53,6 +53,7 @@ constexpr int kGuardWarp = 11;
 constexpr int kBuckets = 64;    // of the scheduler's order
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;   // log2 units by which a row's maximum may pass its reference
+constexpr float kFar = 4096.f;  // log2 units from which on a reference is subtracted before the scale
 
 // One work item as the scheduler publishes it (two 16-byte words).
 struct __align__(16) Item {
@@ -357,21 +358,29 @@ __device__ __forceinline__ bool finite16(uint32_t half) {
   return (half & e) != e;
 }
 
-// A row's reference, moved to the step's maximum `now` (log2 units) where that passes it by more than
-// kSlack; the row's sum and output so far follow. The previous product is done: the thread that
+// What a row's weights are relative to: a score (`raw`), and that times c, rounded (`log`). The
+// rounding is a factor of all of the row's weights that its sum has too, below 2^(2^-12) while |log| <
+// kFar. Beyond, it may pass the exponent's range (at 2^32 it is up to 2^128): there the difference
+// from `raw` comes before the scale (`far`: a row of the warp is such a one). Subtracted from every score
+// it took 3 % of the long prompts' time.
+struct Reference {
+  float raw, log;
+  bool far;
+};
+// A row's reference, moved to the step's maximum `top` where that passes it by more than kSlack (after
+// the scale c); the row's sum and output so far follow. The previous product is done: the thread that
 // issued it issued these scores after it.
-__device__ __forceinline__ void move_reference(uint32_t to, int dim, float now, bool first, float &m,
-                                               float &sum) {
-  if (first) {
-    m = now;
-    return;
-  }
-  const bool grown = now > m + kSlack;
-  if (!__any_sync(0xffffffffu, grown)) return;
-  const float next = grown ? now : m;
-  const float f = grown ? ex2_approx(m - next) : 1.f;
+__device__ __forceinline__ void move_reference(uint32_t to, int dim, float c, float top, bool first,
+                                               Reference &r, float &sum) {
+  const float now = top * c;
+  const bool grown = now > r.log + kSlack;
+  if (!first && !__any_sync(0xffffffffu, grown)) return;
+  float f = ex2_approx((r.raw - top) * c);
+  if (first || grown) r.raw = top, r.log = now;
+  r.far = __any_sync(0xffffffffu, fabsf(r.log) >= kFar && r.log != -INFINITY);
+  if (first) return;
+  if (!grown) f = 1.f;
   sum *= f;
-  m = next;
 #pragma unroll 1
   for (int d = 0; d < dim; d += 16) {
     uint32_t x[16];
@@ -410,16 +419,16 @@ __device__ __forceinline__ void hand_over_weights(uint64_t *p_full) {
   if (threadIdx.x % 32 == 0) mbar_arrive(p_full);
 }
 
-// Scores, weights and sums of one step for this thread's row, through m (reference, log2 units) and
-// sum. Where some row of the tile sees the step in part (`masked`), this one sees `vis` keys of it
+// Scores, weights and sums of one step for this thread's row, through its reference m and sum; c is
+// scale log2(e). Where some row of the tile sees the step in part (`masked`), this one sees `vis` keys of it
 // and the tile `blocks` blocks of 32; the products skip the others. The weights are handed over in
 // two halves (p_full[0], p_full[2]), so that the product with V starts under the second. One form for
 // both kinds of step: two thrashed the instruction cache. loaded() is called when the scores are in
 // registers, before() before the output or the weights' columns (at tp) are touched.
 template <bool kBf16, int kBlocks, class Loaded, class Before>
 __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, float c, bool masked,
-                                             int vis, int blocks, bool first, float &m, float &sum,
-                                             uint32_t tp, uint64_t *p_full, Loaded &&loaded,
+                                             int vis, int blocks, bool first, Reference &m,
+                                             float &sum, uint32_t tp, uint64_t *p_full, Loaded &&loaded,
                                              Before &&before) {
   if (masked) {
     // what a row does not see becomes -inf in TMEM, in the blocks that some row of the warp sees in part
@@ -456,8 +465,22 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
 #pragma unroll
   for (int i = 1; i < kBlocks; ++i) top = fmaxf(top, tops[i]);
   if (!before()) return false;
-  move_reference(to, dim, top * c, first, m, sum);
-  const float base = m == -INFINITY ? 0.f : m;
+  move_reference(to, dim, c, top, first, m, sum);
+  float base = m.log == -INFINITY ? 0.f : m.log;
+  if (__builtin_expect(m.far, 0)) {
+    const bool far = fabsf(base) >= kFar;
+    const float from = far ? -m.raw : 0.f;
+    const uint64_t from2 = pair(from, from);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const float2 x = unpair(add2(pair(v[i][e], v[i][e + 1]), from2));
+        v[i][e] = __float_as_uint(x.x);
+        v[i][e + 1] = __float_as_uint(x.y);
+      }
+    if (far) base = 0.f;
+  }
   const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
   uint64_t s0 = 0, s1 = 0;
 #pragma unroll
@@ -965,7 +988,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int whole = r.first / kKeys;  // steps that every row of the tile sees in full
       const int mine = t * tokens + token;  // token within the item
       const int sees = p.causal ? min(seen.k_len, seen.visible + mine) : seen.k_len;
-      float m = -INFINITY, sum = 0.f;
+      Reference m = {-INFINITY, -INFINITY, false};
+      float sum = 0.f;
       for (int j = 0; j < r.steps; ++j) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], s_phase, abort_flag));
         if (!ok) break;
@@ -1010,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
       const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
       uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
-      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = (m + log2f(sum)) * kLn2;
+      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = (m.log + log2f(sum)) * kLn2;
       if (r.steps > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag));
         if (!ok) break;
@@ -1072,7 +1096,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Parts<kDim> to_join = Parts<kDim>::of(p.workspace, p.parts_max);
           const size_t tile = static_cast<size_t>(it.part - 1) * 2 + t;
           if (live) {
-            if (d == 0) to_join.ml[tile * 128 + row] = make_float2(m, sum);
+            if (d == 0) to_join.ml[tile * 128 + row] = make_float2(m.raw, sum);
             float4 *o = to_join.o + (tile * (kDim / 4) + d / 4) * 128 + row;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -1129,8 +1153,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of the cut items: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the parts in
-// order. The CTAs of a part take its share of the item's rows, 16 channels each: a thread for a row and
+// Joins the parts of the cut items: out = sum_i f_i o_i / sum_i f_i l_i, f_i = 2^(c (m_i - M)), over the
+// parts in order. The CTAs of a part take its share of the item's rows, 16 channels each: a thread for a row and
 // four channels, rows next to one another.
 template <bool kBf16, int kDim>
 __global__ void __launch_bounds__(256) attention_packed_join_kernel(const PackedArgs p) {
@@ -1156,7 +1180,7 @@ __global__ void __launch_bounds__(256) attention_packed_join_kernel(const Packed
       const size_t at = static_cast<size_t>(first) + i * p.kv_heads;
       const float2 ml = w.ml[at * 256 + row];
       if (ml.x == -INFINITY && ml.y == 0.f) continue;  // sees none of the part's keys
-      const float f = top == -INFINITY ? 1.f : ex2_approx(ml.x - top);
+      const float f = top == -INFINITY ? 1.f : ex2_approx((ml.x - top) * p.scale_log2);
       const float4 v = w.o[((at * 2 + t) * (kDim / 4) + d4) * 128 + in];
       sum = fmaf(ml.y, f, sum);
       acc.x = fmaf(v.x, f, acc.x);
@@ -1169,7 +1193,7 @@ __global__ void __launch_bounds__(256) attention_packed_join_kernel(const Packed
     const uint32_t head = part.head * p.group + in % p.group;
     *reinterpret_cast<uint2 *>(p.out + out_row * p.out_token + head * p.out_head + 4 * d4) =
         make_uint2(Elem<kBf16>::pack(acc.x * inv, acc.y * inv), Elem<kBf16>::pack(acc.z * inv, acc.w * inv));
-    if (p.lse && d4 == 0) p.lse[out_row * p.q_heads + head] = (top + log2f(sum)) * kLn2;
+    if (p.lse && d4 == 0) p.lse[out_row * p.q_heads + head] = (top * p.scale_log2 + log2f(sum)) * kLn2;
   }
 }
 

@@ -481,12 +481,13 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             top = fmaxf(top, m[h][e]);
-            const float base = top == -INFINITY ? 0.f : top * c2;
-            keep[h][e] = ex2_approx(fmaf(m[h][e], c2, -base));
+            // differences before the scale: a rounded top c2 may be off by more than the exponent's range
+            const float from = top == -INFINITY ? 0.f : top;
+            keep[h][e] = ex2_approx((m[h][e] - from) * c2);
             moved |= top != m[h][e];
             m[h][e] = top;
-            p4[e] = ex2_approx(fmaf(s4[e], c2, -base));
-            p4[2 + e] = ex2_approx(fmaf(s4[2 + e], c2, -base));
+            p4[e] = ex2_approx((s4[e] - from) * c2);
+            p4[2 + e] = ex2_approx((s4[2 + e] - from) * c2);
             l[h][e] = fmaf(l[h][e], keep[h][e], p4[e] + p4[2 + e]);
           }
           w[h][0] = transposed(Elem<kBf16>::pack(p4[0], p4[1]));
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t r = warp * 16 + 8 * h + cq + e;
-          if (ra == 0) ml[r] = make_float2(m[h][e] * c2, l[h][e]);
+          if (ra == 0) ml[r] = make_float2(m[h][e], l[h][e]);
 #pragma unroll
           for (int n = 0; n < kSteps; ++n) {
             to[r * kDim + 16 * n + ra] = o[h][n][e];
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
               const float2 part = part_of(ml + w * 16 + r, c), v = part_of(to + (w * 16 + r) * kDim + d, c);
-              const float f = top == -INFINITY ? 1.f : ex2_approx(part.x - top);
+              const float f = top == -INFINITY ? 1.f : ex2_approx((part.x - top) * c2);
               sum = fmaf(part.y, f, sum);
               a = fmaf(v.x, f, a);
               b = fmaf(v.y, f, b);
@@ -578,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           *reinterpret_cast<uint32_t *>(p.out + static_cast<int64_t>(at.s) * p.out_seq + (h0 + r) * p.out_head + d) =
               Elem<kBf16>::pack(a * inv, b * inv);
-          if (p.lse && d == 0) p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = (top + log2f(sum)) * kLn2;
+          if (p.lse && d == 0) p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = (top * c2 + log2f(sum)) * kLn2;
         }
       };
       if (pl.cluster > 1) {
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
           const uint32_t r = 8 * h + cq + e;
           if (r >= heads) continue;
           const size_t to = ((warp0 + warp) * 2 + slot) * pl.rows + r;
-          if (ra == 0) part.ml[to] = make_float2(m[h][e] * c2, l[h][e]);
+          if (ra == 0) part.ml[to] = make_float2(m[h][e], l[h][e]);
 #pragma unroll
           for (int n = 0; n < kSteps; ++n) {
             part.o[to * kDim + 16 * n + ra] = o[h][n][e];
@@ -633,8 +634,8 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
   cp_async_wait<0>();
 }
 
-// Joins the units that several stretches share: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over
-// the stretches i in order; and writes the rows of empty sequences. kJoin warps take every kJoin-th
+// Joins the units that several stretches share: out = sum_i f_i o_i / sum_i f_i l_i, f_i =
+// 2^(c (m_i - M)), over the stretches i in order; and writes the rows of empty sequences. kJoin warps take every kJoin-th
 // part of a (sequence, query head), then meet in shared memory: 4 where units have few parts, 32
 // where they have more than 16 (4 warps took 20 us for 148 parts; 32, or a single one, 2 to 4 us
 // more than 4 for the few parts of 64 sequences of 1..4096 tokens). What a unit's parts are the first
@@ -652,6 +653,7 @@ __global__ void __launch_bounds__(kJoin * 32)
   const uint32_t hb = h / group * blocks + h % group / 16, r = h % group % 16;
   pdl_wait();
   pdl_trigger();
+  const float c2 = p.scale * kLog2e;
   const Partials w = partials_of(p, pl);
   Share share = w.shares[static_cast<size_t>(s) * pl.head_blocks + hb];  // of an empty one: not read
   if (cached_tokens(p, s, false) == 0) share = {0, 0};
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(kJoin * 32)
   for (int i = 16; i > 0; i /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
   float sum = 0.f, acc[kLane] = {};
   auto add = [&](const float2 &x, const float(&o)[kLane]) {
-    const float f = top == -INFINITY ? 1.f : ex2_approx(x.x - top);
+    const float f = top == -INFINITY ? 1.f : ex2_approx((x.x - top) * c2);
     sum = fmaf(x.y, f, sum);
 #pragma unroll
     for (int e = 0; e < kLane; ++e) acc[e] = fmaf(o[e], f, acc[e]);
@@ -715,7 +717,7 @@ __global__ void __launch_bounds__(kJoin * 32)
 #pragma unroll
   for (int e = 0; e < kLane; e += 2)
     *reinterpret_cast<uint32_t *>(dst + e) = Elem<kBf16>::pack(acc[e] * inv, acc[e + 1] * inv);
-  if (p.lse && lane == 0) p.lse[row] = (top + log2f(sum)) * kLn2;
+  if (p.lse && lane == 0) p.lse[row] = (top * c2 + log2f(sum)) * kLn2;
 }
 
 size_t attention_paged_workspace(const PagedAttention &p) {

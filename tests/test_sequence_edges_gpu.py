@@ -1,0 +1,81 @@
+"""Packed attention, rotated cache append and paged attention where their numbers and their arguments
+reach an edge: scores beyond f32's integers, weights far below the largest, overlapping memory,
+gradients that would be lost. Bounds are derived beside each test, with u = finfo(dtype).eps / 2.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+import dinov3_b200 as dv  # noqa: E402
+from test_sequence_gpu import DEV, both, check, cu_of, dims, gen, ints, paged_cache, randn  # noqa: E402
+
+
+def fill_cache(keys, values, page, pool_seed):
+    """Paged caches [pages, heads, page, dim] that hold the rows [n, heads, dim], and their table."""
+    n, heads, dim = keys.shape
+    k, v, table = paged_cache(pool_seed, [n], heads, page, dim, keys.dtype)
+    pos = torch.arange(n, device=DEV)
+    ids, slot = table[0].long()[pos // page], pos % page
+    k[ids, :, slot], v[ids, :, slot] = keys, values
+    return k, v, table
+
+
+def every_form(q, k, v, scale):
+    """(name, out, lse) of one query row over keys [n, heads, dim] by each way there is to ask for it."""
+    n, hq = k.shape[0], q.shape[1]
+    for name, causal in (("packed", False), ("packed causal", True)):
+        lse = torch.empty(1, hq, device=DEV)
+        out = dv.attention_packed(q, k, v, ints([0, 1]), ints([0, n]), causal=causal, scale=scale, lse=lse)
+        yield name, out[0], lse[0]
+    kc, vc, table = fill_cache(k, v, 16, 90)
+    for max_len in (n, 256, 1 << 20):
+        wide = torch.full((1, -(-max_len // 16)), -1, dtype=torch.int32, device=DEV)  # the table bounds max_len
+        wide[:, :min(table.shape[1], wide.shape[1])] = table[:, :wide.shape[1]]
+        if wide.shape[1] < table.shape[1]:
+            wide = table
+        lse = torch.empty(1, hq, device=DEV)
+        out = dv.attention_paged(q, kc, vc, wide, ints([n]), max_len=max_len, scale=scale, lse=lse)
+        yield f"paged, bound {max_len}", out[0], lse[0]
+
+
+# ---- scores past f32's integers --------------------------------------------------------------
+@pytest.mark.parametrize("n", [40, 300, 5000])
+@pytest.mark.parametrize("order", ["up", "down", "twice"])
+@dims
+@both
+def test_scores_far_beyond_one(n, order, dim, dtype):
+    """q . k of 2^28 to 2^30 and 2^90 to 2^92, exact in f32 (one channel, short mantissas): the one largest score has
+    all the weight, two equal ones half each. Any score differs from the largest by more than 2^20, so
+    that the others' weights are exactly 0, and the result is that value, or the mean of two, rounded once."""
+    g = gen(80)
+    big = 2.0 ** 15 if dtype == torch.float16 else 2.0 ** 46
+    hq, hkv = 6, 2
+    steps = torch.arange(n, device=DEV) % 64
+    x = (1 + steps / 64.0) if order == "up" else (2 - steps / 64.0)  # 7 bits
+    x = x.clamp(max=1.9375)
+    x[n // 3] = 1.96875  # the largest: 1 + 31/32
+    if order == "twice":
+        x[n - 2] = 1.96875
+    k = torch.zeros(n, hkv, dim, device=DEV, dtype=dtype)
+    k[:, :, 3] = (x * big / 2)[:, None].to(dtype)
+    assert torch.equal(k[:, 0, 3].float(), x * big / 2)
+    q = torch.zeros(1, hq, dim, device=DEV, dtype=dtype)
+    q[0, :, 3] = (torch.tensor([1, 1.125, 1.25, 1.375, 1.5, 1.75], device=DEV) * big / 2).to(dtype)
+    v = randn(g, n, hkv, dim, dtype=dtype)
+    top = v[n // 3].double()
+    if order == "twice":
+        top = (top + v[n - 2].double()) / 2
+    top = top.repeat_interleave(hq // hkv, 0)
+    for scale in (1.0, 0.125, 777.0):
+        score = q[0, :, 3].double() * (1.96875 * big / 2) * torch.tensor(scale, dtype=torch.float32).double().to(DEV)
+        want_lse = score + (math.log(2.0) if order == "twice" else 0.0)
+        for name, out, lse in every_form(q, k, v, scale):
+            check(out, top, top.abs() * torch.finfo(dtype).eps / 2 + (2.0 ** -25 if dtype == torch.float16 else 0.0), name)
+            # scale log2(e), its product with the score and that with ln 2 are rounded to f32
+            check(lse, want_lse, want_lse.abs() * 2.0 ** -21, name + ", log-sum")
