@@ -18,8 +18,8 @@
 //              2^(s c - m c) with c = scale log2(e), f32 sum of the unrounded weights, P (rounded to
 //              the element type) back to TMEM over the consumed scores. The reference m only moves
 //              when the maximum has grown by more than 2^8 over it: any m gives the same quotient,
-//              and sums and weights up to 2^8 too large lose nothing in f32, f16 or bf16; the row's
-//              output is then rescaled in TMEM. At an item's end O / sum goes through a staging
+//              and sums and weights up to 2^8 too large lose nothing in f32, bf16 or f16 (whose
+//              weights end at 2^15, see sequence.cuh); the row's output is then rescaled in TMEM. At an item's end O / sum goes through a staging
 //              tile to global memory. Of a last, partly visible step only the blocks of 32 keys
 //              that some row sees are computed.
 //   warp 8     TMA producer: Q tiles, then K and V tiles in turn through one ring of stages.
@@ -51,8 +51,10 @@ constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;  // TMEM allocator; issues tile 0's MMAs, warp 10 tile 1's
 constexpr int kGuardWarp = 11;
 constexpr int kBuckets = 64;    // of the scheduler's order
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 8.f;   // log2 units by which a row's maximum may pass its reference
+// Log2 units by which a row's maximum may pass its reference. 4 would leave f16 weights four bits more
+// below the largest, but moved the references of 8192 causal tokens (32/8 heads of 128) so much more
+// often that they took 665 us and not 569.
+constexpr int kSlack = 8;
 constexpr float kFar = 4096.f;  // log2 units from which on a reference is subtracted before the scale
 
 // One work item as the scheduler publishes it (two 16-byte words).
@@ -393,7 +395,7 @@ __device__ __forceinline__ void move_reference(uint32_t to, int dim, float c, fl
   }
 }
 
-// The weights of 32 scores, 2^(s c - base), stored over consumed scores and added to (s0, s1).
+// The weights of 32 scores, 2^(s c + base), stored over consumed scores and added to (s0, s1).
 template <bool kBf16>
 __device__ __forceinline__ void weigh(uint32_t to, const uint32_t (&v)[32], uint64_t c2,
                                       uint64_t base2, uint64_t &s0, uint64_t &s1) {
@@ -481,7 +483,8 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
       }
     if (far) base = 0.f;
   }
-  const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
+  base = weight_shift<kBf16>(kSlack) - base;
+  const uint64_t c2 = pair(c, c), base2 = pair(base, base);
   uint64_t s0 = 0, s1 = 0;
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) {
@@ -1034,7 +1037,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
       const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
       uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
-      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = (m.log + log2f(sum)) * kLn2;
+      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = log_sum<kBf16>(m.log, sum, kSlack);
       if (r.steps > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag));
         if (!ok) break;
@@ -1193,7 +1196,7 @@ __global__ void __launch_bounds__(256) attention_packed_join_kernel(const Packed
     const uint32_t head = part.head * p.group + in % p.group;
     *reinterpret_cast<uint2 *>(p.out + out_row * p.out_token + head * p.out_head + 4 * d4) =
         make_uint2(Elem<kBf16>::pack(acc.x * inv, acc.y * inv), Elem<kBf16>::pack(acc.z * inv, acc.w * inv));
-    if (p.lse && d4 == 0) p.lse[out_row * p.q_heads + head] = (top * p.scale_log2 + log2f(sum)) * kLn2;
+    if (p.lse && d4 == 0) p.lse[out_row * p.q_heads + head] = log_sum<kBf16>(top * p.scale_log2, sum, kSlack);
   }
 }
 

@@ -45,7 +45,6 @@ constexpr uint32_t kLeast = 4;   // tiles that a warp takes at least
 constexpr uint32_t kShort = 16;  // tiles up to which a unit is not split
 constexpr uint32_t kUnit = 2;    // what a unit's start and end cost, in tiles
 constexpr uint32_t kJoinTiles = 4;  // what the joining launch costs, in a warp's tiles
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A warp's shared memory: stages of K and V, and the addresses of the rows of the tiles in flight
 // and the next (8-byte pointers into K and V; 0: no such row).
@@ -374,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
 
   const uint32_t ra = lane / 4, cq = 2 * (lane % 4);
   const float c2 = p.scale * kLog2e;
+  constexpr float kShift = weight_shift<kBf16>(0);
   // Q^T as the products' B operand: head lane / 4 of each 8, channels 2 (lane % 4) of each half step
   uint32_t q[kHeads8][kSteps][2], qn[kHeads8][kSteps][2];
   auto load_q = [&](uint32_t s, uint32_t hb) {
@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
             keep[h][e] = ex2_approx((m[h][e] - from) * c2);
             moved |= top != m[h][e];
             m[h][e] = top;
-            p4[e] = ex2_approx((s4[e] - from) * c2);
-            p4[2 + e] = ex2_approx((s4[2 + e] - from) * c2);
+            p4[e] = ex2_approx(fmaf(s4[e] - from, c2, kShift));
+            p4[2 + e] = ex2_approx(fmaf(s4[2 + e] - from, c2, kShift));
             l[h][e] = fmaf(l[h][e], keep[h][e], p4[e] + p4[2 + e]);
           }
           w[h][0] = transposed(Elem<kBf16>::pack(p4[0], p4[1]));
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           *reinterpret_cast<uint32_t *>(p.out + static_cast<int64_t>(at.s) * p.out_seq + (h0 + r) * p.out_head + d) =
               Elem<kBf16>::pack(a * inv, b * inv);
-          if (p.lse && d == 0) p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = (top * c2 + log2f(sum)) * kLn2;
+          if (p.lse && d == 0) p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + r] = log_sum<kBf16>(top * c2, sum, 0);
         }
       };
       if (pl.cluster > 1) {
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
         for (int e = 0; e < 2; ++e) {
           inv[e] = l[h][e] == 0.f ? 0.f : 1.f / l[h][e];
           if (p.lse && ra == 0 && 8 * h + cq + e < heads)
-            p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + 8 * h + cq + e] = (m[h][e] * c2 + log2f(l[h][e])) * kLn2;
+            p.lse[static_cast<int64_t>(at.s) * p.q_heads + h0 + 8 * h + cq + e] = log_sum<kBf16>(m[h][e] * c2, l[h][e], 0);
         }
         uint16_t *dst = p.out + static_cast<int64_t>(at.s) * p.out_seq + (h0 + 8 * h + ra) * p.out_head + cq;
 #pragma unroll
@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(kJoin * 32)
 #pragma unroll
   for (int e = 0; e < kLane; e += 2)
     *reinterpret_cast<uint32_t *>(dst + e) = Elem<kBf16>::pack(acc[e] * inv, acc[e + 1] * inv);
-  if (p.lse && lane == 0) p.lse[row] = (top * c2 + log2f(sum)) * kLn2;
+  if (p.lse && lane == 0) p.lse[row] = log_sum<kBf16>(top * c2, sum, 0);
 }
 
 size_t attention_paged_workspace(const PagedAttention &p) {

@@ -28,6 +28,23 @@ struct Elem<true> {
   }
 };
 
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// The softmax's weights are rounded to the element type, as which the tensor cores take them; their sum is
+// of the unrounded ones. bf16 has f32's range. In f16 a weight 17 e-folds below the largest would
+// be lost if that were 1 (one strong key before 2^17 weak ones: results 16 to 20 % off), so weights and
+// sum carry a factor 2^shift that leaves the largest 2^15: f16 ends at 65504, `slack` is how far (log2) a
+// weight may pass its reference, and the factor drops out of their quotient.
+template <bool kBf16>
+__host__ __device__ constexpr int weight_shift(int slack) {
+  return kBf16 ? 0 : 15 - slack;
+}
+// log of the unshifted sum: reference (log2 units) and sum of such weights.
+template <bool kBf16>
+__device__ __forceinline__ float log_sum(float reference, float sum, int slack) {
+  return (reference + log2f(sum * (1.f / (1 << weight_shift<kBf16>(slack))))) * kLn2;
+}
+
 // Rows [begin, end) of packed sequence s, clamped to the tensor's rows whatever cu holds (NULL:
 // one row per sequence).
 __device__ __forceinline__ void sequence_rows(const int32_t *cu, uint32_t s, uint32_t total,

@@ -202,7 +202,8 @@ int dv3k_matmul_swiglu(const uint16_t *h, uint32_t rows, const uint16_t *gateup_
  *   - `dtype` is DV3K_F16 or DV3K_BF16 and holds for every 16-bit tensor of the call; head_dim is
  *     64 or 128; q_heads is a multiple of kv_heads, at most 128 times it, and query head h reads
  *     key-value head h / (q_heads / kv_heads). Scores, the softmax's maximum and sum and every
- *     product's sum are f32; the weights are rounded to `dtype` before the product with v.
+ *     product's sum are f32; the weights are rounded to `dtype` before the product with v (f16
+ *     weights scaled, so that those down to 2^-31 of the largest count).
  *   - A row tensor [rows][heads][head_dim] is given by its row (token) and head strides in
  *     elements, multiples of 8, with head_dim contiguous. Rows or heads of an output do not
  *     overlap, nor does an output overlap an input (but q_out of dv3k_rope_append may be q); arrays of

@@ -79,3 +79,25 @@ def test_scores_far_beyond_one(n, order, dim, dtype):
             check(out, top, top.abs() * torch.finfo(dtype).eps / 2 + (2.0 ** -25 if dtype == torch.float16 else 0.0), name)
             # scale log2(e), its product with the score and that with ln 2 are rounded to f32
             check(lse, want_lse, want_lse.abs() * 2.0 ** -21, name + ", log-sum")
+
+
+# ---- float16 weights far below the largest ---------------------------------------------------
+@pytest.mark.parametrize("n,gap", [(300, 15.5), (8192, 15.5), (8192, 17.0), (8192, 19.0)])
+@pytest.mark.parametrize("strong", ["first", "middle", "last"])
+@dims
+def test_many_weak_keys_beside_a_strong_one(n, gap, strong, dim):
+    """One key of value 0 and n - 1 keys of value 1 whose scores lie `gap` below it, in float16: each weak
+    weight is below the smallest step 2^-24 of a format in which the strong one is 1, and together
+    they are the result. The kernels scale the weights by 2^15, or (packed, whose reference may lie
+    2^8 below the maximum) by 2^7 at least: steps of 2^-31, each weight off by half of one."""
+    at = {"first": 0, "middle": n // 2, "last": n - 1}[strong]
+    q, k, v = (torch.zeros(r, 2, dim, device=DEV, dtype=torch.float16) for r in (1, n, n))
+    q[0, :, 5], k[:, :, 5], v[:] = 1.0, -gap, 1.0
+    k[at, :, 5], v[at] = 0.0, 0.0
+    weak = (n - 1) * math.exp(-gap)
+    want = torch.full((2, dim), weak / (1 + weak), device=DEV, dtype=torch.float64)
+    u = 2.0 ** -11
+    tol = (2 * u + 2.0 ** -16) * want + n * 2.0 ** -32 + 2.0 ** -25
+    for name, out, lse in every_form(q, k, v, 1.0):
+        check(out, want, tol, name)
+        check(lse, torch.full((2,), math.log1p(weak), device=DEV, dtype=torch.float64), torch.full((2,), n * 2.0 ** -24 + 2.0 ** -20, device=DEV, dtype=torch.float64), name + ", log-sum")
