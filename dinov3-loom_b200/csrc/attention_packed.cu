@@ -38,9 +38,11 @@
 // tokens, 6 heads of 64, f16, 23.4 us (14.2 in the steady state of a larger batch).
 //
 // Every wait is bounded; on a timeout the kernel records kErrAttentionWait, raises the CTA's
-// abort flag, lets its own copies and MMAs in flight land, frees TMEM and returns.
+// abort flag, lets its own copies and MMAs in flight land, frees TMEM and returns; the join then leaves
+// the cut items' rows as they were.
 #include <atomic>
 
+#include "packed_parts.h"
 #include "sequence.cuh"
 
 namespace dv3 {
@@ -195,32 +197,6 @@ struct PackedArgs {
   float scale_log2;
 };
 
-// Workspace of the cut items: the parts' number, then for each part what it is, (max, sum) of its
-// 2 x 128 rows, and their outputs, four channels of 128 rows after another.
-struct Part {
-  int32_t q_row, q_count, head, index, parts;
-  int32_t unused[3];
-};
-template <int kDim>
-struct Parts {
-  uint32_t *count;
-  Part *what;
-  float2 *ml;   // [part][2][128]
-  float4 *o;    // [part][2][kDim / 4][128]
-  __host__ __device__ static size_t bytes(uint32_t n) {
-    return 16 + static_cast<size_t>(n) * (sizeof(Part) + 256 * sizeof(float2) + 256 * kDim * sizeof(float));
-  }
-  __device__ static Parts of(void *workspace, uint32_t n) {
-    Parts p;
-    uint8_t *at = static_cast<uint8_t *>(workspace);
-    p.count = reinterpret_cast<uint32_t *>(at);
-    p.what = reinterpret_cast<Part *>(at + 16);
-    p.ml = reinterpret_cast<float2 *>(p.what + n);
-    p.o = reinterpret_cast<float4 *>(p.ml + static_cast<size_t>(n) * 256);
-    return p;
-  }
-};
-
 namespace {
 // A sequence as the scheduler sees it: `n` items of 2 p.tokens query tokens for one key-value head.
 struct Sequence {
@@ -259,6 +235,7 @@ __device__ __forceinline__ uint32_t parts_of(uint32_t c, uint32_t width, uint32_
 }
 
 // Entry `index` of the order, for key-value head `head`; whole warp.
+template <int kDim>
 __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_t index, uint32_t head) {
   const uint32_t lane = threadIdx.x & 31u;
   Item it = {};
@@ -307,7 +284,7 @@ __device__ __forceinline__ Item find_item(const PackedArgs &p, Order &o, uint32_
         const uint32_t place = index * p.kv_heads + head;
         it.part = static_cast<int32_t>(place) + 1;
         if (lane == 0) {
-          Part *w = reinterpret_cast<Part *>(static_cast<uint8_t *>(p.workspace) + 16) + place;
+          Part *w = Parts<kDim>::of(p.workspace, p.parts_max).what + place;
           w->q_row = it.q_row;
           w->q_count = it.q_count;
           w->head = it.head;
@@ -647,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       Item it = {};
       if (at < n_items)
-        it = find_item(p, o, static_cast<uint32_t>(at / p.kv_heads), static_cast<uint32_t>(at % p.kv_heads));
+        it = find_item<kDim>(p, o, static_cast<uint32_t>(at / p.kv_heads), static_cast<uint32_t>(at % p.kv_heads));
       // the up-and-down order may leave one CTA an item in a round in which others have none
       if (static_cast<uint64_t>(k) * gridDim.x >= n_items) it.part = -1;
       ok = __all_sync(0xffffffffu, mbar_wait(&sched_empty[k % 3], ((k / 3) & 1) ^ 1u, abort_flag));
@@ -1099,8 +1076,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Parts<kDim> to_join = Parts<kDim>::of(p.workspace, p.parts_max);
           const size_t tile = static_cast<size_t>(it.part - 1) * 2 + t;
           if (live) {
-            if (d == 0) to_join.ml[tile * 128 + row] = make_float2(m.raw, sum);
-            float4 *o = to_join.o + (tile * (kDim / 4) + d / 4) * 128 + row;
+            if (d == 0) reinterpret_cast<float2 *>(to_join.ml)[tile * 128 + row] = make_float2(m.raw, sum);
+            float4 *o = reinterpret_cast<float4 *>(to_join.o) + (tile * (kDim / 4) + d / 4) * 128 + row;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               o[e * 128] = make_float4(__uint_as_float(x[e / 8][4 * e % 32]), __uint_as_float(x[e / 8][4 * e % 32 + 1]),
@@ -1150,6 +1127,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (p.parts_max && threadIdx.x == 0)
+    Parts<kDim>::of(p.workspace, p.parts_max).done[blockIdx.x] = *abort_flag ? Parts<kDim>::kGaveUp : Parts<kDim>::kDone;
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
@@ -1163,8 +1142,12 @@ template <bool kBf16, int kDim>
 __global__ void __launch_bounds__(256) attention_packed_join_kernel(const PackedArgs p) {
   pdl_wait();
   const Parts<kDim> w = Parts<kDim>::of(p.workspace, p.parts_max);
-  if (blockIdx.x >= *w.count) return;
+  // loaded together; what is not a part's is not used
+  const uint32_t count = *w.count;
   const Part part = w.what[blockIdx.x];
+  if (!__syncthreads_and(w.finished(p.parts_max, threadIdx.x, 256)) || blockIdx.x >= count) return;
+  const float2 *mls = reinterpret_cast<const float2 *>(w.ml);
+  const float4 *os = reinterpret_cast<const float4 *>(w.o);
   // the item's parts stand kv_heads apart
   const uint32_t first = blockIdx.x - part.index * p.kv_heads;
   const int from = 256 * part.index / part.parts, rows = 256 * (part.index + 1) / part.parts - from;
@@ -1176,15 +1159,15 @@ __global__ void __launch_bounds__(256) attention_packed_join_kernel(const Packed
     float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
     for (int i = 0; i < part.parts; ++i)
-      top = fmaxf(top, w.ml[(static_cast<size_t>(first) + i * p.kv_heads) * 256 + row].x);
+      top = fmaxf(top, mls[(static_cast<size_t>(first) + i * p.kv_heads) * 256 + row].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = 0; i < part.parts; ++i) {
       const size_t at = static_cast<size_t>(first) + i * p.kv_heads;
-      const float2 ml = w.ml[at * 256 + row];
+      const float2 ml = mls[at * 256 + row];
       if (ml.x == -INFINITY && ml.y == 0.f) continue;  // sees none of the part's keys
       const float f = top == -INFINITY ? 1.f : ex2_approx((ml.x - top) * p.scale_log2);
-      const float4 v = w.o[((at * 2 + t) * (kDim / 4) + d4) * 128 + in];
+      const float4 v = os[((at * 2 + t) * (kDim / 4) + d4) * 128 + in];
       sum = fmaf(ml.y, f, sum);
       acc.x = fmaf(v.x, f, acc.x);
       acc.y = fmaf(v.y, f, acc.y);
