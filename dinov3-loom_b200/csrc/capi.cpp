@@ -539,14 +539,28 @@ const char *check_heads(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, 
   return nullptr;
 }
 
+const char *check_pages(uint32_t page_size, uint32_t max_pages) {
+  if (page_size == 0 || page_size > 65536) return "page_size must be 1..65536";
+  if (static_cast<uint64_t>(max_pages) * page_size > 0x7fffffffull)
+    return "max_pages x page_size must be below 2^31";
+  return nullptr;
+}
+
+constexpr uint32_t kMostRows = 0x7fffff00u;  // rows or sequences of a call
+
+bool paged_rows_ok(const dv3k_paged_attention &a) {
+  return static_cast<uint64_t>(a.n_seq) * a.q_heads <= kMostRows;
+}
+bool packed_rows_ok(const dv3k_packed_attention &a) {
+  return a.total_q <= kMostRows && a.total_k <= kMostRows && a.n_seq <= kMostRows;
+}
+
 const char *check_cache(const void *k, const void *v, int64_t k_page, int64_t v_page,
                         const int32_t *table, int64_t table_stride, uint32_t n_seq,
                         uint32_t max_pages, uint32_t n_pages, uint32_t page_size, uint32_t kv_heads,
                         uint32_t head_dim) {
-  if (page_size == 0 || page_size > 65536) return "page_size must be 1..65536";
+  if (const char *e = check_pages(page_size, max_pages)) return e;
   if (n_pages > 0x7fffffffu) return "n_pages must be below 2^31";
-  if (static_cast<uint64_t>(max_pages) * page_size > 0x7fffffffull)
-    return "max_pages x page_size must be below 2^31";
   if (n_pages > 0 && (!k || !v)) return "null cache";
   if (!all_aligned(k, v)) return "pointers must be 16-byte aligned";
   const int64_t least = static_cast<int64_t>(kv_heads) * page_size * head_dim;
@@ -602,8 +616,7 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
   if (a->q_heads == 0) return bad_args("q_heads must be positive");
   if (a->causal > 1 || a->reserved != 0) return bad_args("causal must be 0 or 1, reserved 0");
   if (!scale_ok(a->scale)) return bad_args("scale must be positive and finite");
-  if (a->total_q > 0x7fffff00u || a->total_k > 0x7fffff00u || a->n_seq > 0x7fffff00u)
-    return bad_args("too many rows or sequences");
+  if (!packed_rows_ok(*a)) return bad_args("too many rows or sequences");
   if (!strides_ok(a->q_token, a->total_q, a->q_head, a->q_heads) ||
       !strides_ok(a->k_token, a->total_k, a->k_head, a->kv_heads) ||
       !strides_ok(a->v_token, a->total_k, a->v_head, a->kv_heads) ||
@@ -657,7 +670,9 @@ int dv3k_attention_packed(const dv3k_packed_attention *a, void *stream) {
 }
 
 size_t dv3k_attention_packed_workspace(const dv3k_packed_attention *a) {
-  if (!a || check_heads(a->q_heads, a->kv_heads, a->head_dim, DV3K_F16) || a->q_heads == 0) return 0;
+  // 0 for what the launch refuses
+  if (!a || check_heads(a->q_heads, a->kv_heads, a->head_dim, DV3K_F16) || a->q_heads == 0 || !packed_rows_ok(*a))
+    return 0;
   dv3::PackedAttention p = {};
   p.n_seq = a->n_seq;
   p.total_q = a->total_q;
@@ -676,7 +691,7 @@ int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {
     return bad_args("q and q_heads go together");
   if (a->rot_dim % 16 != 0 || a->rot_dim > a->head_dim)
     return bad_args("rot_dim must be a multiple of 16 up to head_dim");
-  if (a->total > 0x7fffff00u || a->n_seq > 0x7fffff00u) return bad_args("too many rows or sequences");
+  if (a->total > kMostRows || a->n_seq > kMostRows) return bad_args("too many rows or sequences");
   if (!a->cu_new && a->total != a->n_seq)
     return bad_args("without cu_new every sequence has one row: total must equal n_seq");
   if ((a->q_heads > 0 && (!strides_ok(a->q_token, a->total, a->q_head, a->q_heads) ||
@@ -741,8 +756,9 @@ int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {
 }
 
 size_t dv3k_attention_paged_workspace(const dv3k_paged_attention *a) {
+  // 0 for what the launch refuses
   if (!a || check_heads(a->q_heads, a->kv_heads, a->head_dim, DV3K_F16) || a->q_heads == 0 ||
-      a->n_seq == 0 || a->n_seq > 0x7fffff00u)
+      a->n_seq == 0 || !paged_rows_ok(*a) || check_pages(a->page_size, a->max_pages))
     return 0;
   return dv3::attention_paged_workspace(paged_args(*a));
 }
@@ -752,8 +768,7 @@ int dv3k_attention_paged(const dv3k_paged_attention *a, void *stream) {
   if (const char *e = check_heads(a->q_heads, a->kv_heads, a->head_dim, a->dtype)) return bad_args(e);
   if (a->q_heads == 0) return bad_args("q_heads must be positive");
   if (!scale_ok(a->scale)) return bad_args("scale must be positive and finite");
-  if (static_cast<uint64_t>(a->n_seq) * a->q_heads > 0x7fffff00u)
-    return bad_args("too many sequences and heads");
+  if (!paged_rows_ok(*a)) return bad_args("too many sequences and heads");
   if (!strides_ok(a->q_seq, a->n_seq, a->q_head, a->q_heads) ||
       !strides_ok(a->out_seq, a->n_seq, a->out_head, a->q_heads))
     return bad_args("strides must be positive multiples of 8 elements");

@@ -101,3 +101,18 @@ def test_many_weak_keys_beside_a_strong_one(n, gap, strong, dim):
     for name, out, lse in every_form(q, k, v, 1.0):
         check(out, want, tol, name)
         check(lse, torch.full((2,), math.log1p(weak), device=DEV, dtype=torch.float64), torch.full((2,), n * 2.0 ** -24 + 2.0 ** -20, device=DEV, dtype=torch.float64), name + ", log-sum")
+
+
+# ---- arguments -------------------------------------------------------------------------------
+def refused(call, text):
+    with pytest.raises(dv.DINOv3Error) as e:
+        call()
+    assert e.value.code == dv.INVALID_ARGUMENT and text in str(e.value), str(e.value)
+
+
+def test_caches_without_slots_are_refused():
+    q, none = torch.zeros(2, 4, 64, device=DEV, dtype=torch.float16), torch.empty(3, 4, 0, 64, device=DEV, dtype=torch.float16)
+    table, n = ints([[0, 1], [2, 0]]), ints([1, 1])
+    refused(lambda: dv.attention_paged(q, none, none, table, n), "page_size")
+    refused(lambda: dv.attention_paged(q, none, none, table, n, workspace=torch.empty(1 << 20, dtype=torch.uint8, device=DEV)), "page_size")
+    refused(lambda: dv.rope_append(q, q, q, none, none, table, n), "page_size")

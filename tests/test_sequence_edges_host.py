@@ -1,6 +1,7 @@
 """What the packed and paged operators' host side and package do at their edges, without a GPU."""
 import os
 import subprocess
+import sys
 
 from conftest import ROOT
 
@@ -53,3 +54,30 @@ def test_the_join_waits_for_every_block_of_the_launch_before(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-I" + CSRC, str(source), "-o", str(tmp_path / "parts")], check=True)
     got = subprocess.run([str(tmp_path / "parts")], capture_output=True, text=True)
     assert got.stdout == "ok\n", got.stdout
+
+
+SIZES = """
+import sys
+sys.path[:0] = sys.argv[1:]
+from dinov3_b200 import _lib
+from test_sequence_host import PACKED, PACKED_STRUCT, PAGED, PAGED_STRUCT, packed_ok, paged_ok
+lib = _lib.load()
+packed = lambda **c: lib.dv3k_attention_packed_workspace(PACKED_STRUCT.pack(*(dict(packed_ok, **c)[f] for f in PACKED)))
+paged = lambda **c: lib.dv3k_attention_paged_workspace(PAGED_STRUCT.pack(*(dict(paged_ok, **c)[f] for f in PAGED)))
+long = dict(max_pages=4096, max_len=65536)
+assert packed(total_k=4096) > 0 and paged(**long) > 0
+for c in (dict(page_size=0), dict(page_size=65537), dict(page_size=2**32 - 1), dict(max_pages=2**31), dict(n_seq=0), dict(n_seq=2**29), dict(n_seq=2**32 - 1),
+          dict(q_heads=0), dict(q_heads=5), dict(kv_heads=0), dict(head_dim=0), dict(q_heads=258)):
+    assert paged(**dict(long, **c)) == 0, c
+    assert paged(**c) == 0, c
+for c in (dict(n_seq=0), dict(n_seq=2**32 - 1), dict(total_q=0), dict(total_q=2**32 - 1), dict(total_k=2**32 - 1), dict(q_heads=0), dict(q_heads=5),
+          dict(kv_heads=0), dict(head_dim=80), dict(q_heads=258)):
+    assert packed(**dict(dict(total_k=4096), **c)) == 0, c
+print("ok")
+"""
+
+
+def test_size_calls_of_what_the_launch_refuses():
+    """No workspace, and no crash, for arguments that no call accepts."""
+    got = subprocess.run([sys.executable, "-c", SIZES, os.path.join(ROOT, "dinov3-loom_b200"), os.path.join(ROOT, "tests")], capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout == "ok\n", (got.returncode, got.stderr[-1500:])
