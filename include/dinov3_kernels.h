@@ -206,8 +206,10 @@ int dv3k_matmul_swiglu(const uint16_t *h, uint32_t rows, const uint16_t *gateup_
  *     weights scaled, so that those down to 2^-31 of the largest count).
  *   - A row tensor [rows][heads][head_dim] is given by its row (token) and head strides in
  *     elements, multiples of 8, with head_dim contiguous. Rows or heads of an output do not
- *     overlap, nor does an output overlap an input (but q_out of dv3k_rope_append may be q); arrays of
- *     4-byte words are 4-byte aligned, all else 16-byte.
+ *     overlap, nor does an output (lse, status and the workspace among them) overlap an input or another output
+ *     (but q_out of dv3k_rope_append may be q). Views that lie side by side in one buffer are fine
+ *     where they have its strides; what shares memory, or may under strides that differ, is refused.
+ *     Arrays of 4-byte words are 4-byte aligned, all else 16-byte.
  *   - `cu` arrays [n_seq + 1] (i32, device) hold the first row of each sequence and the end of the
  *     last, ascending. Sequences may be empty. Rows before cu[0] or from cu[n_seq] on are left as
  *     they were. Values outside the tensor are clamped to it.

@@ -116,3 +116,40 @@ def test_caches_without_slots_are_refused():
     refused(lambda: dv.attention_paged(q, none, none, table, n), "page_size")
     refused(lambda: dv.attention_paged(q, none, none, table, n, workspace=torch.empty(1 << 20, dtype=torch.uint8, device=DEV)), "page_size")
     refused(lambda: dv.rope_append(q, q, q, none, none, table, n), "page_size")
+
+
+def test_outputs_beside_inputs_in_one_buffer():
+    """Views that share a buffer but no element are taken; those that share one are refused and leave
+    the buffer as it was."""
+    g, t, dim, cu = gen(83), 150, 64, ints([0, 100, 150])
+    qkv = randn(g, t, 12, dim, dtype=torch.float16)  # 4 query, 2 key, 2 value heads, 4 of the result
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:8]
+    want = dv.attention_packed(q, k, v, cu, causal=True)
+    dv.attention_packed(q, k, v, cu, causal=True, out=qkv[:, 8:])
+    assert torch.equal(qkv[:, 8:], want)
+    heads = qkv.transpose(0, 1).contiguous().transpose(0, 1)
+    dv.attention_packed(heads[:, :4], heads[:, 4:6], heads[:, 6:8], cu, causal=True, out=heads[:, 8:])
+    assert torch.equal(heads[:, 8:], want)
+    both_rows = torch.cat([qkv[:, :4], torch.zeros_like(qkv[:, :4])])  # queries, then results
+    dv.attention_packed(both_rows[:t], k, v, cu, causal=True, out=both_rows[t:])
+    assert torch.equal(both_rows[t:], want)
+    before = qkv.clone()
+    for out in (qkv[:, 1:5], qkv[:, 7:11], qkv[:, 4:8], q):
+        refused(lambda: dv.attention_packed(q, k, v, cu, out=out), "overlap")
+    refused(lambda: dv.attention_packed(both_rows[:t], k, v, cu, out=both_rows[t - 1:-1]), "overlap")
+    assert torch.equal(qkv, before)
+
+    pool, lens, table = torch.zeros(12, 2, 2, 16, dim, device=DEV, dtype=torch.float16), ints([100, 50]), ints([[0, 1, 2, 3, 4, 5, 6], [7, 8, 9, 10, -1, -1, -1]])
+    kc, vc = pool[:, 0], pool[:, 1]
+    cos = torch.rand(128, 32, device=DEV)
+    apart_q = dv.rope_append(q, k, v, kc, vc, table, lens, cos, cos, cu_new=cu)
+    again, kept = qkv.clone(), pool.clone()
+    mine = again[:, :4]  # in place within the fused rows
+    assert dv.rope_append(mine, again[:, 4:6], again[:, 6:8], kc, vc, table, lens, cos, cos, cu_new=cu, q_out=mine) is mine
+    assert torch.equal(mine, apart_q) and torch.equal(again[:, 4:], qkv[:, 4:]) and torch.equal(pool, kept)
+    refused(lambda: dv.rope_append(q, k, v, kc, vc, table, lens, cos, cos, cu_new=cu, q_out=qkv[:, 1:5]), "overlap")
+    refused(lambda: dv.rope_append(q, k, v, kc, kc, table, lens, cos, cos, cu_new=cu), "overlap")
+    rows = pool[0].view(-1, 2, dim)[:2]  # two rows inside the first page
+    refused(lambda: dv.rope_append(None, rows, rows, kc, vc, table, ints([1, 1])), "overlap")
+    refused(lambda: dv.attention_paged(q[:2], kc, vc, table, lens, out=pool[3].view(-1, 4, dim)[:2]), "overlap")
+    assert torch.equal(qkv, before) and torch.equal(pool, kept)

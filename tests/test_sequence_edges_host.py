@@ -3,6 +3,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 from conftest import ROOT
 
 CSRC = os.path.join(ROOT, "dinov3-loom_b200", "csrc")
@@ -81,3 +83,104 @@ def test_size_calls_of_what_the_launch_refuses():
     """No workspace, and no crash, for arguments that no call accepts."""
     got = subprocess.run([sys.executable, "-c", SIZES, os.path.join(ROOT, "dinov3-loom_b200"), os.path.join(ROOT, "tests")], capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout == "ok\n", (got.returncode, got.stderr[-1500:])
+
+
+REGIONS = r"""
+#include <cstdio>
+#include <random>
+#include <set>
+#include "regions.h"
+using dv3::Region;
+static std::set<uintptr_t> bytes_of(const Region &r) {
+  std::set<uintptr_t> s;
+  for (uint32_t i = 0; i < r.n_outer; ++i)
+    for (uint32_t j = 0; j < r.n_inner; ++j)
+      for (int64_t b = 0; b < r.bytes; ++b) s.insert(reinterpret_cast<uintptr_t>(r.base) + i * r.outer + j * r.inner + b);
+  return s;
+}
+static bool share(const Region &a, const Region &b) {
+  const auto x = bytes_of(a), y = bytes_of(b);
+  for (uintptr_t i : x)
+    if (y.count(i)) return true;
+  return false;
+}
+static const void *at(int64_t x) { return reinterpret_cast<const void *>(x); }
+int main() {
+  std::mt19937 rng(5);
+  auto pick = [&](int lo, int hi) { return lo + static_cast<int>(rng() % (hi - lo + 1)); };
+  int apart = 0, views = 0;
+  for (int n = 0; n < 20000; ++n) {
+    Region r[2];
+    for (Region &x : r) x = {at(pick(100, 160)), pick(1, 24), pick(1, 24), static_cast<uint32_t>(pick(0, 4)), static_cast<uint32_t>(pick(0, 4)), pick(0, 9)};
+    if (n % 2) r[1].outer = r[0].outer, r[1].inner = r[0].inner;
+    if (dv3::apart(r[0], r[1]) != dv3::apart(r[1], r[0])) return puts("not symmetric"), 1;
+    if (!dv3::apart(r[0], r[1])) continue;
+    ++apart;
+    if (share(r[0], r[1])) return puts("shares"), 1;
+  }
+  // columns of one buffer [rows][columns][8 bytes], and slices of its vectors: told apart exactly
+  for (int n = 0; n < 20000; ++n) {
+    const int rows = pick(1, 4), columns = pick(1, 5), width = pick(1, 8);
+    Region r[2];
+    for (Region &x : r) {
+      const int c0 = pick(0, columns - 1), w0 = pick(0, width - 1);
+      x = {at(1000 + c0 * width + w0), columns * width, width, static_cast<uint32_t>(rows), static_cast<uint32_t>(pick(1, columns - c0)), pick(1, width - w0)};
+      if (pick(0, 1)) std::swap(x.outer, x.inner), std::swap(x.n_outer, x.n_inner);
+    }
+    ++views;
+    if (dv3::apart(r[0], r[1]) == share(r[0], r[1])) return puts("views"), 1;
+  }
+  // nothing, and strides whose product passes 64 bits
+  if (!dv3::apart({nullptr, 1, 1, 1, 1, 1}, {at(5), 1, 1, 1, 1, 1})) return puts("null"), 1;
+  const Region far = {at(1 << 20), int64_t{1} << 38, int64_t{1} << 38, 0x7fffffffu, 0x7fffffffu, 256};
+  if (dv3::apart(far, {at((1 << 20) + (int64_t{1} << 39)), 256, 256, 1, 1, 256}) || !dv3::apart(far, {at(1 << 19), 256, 256, 4, 4, 256})) return puts("far"), 1;
+  printf("ok %d\n", apart > 3000);
+}
+"""
+
+
+def test_regions_are_told_apart(tmp_path):
+    source = tmp_path / "regions.cpp"
+    source.write_text(REGIONS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-I" + CSRC, str(source), "-o", str(tmp_path / "regions")], check=True)
+    got = subprocess.run([str(tmp_path / "regions")], capture_output=True, text=True)
+    assert got.stdout == "ok 1\n", got.stdout
+
+
+from test_sequence_host import (APPEND, APPEND_STRUCT, BASE, PACKED, PACKED_STRUCT, PAGED, PAGED_STRUCT, append_ok, packed_ok,  # noqa: E402
+                                paged_ok, refused)
+
+FAR = {name: BASE + (i + 1) * (1 << 24) for i, name in enumerate("q k v out lse cu_q cu_k status q_out k_cache v_cache cu_new lens page_table cos sin".split())}
+
+
+def moved(ok):
+    """The arguments with every tensor far from the others: addresses that nothing reads."""
+    return {f: FAR[f] if f in FAR and v else v for f, v in ok.items()}
+
+
+# q is [4][4][64], 2048 bytes; k, v [4][2][64] in rows of 256 elements; caches [8][2][16][64]
+@pytest.mark.parametrize("changes", [
+    dict(out=FAR["q"] + 128), dict(out=FAR["q"] - 16), dict(out=FAR["q"] + 2032), dict(out=FAR["k"] - 128), dict(out=FAR["v"] + 16), dict(out=FAR["cu_q"] - 2032),
+    dict(out=FAR["cu_k"]), dict(lse=FAR["q"] + 4), dict(lse=FAR["v"]), dict(lse=FAR["out"] + 2044), dict(status=FAR["out"]), dict(lse=FAR["cu_q"]),
+    dict(out=FAR["q"], out_token=512), dict(out=FAR["q"] + 64 * 2, q_token=512, out_token=512),
+])
+def test_packed_outputs_that_overlap(changes):
+    refused("dv3k_attention_packed", PACKED_STRUCT, PACKED, moved(packed_ok), "overlap", **changes)
+
+
+@pytest.mark.parametrize("changes", [
+    dict(q_out=FAR["q"] + 128), dict(q_out=FAR["q"] - 2032), dict(q_out=FAR["k"]), dict(q_out=FAR["v"] + 64), dict(q_out=FAR["k_cache"] + 4096),
+    dict(q_out=FAR["cos"]), dict(k_cache=FAR["v_cache"]), dict(k_cache=FAR["v_cache"] + 4096), dict(v_cache=FAR["k_cache"] + 2048), dict(k_cache=FAR["k"]),
+    dict(v_cache=FAR["q"] - 4096), dict(k_cache=FAR["page_table"]), dict(v_cache=FAR["lens"]), dict(k_cache=FAR["sin"]), dict(q_out=FAR["cu_new"]),
+    dict(status=FAR["k_cache"] + 8),
+])
+def test_append_outputs_that_overlap(changes):
+    refused("dv3k_rope_append", APPEND_STRUCT, APPEND, moved(append_ok), "overlap", **changes)
+
+
+@pytest.mark.parametrize("changes", [
+    dict(out=FAR["q"] + 128), dict(out=FAR["k_cache"] + 4096), dict(out=FAR["v_cache"]), dict(out=FAR["page_table"]), dict(out=FAR["lens"] - 1008), dict(lse=FAR["out"]),
+    dict(lse=FAR["q"] + 8), dict(lse=FAR["k_cache"]), dict(status=FAR["out"] + 8),
+])
+def test_paged_outputs_that_overlap(changes):
+    refused("dv3k_attention_paged", PAGED_STRUCT, PAGED, moved(paged_ok), "overlap", **changes)
