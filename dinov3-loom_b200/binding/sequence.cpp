@@ -109,6 +109,7 @@ void *optional(PyObject *o, const char *name, const at::Tensor &like, at::Scalar
   const at::Tensor &t = tensor(o, name);
   if (t.scalar_type() != type || t.device() != like.device() || !t.is_contiguous() || t.sizes() != shape)
     refuse(name, " must be a contiguous ", at::toString(type), " tensor of shape ", shape, " on ", like.device());
+  no_gradient(t, name);
   return t.data_ptr();
 }
 

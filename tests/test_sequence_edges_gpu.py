@@ -153,3 +153,32 @@ def test_outputs_beside_inputs_in_one_buffer():
     refused(lambda: dv.rope_append(None, rows, rows, kc, vc, table, ints([1, 1])), "overlap")
     refused(lambda: dv.attention_paged(q[:2], kc, vc, table, lens, out=pool[3].view(-1, 4, dim)[:2]), "overlap")
     assert torch.equal(qkv, before) and torch.equal(pool, kept)
+
+
+# ---- gradients -------------------------------------------------------------------------------
+def everything(dtype=torch.float16):
+    """The float tensors of a call of each operator by name, and the calls on such a dict."""
+    g = gen(84)
+    t = {n: randn(g, 6, h, 64, dtype=dtype) for n, h in (("q", 4), ("k", 2), ("v", 2), ("out", 4))}
+    t.update({n: torch.zeros(3, 2, 8, 64, device=DEV, dtype=dtype) for n in ("k_cache", "v_cache")})
+    t.update(cos=torch.rand(16, 32, device=DEV), sin=torch.rand(16, 32, device=DEV), lse=torch.zeros(6, 4, device=DEV))
+    cu, table, lens, few = ints([0, 6]), ints([[0, 1]]), ints([6]), ints([[0, 1]] * 6)
+    calls = {
+        "packed": (("q", "k", "v", "out", "lse"), lambda t: dv.attention_packed(t["q"], t["k"], t["v"], cu, out=t["out"], lse=t["lse"])),
+        "append": (("q", "k", "v", "out", "k_cache", "v_cache", "cos", "sin"),
+                   lambda t: dv.rope_append(t["q"], t["k"], t["v"], t["k_cache"], t["v_cache"], table, lens, t["cos"], t["sin"], cu_new=cu, q_out=t["out"])),
+        "paged": (("q", "k_cache", "v_cache", "out", "lse"), lambda t: dv.attention_paged(t["q"], t["k_cache"], t["v_cache"], few, ints([6] * 6), out=t["out"], lse=t["lse"])),
+    }
+    return t, calls
+
+
+@pytest.mark.parametrize("op", ["packed", "append", "paged"])
+def test_tensors_that_want_a_gradient(op):
+    tensors, calls = everything()
+    names, call = calls[op]
+    call(tensors)
+    for name in names:
+        wanting = dict(tensors, **{name: tensors[name].clone().requires_grad_()})
+        refused(lambda: call(wanting), "requires a gradient")
+        with torch.no_grad():
+            call(wanting)
