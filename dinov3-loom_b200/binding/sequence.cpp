@@ -52,6 +52,7 @@ const at::Tensor &tensor(PyObject *o, const char *name) {
 void no_gradient(const at::Tensor &t, const char *name) {
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse(name, " requires a gradient, which this operator does not compute");
+  if (t._fw_grad(0).defined()) refuse(name, " carries a tangent, which this operator does not propagate");
 }
 
 uint32_t first(const at::Tensor &t, const char *name) {

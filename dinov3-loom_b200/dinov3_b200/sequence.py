@@ -10,7 +10,7 @@ face of dv3k_attention_packed, dv3k_rope_append and dv3k_attention_paged
 The calls are asynchronous on torch's current stream of the tensors' device (which need not be the
 current device), can be captured into a CUDA graph, and allocate only what they return (and the
 attentions their scratch, unless it is given) through torch's allocator. They compute no
-gradients: a tensor that wants one is refused. What does not fit raises DINOv3Error
+gradients: a tensor that wants one, or carries a forward-mode tangent, is refused. What does not fit raises DINOv3Error
 (INVALID_ARGUMENT) before anything is launched. `status` is an optional int32 CUDA tensor of two
 words, cleared and read by the caller, that collects what only the device sees (bad pages and
 positions).

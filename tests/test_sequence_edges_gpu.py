@@ -182,3 +182,20 @@ def test_tensors_that_want_a_gradient(op):
         refused(lambda: call(wanting), "requires a gradient")
         with torch.no_grad():
             call(wanting)
+
+
+@pytest.mark.parametrize("op", ["packed", "append", "paged"])
+def test_tensors_that_carry_a_tangent(op):
+    """Forward-mode dual tensors, whose tangent the result would not have; under no_grad as well, which
+    does not switch forward mode off."""
+    from torch.autograd import forward_ad
+
+    tensors, calls = everything()
+    names, call = calls[op]
+    for name in names:
+        with forward_ad.dual_level():
+            dual = dict(tensors, **{name: forward_ad.make_dual(tensors[name].clone(), torch.ones_like(tensors[name]))})
+            refused(lambda: call(dual), "tangent")
+            with torch.no_grad():
+                refused(lambda: call(dual), "tangent")
+    call(tensors)
