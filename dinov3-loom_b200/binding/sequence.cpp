@@ -122,6 +122,15 @@ uint32_t *status_of(PyObject *o, const at::Tensor &like) {
   return static_cast<uint32_t *>(t.data_ptr());
 }
 
+// Counts a given tensor as written, so that autograd notices where it had kept it. Inference tensors
+// have no counter.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject *o) {
+  if (o != Py_None) written(THPVariable_Unpack(o));
+}
+
 // A new tensor from torch's allocator, without the dispatcher's way to it.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
@@ -250,6 +259,8 @@ PyObject *attention_packed(PyObject *, PyObject *const *a, Py_ssize_t n) {
       scratch = scratch_of(a[9], p, packed_workspace_fn, q);
       return packed_fn(&p, stream);
     });
+    written(a[7]);
+    written(a[8]);
     return result(a[7], std::move(out));
   });
 }
@@ -321,6 +332,9 @@ PyObject *rope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     p.kv_heads = static_cast<uint32_t>(k.size(1));
     p.head_dim = size32(k.size(2), "dim");
     on_device(k, [&](void *stream) { return append_fn(&p, stream); });
+    written(k_cache);
+    written(v_cache);
+    if (p.q) written(a[10]);
     if (a[0] == Py_None) Py_RETURN_NONE;
     return result(a[10], std::move(out));
   });
@@ -376,6 +390,8 @@ PyObject *attention_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
       scratch = scratch_of(a[9], p, paged_workspace_fn, q);
       return paged_fn(&p, stream);
     });
+    written(a[7]);
+    written(a[8]);
     return result(a[7], std::move(out));
   });
 }

@@ -199,3 +199,24 @@ def test_tensors_that_carry_a_tangent(op):
             with torch.no_grad():
                 refused(lambda: call(dual), "tangent")
     call(tensors)
+
+
+def test_what_a_call_writes_counts_as_changed():
+    """A tensor that autograd keeps for a backward pass and a call overwrites meanwhile is noticed, as
+    torch's own operators in place are; inference tensors, which have no counter, are written."""
+    tensors, calls = everything(torch.bfloat16)
+    written = {"packed": ("out", "lse"), "append": ("out", "k_cache", "v_cache"), "paged": ("out", "lse")}
+    for op, (names, call) in calls.items():
+        before = {n: tensors[n]._version for n in names}
+        call(tensors)
+        assert {n for n in names if tensors[n]._version != before[n]} == set(written[op]), op
+        call({n: x.detach() for n, x in tensors.items()})
+        with torch.inference_mode():
+            held = {n: x.clone() for n, x in tensors.items()}
+            call(held)
+        call(held)
+    weight = torch.ones(64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    loss = (tensors["k_cache"] * weight).sum()
+    calls["append"][1](tensors)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
