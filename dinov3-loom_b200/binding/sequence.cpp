@@ -287,6 +287,7 @@ PyObject *rope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
       p.cu_new = static_cast<const int32_t *>(cu.data_ptr());
     }
     if ((a[7] == Py_None) != (a[8] == Py_None)) refuse("cos and sin go together");
+    if (a[0] == Py_None && a[10] != Py_None) refuse("q_out goes with q");
     if (a[7] != Py_None) {
       const at::Tensor &cos = tensor(a[7], "cos");
       if (cos.dim() != 2) refuse("cos must be [positions, rot_dim / 2]");
@@ -334,7 +335,7 @@ PyObject *rope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     on_device(k, [&](void *stream) { return append_fn(&p, stream); });
     written(k_cache);
     written(v_cache);
-    if (p.q) written(a[10]);
+    written(a[10]);
     if (a[0] == Py_None) Py_RETURN_NONE;
     return result(a[10], std::move(out));
   });

@@ -220,3 +220,9 @@ def test_what_a_call_writes_counts_as_changed():
     calls["append"][1](tensors)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_an_output_for_queries_that_are_not_given():
+    tensors, _ = everything()
+    refused(lambda: dv.rope_append(None, tensors["k"][:1], tensors["v"][:1], tensors["k_cache"], tensors["v_cache"], ints([[0, 1]]), ints([1]), q_out=tensors["out"][:1]),
+            "q_out goes with q")
