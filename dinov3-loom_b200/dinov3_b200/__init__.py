@@ -35,7 +35,6 @@ OK, INVALID_ARGUMENT, WEIGHTS, DEVICE, POISONED = range(5)
 __all__ = [
     "DINOv3", "DINOv3Error", "Options", "ForwardTimings", "Distribution", "LibraryMissing",
     "IMAGE_ELEMENTS", "TOKENS", "HIDDEN", "pack_f16", "hub_weights",
-    "attention_packed", "rope_append", "attention_paged",
 ]
 
 
@@ -271,7 +270,8 @@ def hub_weights(offline: bool = False) -> str:
 
 
 def __getattr__(name):
-    # the sequence operators take torch tensors: torch is imported when the first one is named
+    # the sequence operators take torch tensors: torch is imported when the first one is named (and
+    # they are not in __all__, so that a star import does without it)
     if name in ("attention_packed", "rope_append", "attention_paged"):
         from . import sequence
 

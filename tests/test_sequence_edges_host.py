@@ -184,3 +184,24 @@ def test_append_outputs_that_overlap(changes):
 ])
 def test_paged_outputs_that_overlap(changes):
     refused("dv3k_attention_paged", PAGED_STRUCT, PAGED, moved(paged_ok), "overlap", **changes)
+
+
+STAR = """
+import sys
+sys.path.insert(0, sys.argv[1])
+sys.modules["torch"] = None  # an import of it raises
+from dinov3_b200 import *
+import dinov3_b200
+assert DINOv3 is dinov3_b200.DINOv3 and "attention_packed" not in globals()
+assert not any(m == "torch" or m.startswith("torch.") for m in sys.modules if sys.modules[m])
+try:
+    dinov3_b200.attention_packed
+except ImportError as e:
+    print("ok")
+"""
+
+
+def test_a_star_import_needs_no_torch():
+    """What every name of the package but the sequence operators' needs."""
+    got = subprocess.run([sys.executable, "-c", STAR, os.path.join(ROOT, "dinov3-loom_b200")], capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout == "ok\n", got.stderr[-1500:]
