@@ -205,3 +205,84 @@ def test_a_star_import_needs_no_torch():
     """What every name of the package but the sequence operators' needs."""
     got = subprocess.run([sys.executable, "-c", STAR, os.path.join(ROOT, "dinov3-loom_b200")], capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout == "ok\n", got.stderr[-1500:]
+
+
+STUB = """#!/bin/sh
+# in nvcc's place: notes the call, makes the output
+while [ $# -gt 0 ]; do case "$1" in
+  -ltorch_cuda) binding=1;;
+  -o) shift; out="$1";;
+esac; shift; done
+echo "$out" >> "$(dirname "$0")/calls"
+if [ "$binding" ] && [ -e "$(dirname "$0")/broken" ]; then echo "no such header"; exit 1; fi
+: > "$out"
+"""
+
+
+@pytest.fixture
+def builder(tmp_path, monkeypatch):
+    """build.py with a stub for nvcc, its outputs in a folder of their own, and a torch of a few files."""
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("dv3_build_under_test", os.path.join(ROOT, "dinov3-loom_b200", "build.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    nvcc = tmp_path / "nvcc"
+    nvcc.write_text(STUB)
+    nvcc.chmod(0o755)
+    torch = tmp_path / "torch"
+    (torch / "lib").mkdir(parents=True)
+    (torch / "version.py").write_text("__version__ = '1'\n")
+    (torch / "lib" / "libtorch_cuda.so").write_text("")
+    for name, to in (("NVCC", nvcc), ("BUILD", tmp_path / "objects"), ("LIB", tmp_path / "libdinov3.so"), ("BINDING_LIB", tmp_path / "_sequence.so")):
+        monkeypatch.setattr(mod, name, str(to))
+    found = type("Spec", (), {"submodule_search_locations": [str(torch)]})()
+    monkeypatch.setattr(mod.importlib.util, "find_spec", lambda name: found)
+
+    def calls():
+        log = tmp_path / "calls"
+        got = log.read_text().split() if log.exists() else []
+        log.write_text("")
+        return got
+
+    mod.tmp, mod.torch, mod.calls = tmp_path, torch, calls
+    return mod
+
+
+def test_the_library_builds_whatever_torch_is(builder, capfd, monkeypatch):
+    (builder.torch / "lib" / "libtorch_cuda.so").unlink()
+    builder.build()
+    assert os.path.exists(builder.LIB) and not os.path.exists(builder.BINDING_LIB) and "CUDA" in capfd.readouterr().err
+    (builder.torch / "lib" / "libtorch_cuda.so").write_text("")
+    (builder.tmp / "broken").write_text("")
+    os.unlink(builder.LIB)
+    builder.build()
+    assert os.path.exists(builder.LIB) and not os.path.exists(builder.BINDING_LIB) and "no such header" in capfd.readouterr().err
+    (builder.tmp / "broken").unlink()
+    builder.build()
+    assert os.path.exists(builder.BINDING_LIB) and capfd.readouterr().err == ""
+    monkeypatch.setattr(builder.importlib.util, "find_spec", lambda name: None)
+    builder.build(force=True)
+    assert capfd.readouterr().err == ""
+
+
+def test_the_binding_follows_torch_and_python(builder, monkeypatch):
+    binding = [builder.BINDING_LIB]
+    builder.build()
+    assert builder.calls().count(binding[0]) == 1
+    builder.build()
+    assert builder.calls() == []
+    (builder.torch / "version.py").write_text("__version__ = '2'\n")
+    builder.build()
+    assert builder.calls() == binding
+    builder.build()
+    assert builder.calls() == []
+    soabi = builder.sysconfig.get_config_var
+    monkeypatch.setattr(builder.sysconfig, "get_config_var", lambda name: "cpython-399" if name == "SOABI" else soabi(name))
+    builder.build()
+    assert builder.calls() == binding
+    # one that was built for another torch and cannot be built for this one goes: it might not load, or crash
+    (builder.torch / "version.py").write_text("__version__ = '3'\n")
+    (builder.tmp / "broken").write_text("")
+    builder.build()
+    assert not os.path.exists(builder.BINDING_LIB)
