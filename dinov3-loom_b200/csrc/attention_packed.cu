@@ -1208,6 +1208,7 @@ struct Items {
   uint64_t most;       // items at most: one partly filled one per sequence
   uint32_t parts_max;  // see PackedArgs
 };
+uint32_t most_parts(uint32_t sms) { return 2 * sms; }
 Items items_of(const PackedAttention &p, uint32_t sms) {
   Items x;
   x.tokens = 128 / (p.q_heads / p.kv_heads);
@@ -1216,7 +1217,7 @@ Items items_of(const PackedAttention &p, uint32_t sms) {
   // the whole) and long (more than 8 steps, and sequences of more than 4 on average: a join that has
   // nothing to do costs a short call 2.5 us). A part costs its own start and end and 133 KB of partial
   // results at 128 channels, so there are two for each CTA at most.
-  x.parts_max = x.most < 4ull * sms && p.total_k > 8 * 128 && p.total_k / p.n_seq > 4 * 128 ? 2 * sms : 0;
+  x.parts_max = x.most < 4ull * sms && p.total_k > 8 * 128 && p.total_k / p.n_seq > 4 * 128 ? most_parts(sms) : 0;
   return x;
 }
 }  // namespace
@@ -1228,6 +1229,13 @@ size_t attention_packed_workspace(const PackedAttention &p) {
   const uint32_t parts = items_of(p, static_cast<uint32_t>(sm_count(dev))).parts_max;
   if (parts == 0) return 0;
   return p.head_dim == 64 ? Parts<64>::bytes(parts) : Parts<128>::bytes(parts);
+}
+
+size_t attention_packed_workspace_bound(uint32_t head_dim) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint32_t parts = most_parts(static_cast<uint32_t>(sm_count(dev)));
+  return head_dim == 64 ? Parts<64>::bytes(parts) : Parts<128>::bytes(parts);
 }
 
 cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,

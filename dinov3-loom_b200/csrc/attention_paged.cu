@@ -127,11 +127,15 @@ struct Plan {
   bool crowd;                        // many stretches share a unit
 };
 
-Plan plan_of(const PagedAttention &p) {
+// CTAs that run at once.
+uint32_t cta_slots(const PagedAttention &p) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const uint64_t slots = static_cast<uint64_t>(sm_count(dev)) *
-                         (p.head_dim == 64 ? Ring<64>::kPerSm : Ring<128>::kPerSm);
+  return static_cast<uint32_t>(sm_count(dev)) * (p.head_dim == 64 ? Ring<64>::kPerSm : Ring<128>::kPerSm);
+}
+
+Plan plan_of(const PagedAttention &p) {
+  const uint64_t slots = cta_slots(p);
   const uint32_t group = p.q_heads / p.kv_heads;
   Plan s;
   s.head_blocks = p.kv_heads * ((group + 15) / 16);
@@ -720,11 +724,22 @@ __global__ void __launch_bounds__(kJoin * 32)
   if (p.lse && lane == 0) p.lse[row] = log_sum<kBf16>(top * c2, sum, 0);
 }
 
-size_t attention_paged_workspace(const PagedAttention &p) {
-  const Plan pl = plan_of(p);
-  if (pl.units) return 0;
+namespace {
+size_t workspace_of(const PagedAttention &p, const Plan &pl) {
   const size_t n = (static_cast<size_t>(pl.grid) * kWarps * 2 * pl.rows + 1) / 2 * 2;
   return shares_bytes(p, pl) + n * (p.head_dim + 2) * sizeof(float);
+}
+}  // namespace
+
+size_t attention_paged_workspace(const PagedAttention &p) {
+  const Plan pl = plan_of(p);
+  return pl.units ? 0 : workspace_of(p, pl);
+}
+
+size_t attention_paged_workspace_bound(const PagedAttention &p) {
+  Plan pl = plan_of(p);
+  pl.grid = cta_slots(p);  // of any plan at most, and the shares grow with the sequences
+  return workspace_of(p, pl);
 }
 
 namespace {

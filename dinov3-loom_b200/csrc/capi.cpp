@@ -723,6 +723,10 @@ size_t dv3k_attention_packed_workspace(const dv3k_packed_attention *a) {
   return dv3::attention_packed_workspace(p);
 }
 
+size_t dv3k_attention_packed_workspace_bound(uint32_t head_dim) {
+  return head_dim == 64 || head_dim == 128 ? dv3::attention_packed_workspace_bound(head_dim) : 0;
+}
+
 int dv3k_rope_append(const dv3k_rope_append_args *a, void *stream) {
   if (!a) return bad_args("null arguments");
   if (const char *e = check_heads(a->q_heads, a->kv_heads, a->head_dim, a->dtype)) return bad_args(e);
@@ -813,6 +817,18 @@ size_t dv3k_attention_paged_workspace(const dv3k_paged_attention *a) {
       a->n_seq == 0 || !paged_rows_ok(*a) || check_pages(a->page_size, a->max_pages))
     return 0;
   return dv3::attention_paged_workspace(paged_args(*a));
+}
+
+size_t dv3k_attention_paged_workspace_bound(uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads,
+                                            uint32_t head_dim) {
+  dv3k_paged_attention a = {};
+  a.n_seq = n_seq;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.page_size = 1;
+  if (check_heads(q_heads, kv_heads, head_dim, DV3K_F16) || q_heads == 0 || n_seq == 0 || !paged_rows_ok(a)) return 0;
+  return dv3::attention_paged_workspace_bound(paged_args(a));
 }
 
 int dv3k_attention_paged(const dv3k_paged_attention *a, void *stream) {

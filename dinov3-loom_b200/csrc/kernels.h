@@ -204,7 +204,9 @@ struct PackedAttention {
   float scale;
   void *workspace;
 };
-size_t attention_packed_workspace(const PackedAttention &p);  // bytes, on the current device
+// Bytes, on the current device: of this call; and of any call with that head_dim.
+size_t attention_packed_workspace(const PackedAttention &p);
+size_t attention_packed_workspace_bound(uint32_t head_dim);
 // cudaErrorInvalidValue with *err set where a tensor map cannot be built.
 cudaError_t launch_attention_packed(const PackedAttention &p, bool bf16, cudaStream_t stream,
                                     std::string *err);
@@ -247,7 +249,9 @@ struct PagedAttention {
   uint32_t n_seq, max_len, max_pages, n_pages, q_heads, kv_heads, head_dim;
   float scale;
 };
-size_t attention_paged_workspace(const PagedAttention &p);  // bytes, on the current device
+// Bytes, on the current device: of this call; and of any call with its heads and no more sequences.
+size_t attention_paged_workspace(const PagedAttention &p);
+size_t attention_paged_workspace_bound(const PagedAttention &p);
 cudaError_t launch_attention_paged(const PagedAttention &p, bool bf16, cudaStream_t stream);
 
 // ---- bandwidth kernels (elementwise.cu) ----

@@ -14,8 +14,8 @@ floats). Errors raise DINOv3Error carrying the library's status code and message
 reference's error texts). All compute runs in the CUDA library; there is no CPU path.
 
 For sequences beside the model's own forward (images of other sizes packed into one batch, a
-decoder behind the tokens), on CUDA tensors: attention_packed, rope_append, attention_paged
-(sequence.py).
+decoder behind the tokens), on CUDA tensors: attention_packed, rope_append, attention_paged, and the
+sizes of their workspaces (sequence.py).
 """
 from __future__ import annotations
 
@@ -272,7 +272,7 @@ def hub_weights(offline: bool = False) -> str:
 def __getattr__(name):
     # the sequence operators take torch tensors: torch is imported when the first one is named (and
     # they are not in __all__, so that a star import does without it)
-    if name in ("attention_packed", "rope_append", "attention_paged"):
+    if name in ("attention_packed", "rope_append", "attention_paged", "attention_packed_workspace", "attention_paged_workspace"):
         from . import sequence
 
         globals()[name] = getattr(sequence, name)

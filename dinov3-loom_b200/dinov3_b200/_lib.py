@@ -98,6 +98,8 @@ SIGNATURES = {
     "dv3k_attention_paged": ([ctypes.c_char_p, _P], _I),
     "dv3k_attention_packed_workspace": ([ctypes.c_char_p], _SZ),
     "dv3k_attention_paged_workspace": ([ctypes.c_char_p], _SZ),
+    "dv3k_attention_packed_workspace_bound": ([_U32], _SZ),
+    "dv3k_attention_paged_workspace_bound": ([_U32, _U32, _U32, _U32], _SZ),
     "dv3k_gateup_source_row": ([_U32], _U32),
     "dv3k_bounded_wait_selftest": ([ctypes.c_uint64, _P, _P], _I),
 }

@@ -44,8 +44,29 @@ def attention_packed(q, k, v, cu_q, cu_k=None, *, causal=False, scale=None, out=
     q [total_q, q_heads, dim]; k, v [total_k, kv_heads, dim]; cu_q, cu_k int32 [n_seq + 1] (cu_k None:
     cu_q). scale defaults to dim ** -0.5. `out` may be given; rows outside the sequences are left as
     they were. `lse`, float32 [total_q, q_heads], is filled where given. `workspace`: a uint8 tensor of
-    dv3k_attention_packed_workspace's size to use instead of a new one."""
+    attention_packed_workspace(dim) bytes to use instead of a new one."""
     return _sequence.attention_packed(q, k, v, cu_q, cu_k, causal, scale, out, lse, workspace, status)
+
+
+def attention_packed_workspace(dim, device=None) -> int:
+    """Bytes of a workspace that every attention_packed with that head dim can use on the device (None:
+    the current one). Calls that may overlap on the GPU (two streams, two graphs) need one each."""
+    with torch.cuda.device(device):
+        return _size(_lib.load().dv3k_attention_packed_workspace_bound(dim), "no call has head dim", dim)
+
+
+def attention_paged_workspace(n_seq, q_heads, kv_heads, dim, device=None) -> int:
+    """Bytes of a workspace that every attention_paged with these heads and up to n_seq sequences of any
+    length can use on the device (None: the current one). Calls that may overlap need one each."""
+    with torch.cuda.device(device):
+        return _size(_lib.load().dv3k_attention_paged_workspace_bound(n_seq, q_heads, kv_heads, dim), "no call has n_seq, q_heads, kv_heads, dim",
+                     n_seq, q_heads, kv_heads, dim)
+
+
+def _size(n, refusal, *what):
+    if n == 0:
+        _refuse(f"{refusal} {', '.join(map(str, what))}")
+    return n
 
 
 def rope_append(q, k, v, k_cache, v_cache, page_table, lens, cos=None, sin=None, *, cu_new=None, q_out=None, status=None):
@@ -66,5 +87,5 @@ def attention_paged(q, k_cache, v_cache, page_table, lens, *, max_len=None, scal
     q [n_seq, q_heads, dim]; caches [pages, kv_heads, page_size, dim]; page_table int32 [n_seq,
     max_pages]; lens int32 [n_seq]. max_len bounds lens (default: what page_table holds) and decides
     how far sequences are split. `lse`, float32 [n_seq, q_heads], is filled where given. `workspace`:
-    a uint8 tensor of dv3k_attention_paged_workspace's size to use instead of a new one."""
+    a uint8 tensor of attention_paged_workspace(...) bytes to use instead of a new one."""
     return _sequence.attention_paged(q, k_cache, v_cache, page_table, lens, max_len, scale, out, lse, workspace, status)

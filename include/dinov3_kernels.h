@@ -233,7 +233,9 @@ enum { DV3K_F16 = 0, DV3K_BF16 = 1 };
  *   - workspace: dv3k_attention_packed_workspace(args) bytes on the current device (0 unless few
  *     queries may see many keys; NULL will do then), 16-byte aligned, scratch of this call. Calls that
  *     may overlap on the GPU (on two streams, or in two graphs) need one each. It reads n_seq, total_q,
- *     total_k, q_heads, kv_heads and head_dim. */
+ *     total_k, q_heads, kv_heads and head_dim. A smaller call may need more than a larger one:
+ *     ask for each, or allocate dv3k_attention_packed_workspace_bound(head_dim) bytes, which are enough for
+ *     every call with that head_dim on the current device. */
 typedef struct {
   const void *q, *k, *v;
   void *out;
@@ -249,6 +251,7 @@ typedef struct {
 } dv3k_packed_attention;
 int dv3k_attention_packed(const dv3k_packed_attention *args, void *stream);
 size_t dv3k_attention_packed_workspace(const dv3k_packed_attention *args);
+size_t dv3k_attention_packed_workspace_bound(uint32_t head_dim);
 
 /* Rotate new queries and keys by their positions and append the keys and values to the cache.
  * Row t of sequence s (cu_new; NULL: row t is sequence t's only one and total == n_seq) stands at
@@ -283,7 +286,9 @@ int dv3k_rope_append(const dv3k_rope_append_args *args, void *stream);
  *   - workspace: dv3k_attention_paged_workspace(args) bytes on the current device (0: NULL will do),
  *     16-byte aligned, scratch of this call. Calls that may overlap on the GPU (on two streams, or
  *     in two graphs) need one each. It reads n_seq, max_len,
- *     max_pages, page_size, q_heads, kv_heads and head_dim. */
+ *     max_pages, page_size, q_heads, kv_heads and head_dim. A smaller call may need more than a larger one:
+ *     ask for each, or allocate dv3k_attention_paged_workspace_bound(...) bytes, which are enough for every
+ *     call with those heads and no more sequences on the current device, whatever the lengths. */
 typedef struct {
   const void *q, *k_cache, *v_cache;
   void *out;
@@ -298,6 +303,8 @@ typedef struct {
 } dv3k_paged_attention;
 int dv3k_attention_paged(const dv3k_paged_attention *args, void *stream);
 size_t dv3k_attention_paged_workspace(const dv3k_paged_attention *args);
+size_t dv3k_attention_paged_workspace_bound(uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads,
+                                            uint32_t head_dim);
 
 /* Row of the reference's concatenated gate||up matrix ([3072][384], src/weights.rs:103-108)
  * that packed row `packed_row` (< 3072) of gateup_w holds. Host function. */

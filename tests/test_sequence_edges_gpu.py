@@ -226,3 +226,23 @@ def test_an_output_for_queries_that_are_not_given():
     tensors, _ = everything()
     refused(lambda: dv.rope_append(None, tensors["k"][:1], tensors["v"][:1], tensors["k_cache"], tensors["v_cache"], ints([[0, 1]]), ints([1]), q_out=tensors["out"][:1]),
             "q_out goes with q")
+
+
+# ---- workspaces ------------------------------------------------------------------------------
+def test_one_workspace_for_calls_of_any_length():
+    """Calls from one token to a long split in one workspace of the bounding size, as without one."""
+    g, hq, hkv, dim = gen(85), 8, 2, 64
+    paged = torch.full((dv.attention_paged_workspace(40, hq, hkv, dim),), 255, dtype=torch.uint8, device=DEV)
+    packed = torch.full((dv.attention_packed_workspace(dim, DEV),), 255, dtype=torch.uint8, device=DEV)
+    for lens in ([1], [300], [70, 5000], [8, 0, 900] * 10, [2000] * 40, [20000]):
+        k, v, table = paged_cache(86, lens, hkv, 16, dim, torch.float16)
+        q = randn(g, len(lens), hq, dim, dtype=torch.float16)
+        for max_len in (None, 64, max(lens)):
+            want = dv.attention_paged(q, k, v, table, ints(lens), max_len=max_len)
+            assert torch.equal(want, dv.attention_paged(q, k, v, table, ints(lens), max_len=max_len, workspace=paged))
+        k, v = randn(g, sum(lens), hkv, dim, dtype=torch.float16), randn(g, sum(lens), hkv, dim, dtype=torch.float16)
+        cu = cu_of([1] * len(lens))
+        want = dv.attention_packed(q, k, v, cu, cu_of(lens), causal=True)
+        assert torch.equal(want, dv.attention_packed(q, k, v, cu, cu_of(lens), causal=True, workspace=packed))
+    for call in (lambda: dv.attention_packed_workspace(96), lambda: dv.attention_paged_workspace(4, 6, 4, 64), lambda: dv.attention_paged_workspace(0, 4, 4, 64)):
+        refused(call, "no call has")

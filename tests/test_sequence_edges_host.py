@@ -286,3 +286,33 @@ def test_the_binding_follows_torch_and_python(builder, monkeypatch):
     (builder.tmp / "broken").write_text("")
     builder.build()
     assert not os.path.exists(builder.BINDING_LIB)
+
+
+def test_one_workspace_for_every_call():
+    """The sizes of single calls go up and down with their arguments; the bounds cover all of them."""
+    import random
+
+    from dinov3_b200 import _lib
+    lib, rng = _lib.load(), random.Random(3)
+    needs = set()
+    for _ in range(3000):
+        kv, group, dim = rng.choice([1, 2, 3, 8, 40]), rng.choice([1, 2, 4, 7, 16, 17, 33, 128]), rng.choice([64, 128])
+        n = int(2 ** rng.uniform(0, 12))
+        heads = dict(q_heads=kv * group, kv_heads=kv, head_dim=dim)
+        page = rng.choice([1, 16, 67])
+        c = dict(paged_ok, n_seq=n, max_len=int(2 ** rng.uniform(0, 22)), page_size=page, max_pages=(1 << 22) // page, **heads)
+        need = lib.dv3k_attention_paged_workspace(PAGED_STRUCT.pack(*(c[f] for f in PAGED)))
+        needs.add(need > 0)
+        for more in (n, n + 1, 2 * n + 5):
+            assert need <= lib.dv3k_attention_paged_workspace_bound(more, kv * group, kv, dim)
+        c = dict(packed_ok, n_seq=n, total_q=int(2 ** rng.uniform(0, 20)), total_k=int(2 ** rng.uniform(0, 24)), **heads)
+        need = lib.dv3k_attention_packed_workspace(PACKED_STRUCT.pack(*(c[f] for f in PACKED)))
+        needs.add(need > 0)
+        assert need <= lib.dv3k_attention_packed_workspace_bound(dim)
+    assert needs == {False, True}
+    # not far above what a call may need: the largest of one long sequence
+    one = dict(paged_ok, n_seq=1, max_len=1 << 22, max_pages=1 << 18, q_heads=32, kv_heads=8, head_dim=128)
+    assert lib.dv3k_attention_paged_workspace_bound(1, 32, 8, 128) <= 1.01 * lib.dv3k_attention_paged_workspace(PAGED_STRUCT.pack(*(one[f] for f in PAGED)))
+    for refused_heads in ((0, 4, 4, 64), (2**30, 4, 4, 64), (4, 5, 4, 64), (4, 4, 0, 64), (4, 4, 4, 80)):
+        assert lib.dv3k_attention_paged_workspace_bound(*refused_heads) == 0
+    assert lib.dv3k_attention_packed_workspace_bound(96) == 0
