@@ -548,9 +548,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (lane == 0) atomicMax(&order[kBuckets], longest);
     __syncthreads();
-    width = max(1u, (order[kBuckets] + kBuckets - 1) / kBuckets);
-    // Few sequences: a warp for each, the classes over its lanes; else a thread, over its own classes.
-    if (p.n_seq <= 96) {
+    // Few sequences: a warp for each, the classes over its lanes; else a thread, over its own classes
+    // (24 of 1..2048 tokens, 16/8 heads of 64: 79 us with warps, 89 with threads; 256 of them 408 and 410, 256 of 1..16
+    // 66 and 59). Of many, a class is a step wide at least: the search walks all sequences once for
+    // each class that there is (4096 of 1..16 tokens 830 us, 1250 with classes of one key).
+    const bool few = p.n_seq <= 96;
+    width = max(few ? 1u : static_cast<uint32_t>(kKeys), (order[kBuckets] + kBuckets - 1) / kBuckets);
+    if (few) {
       for (uint32_t s = warp; s < p.n_seq; s += kThreads / 32) {
         const Sequence x = sequence_of(p, s);
 #pragma unroll

@@ -585,8 +585,10 @@ constexpr uint32_t kMostRows = 0x7fffff00u;  // rows or sequences of a call
 bool paged_rows_ok(const dv3k_paged_attention &a) {
   return static_cast<uint64_t>(a.n_seq) * a.q_heads <= kMostRows;
 }
+// The packed kernel's search for an item walks the sequences, 32 a turn, while its other roles wait: 2^24
+// of them are a quarter of a second at most, where a wait gives up after two.
 bool packed_rows_ok(const dv3k_packed_attention &a) {
-  return a.total_q <= kMostRows && a.total_k <= kMostRows && a.n_seq <= kMostRows;
+  return a.total_q <= kMostRows && a.total_k <= kMostRows && a.n_seq <= 1u << 24;
 }
 
 const char *check_cache(const void *k, const void *v, int64_t k_page, int64_t v_page,

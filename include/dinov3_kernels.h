@@ -229,7 +229,7 @@ enum { DV3K_F16 = 0, DV3K_BF16 = 1 };
  *   out[i][h] = sum_j w_ij v[j][g] / sum_j w_ij,  w_ij = exp(scale (q[i][h] . k[j][g] - max_j)),
  * over the sequence's keys j < b, where causal over j <= i + b - a of them (a queries, b keys: the
  * last query sees the last key). A row that sees no key gets 0, and -inf in lse. lse (f32
- * [total_q][q_heads], optional) gets log sum_j exp(scale q . k_j). scale > 0.
+ * [total_q][q_heads], optional) gets log sum_j exp(scale q . k_j). scale > 0; at most 2^24 sequences.
  *   - workspace: dv3k_attention_packed_workspace(args) bytes on the current device (0 unless few
  *     queries may see many keys; NULL will do then), 16-byte aligned, scratch of this call. Calls that
  *     may overlap on the GPU (on two streams, or in two graphs) need one each. It reads n_seq, total_q,

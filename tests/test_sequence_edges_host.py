@@ -316,3 +316,8 @@ def test_one_workspace_for_every_call():
     for refused_heads in ((0, 4, 4, 64), (2**30, 4, 4, 64), (4, 5, 4, 64), (4, 4, 0, 64), (4, 4, 4, 80)):
         assert lib.dv3k_attention_paged_workspace_bound(*refused_heads) == 0
     assert lib.dv3k_attention_packed_workspace_bound(96) == 0
+
+
+def test_more_sequences_than_a_search_may_walk():
+    refused("dv3k_attention_packed", PACKED_STRUCT, PACKED, packed_ok, "too many", n_seq=(1 << 24) + 1)
+    refused("dv3k_attention_packed", PACKED_STRUCT, PACKED, packed_ok, "overlap", n_seq=1 << 24)  # not for their number
