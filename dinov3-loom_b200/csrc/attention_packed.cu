@@ -595,6 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t steps = sum_of(static_cast<uint64_t>(n0) * steps_of(c0, width) +
                                       static_cast<uint64_t>(n1) * steps_of(c1, width)) * p.kv_heads;
         uint64_t cut;
+        // 4 steps at least: 2 take 16.0 us and not 17.9 for one query behind 1100 keys, but 28.8 and not 23.9
+        // where one sequence of 8000 keys stands among sixteen
         o.part = max(4u, static_cast<uint32_t>((steps * 3 / 2 + gridDim.x - 1) / gridDim.x));
         while (true) {  // until the parts fit the workspace
           const uint32_t p0 = parts_of(c0, width, o.part), p1 = parts_of(c1, width, o.part);
@@ -1218,9 +1220,12 @@ Items items_of(const PackedAttention &p, uint32_t sms) {
   x.tokens = 128 / (p.q_heads / p.kv_heads);
   x.most = ((static_cast<uint64_t>(p.total_q) + 2 * x.tokens - 1) / (2 * x.tokens) + p.n_seq) * p.kv_heads;
   // Items are cut where they may be few (fewer than four a CTA: beyond, an uneven end is short beside
-  // the whole) and long (more than 8 steps, and sequences of more than 4 on average: a join that has
-  // nothing to do costs a short call 2.5 us). A part costs its own start and end and 133 KB of partial
-  // results at 128 channels, so there are two for each CTA at most.
+  // the whole) and long: more than 8 steps in all (one query, 32/8 heads of 128: 900 keys 18.9 us cut and 20.2
+  // uncut, 1100 17.9 and 22.6, 8000 25 and 120), more than 4 on average. The average hides how uneven
+  // the lengths are: four sequences of 64 queries lose up to 7 us behind 600 keys each (24.6 and 17.6), 4 behind
+  // 800, nothing behind 1200, and gain 16 where one of them has 2000 and the others 100 (22.7 and 38.5). A part
+  // costs its own start and end and 133 KB of partial results at 128 channels, so there are two for each
+  // CTA at most.
   x.parts_max = x.most < 4ull * sms && p.total_k > 8 * 128 && p.total_k / p.n_seq > 4 * 128 ? most_parts(sms) : 0;
   return x;
 }
