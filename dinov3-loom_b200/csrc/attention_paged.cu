@@ -41,9 +41,14 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;  // keys
-constexpr uint32_t kLeast = 4;   // tiles that a warp takes at least
-constexpr uint32_t kShort = 16;  // tiles up to which a unit is not split
-constexpr uint32_t kUnit = 2;    // what a unit's start and end cost, in tiles
+// Times in us at 32/8 heads of 128 unless said. Tiles that a warp takes at least: 32 sequences of 1..300 keys
+// take 10.9 with 4, 14.2 with 8; 9.9 with 2, which gains nowhere else.
+constexpr uint32_t kLeast = 4;
+// Tiles up to which a unit is not split. 256 sequences of 201 keys, 6 heads of 64, take 17.9 with 16 and 24.4 split (8);
+// with 32 they would take 23.6 and not 30.4 at 300 keys each, but 64 of 1..512 keys 29.6 and not 12.8.
+constexpr uint32_t kShort = 16;
+// What a unit's start and end cost, in tiles: 64 sequences of 1..4096 keys take 39.2 with 2 or 4, 55 with 0.
+constexpr uint32_t kUnit = 2;
 constexpr uint32_t kJoinTiles = 4;  // what the joining launch costs, in a warp's tiles
 
 // A warp's shared memory: stages of K and V, and the addresses of the rows of the tiles in flight
