@@ -15,7 +15,7 @@
 // Roles (384 threads):
 //   warps 0-3  softmax and output of tile 0, warps 4-7 of tile 1: one query row per thread (its
 //              TMEM lane). All scores of a step are held in registers: running maximum, w =
-//              2^(s c - m c) with c = scale log2(e), f32 sum of the unrounded weights, P (rounded to
+//              2^(c (s - m)) with c = scale log2(e), f32 sum of the unrounded weights, P (rounded to
 //              the element type) back to TMEM over the consumed scores. The reference m only moves
 //              when the maximum has grown by more than 2^8 over it: any m gives the same quotient,
 //              and sums and weights up to 2^8 too large lose nothing in f32, bf16 or f16 (whose
@@ -337,28 +337,17 @@ __device__ __forceinline__ bool finite16(uint32_t half) {
   return (half & e) != e;
 }
 
-// What a row's weights are relative to: a score (`raw`), and that times c, rounded (`log`). The
-// rounding is a factor of all of the row's weights that its sum has too, below 2^(2^-12) while |log| <
-// kFar. Beyond, it may pass the exponent's range (at 2^32 it is up to 2^128): there the difference
-// from `raw` comes before the scale (`far`: a row of the warp is such a one). Subtracted from every score
-// it took 3 % of the long prompts' time.
-struct Reference {
-  float raw, log;
-  bool far;
-};
-// A row's reference, moved to the step's maximum `top` where that passes it by more than kSlack (after
-// the scale c); the row's sum and output so far follow. The previous product is done: the thread that
-// issued it issued these scores after it.
+// A row's reference m, a score, moved to the step's maximum `top` where that passes it by more than kSlack
+// after the scale c; the row's sum and output so far follow. The previous product is done: the thread
+// that issued it issued these scores after it.
 __device__ __forceinline__ void move_reference(uint32_t to, int dim, float c, float top, bool first,
-                                               Reference &r, float &sum) {
-  const float now = top * c;
-  const bool grown = now > r.log + kSlack;
+                                               float &m, float &sum) {
+  const float rise = (top - m) * c;  // rounded products of the two might not differ
+  const bool grown = rise > kSlack;
   if (!first && !__any_sync(0xffffffffu, grown)) return;
-  float f = ex2_approx((r.raw - top) * c);
-  if (first || grown) r.raw = top, r.log = now;
-  r.far = __any_sync(0xffffffffu, fabsf(r.log) >= kFar && r.log != -INFINITY);
+  if (first || grown) m = top;
   if (first) return;
-  if (!grown) f = 1.f;
+  const float f = grown ? ex2_approx(-rise) : 1.f;
   sum *= f;
 #pragma unroll 1
   for (int d = 0; d < dim; d += 16) {
@@ -406,8 +395,8 @@ __device__ __forceinline__ void hand_over_weights(uint64_t *p_full) {
 // registers, before() before the output or the weights' columns (at tp) are touched.
 template <bool kBf16, int kBlocks, class Loaded, class Before>
 __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, float c, bool masked,
-                                             int vis, int blocks, bool first, Reference &m,
-                                             float &sum, uint32_t tp, uint64_t *p_full, Loaded &&loaded,
+                                             int vis, int blocks, bool first, float &m, float &sum,
+                                             uint32_t tp, uint64_t *p_full, Loaded &&loaded,
                                              Before &&before) {
   if (masked) {
     // what a row does not see becomes -inf in TMEM, in the blocks that some row of the warp sees in part
@@ -445,11 +434,13 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
   for (int i = 1; i < kBlocks; ++i) top = fmaxf(top, tops[i]);
   if (!before()) return false;
   move_reference(to, dim, c, top, first, m, sum);
-  float base = m.log == -INFINITY ? 0.f : m.log;
-  if (__builtin_expect(m.far, 0)) {
-    const bool far = fabsf(base) >= kFar;
-    const float from = far ? -m.raw : 0.f;
-    const uint64_t from2 = pair(from, from);
+  // The weights are 2^(s c - m c). The rounding of m c is a factor of all of a row's weights that its sum
+  // has too, below 2^(2^-12) where it is less than kFar; it grows with m c, past the exponent's range at
+  // 2^32. From kFar on the difference s - m comes before the scale (for every score it took 3 to 4 % of the
+  // long prompts' time).
+  float base = m == -INFINITY ? 0.f : m * c;
+  if (__builtin_expect(fabsf(base) >= kFar, 0)) {
+    const uint64_t from2 = pair(-m, -m);
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -458,7 +449,7 @@ __device__ __forceinline__ bool softmax_step(uint32_t tl, uint32_t to, int dim, 
         v[i][e] = __float_as_uint(x.x);
         v[i][e + 1] = __float_as_uint(x.y);
       }
-    if (far) base = 0.f;
+    base = 0.f;
   }
   base = weight_shift<kBf16>(kSlack) - base;
   const uint64_t c2 = pair(c, c), base2 = pair(base, base);
@@ -974,8 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int whole = r.first / kKeys;  // steps that every row of the tile sees in full
       const int mine = t * tokens + token;  // token within the item
       const int sees = p.causal ? min(seen.k_len, seen.visible + mine) : seen.k_len;
-      Reference m = {-INFINITY, -INFINITY, false};
-      float sum = 0.f;
+      float m = -INFINITY, sum = 0.f;
       for (int j = 0; j < r.steps; ++j) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], s_phase, abort_flag));
         if (!ok) break;
@@ -1020,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t out_row = static_cast<int64_t>(it.q_row) + mine;
       const uint32_t head = static_cast<uint32_t>(it.head) * p.group + sub;
       uint16_t *dst = p.out + out_row * p.out_token + head * p.out_head;
-      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = log_sum<kBf16>(m.log, sum, kSlack);
+      if (live && p.lse && it.part == 0) p.lse[out_row * p.q_heads + head] = log_sum<kBf16>(m * c, sum, kSlack);
       if (r.steps > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], o_phase, abort_flag));
         if (!ok) break;
@@ -1082,7 +1072,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Parts<kDim> to_join = Parts<kDim>::of(p.workspace, p.parts_max);
           const size_t tile = static_cast<size_t>(it.part - 1) * 2 + t;
           if (live) {
-            if (d == 0) reinterpret_cast<float2 *>(to_join.ml)[tile * 128 + row] = make_float2(m.raw, sum);
+            if (d == 0) reinterpret_cast<float2 *>(to_join.ml)[tile * 128 + row] = make_float2(m, sum);
             float4 *o = reinterpret_cast<float4 *>(to_join.o) + (tile * (kDim / 4) + d / 4) * 128 + row;
 #pragma unroll
             for (int e = 0; e < 16; ++e)

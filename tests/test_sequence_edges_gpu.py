@@ -81,6 +81,29 @@ def test_scores_far_beyond_one(n, order, dim, dtype):
             check(lse, want_lse, want_lse.abs() * 2.0 ** -21, name + ", log-sum")
 
 
+@pytest.mark.parametrize("n", [300, 1000, 5000])
+@pytest.mark.parametrize("scale", [1.0, 0.125])
+@dims
+@both
+def test_large_scores_that_creep_up(n, scale, dim, dtype):
+    """Scores near 2^29.8 that grow by one unit in the last place (64) every 128 keys: steps of 64 or 8
+    (in the exponent of e) between groups of keys, where the product with scale log2(e) moves by less than
+    its own rounding. The scores are exact in f32; of their differences' products 2^-22 is lost."""
+    q, k = torch.zeros(1, 4, dim, device=DEV, dtype=dtype), torch.zeros(n, 2, dim, device=DEV, dtype=dtype)
+    q[0, :, 3], k[:, :, 3] = 1.75 * 2.0 ** 14, 1.96875 * 2.0 ** 14
+    step = torch.arange(n, device=DEV) // 128
+    q[0, :, 9], k[:, :, 9] = 8.0, (8.0 * step)[:, None].to(dtype)
+    v = randn(gen(81), n, 2, dim, dtype=dtype)
+    s = step.double() * 64 * scale
+    w = torch.exp(s - s.max())
+    w /= w.sum()
+    want = torch.einsum("j,jhd->hd", w, v.double()).repeat_interleave(2, 0)
+    size = torch.einsum("j,jhd->hd", w, v.double().abs()).repeat_interleave(2, 0)
+    u = torch.finfo(dtype).eps / 2
+    for name, out, lse in every_form(q, k, v, scale):
+        check(out, want, u * want.abs() + (u + 2.0 ** -16) * size + (2.0 ** -25 if dtype == torch.float16 else 0.0), name)
+
+
 # ---- float16 weights far below the largest ---------------------------------------------------
 @pytest.mark.parametrize("n,gap", [(300, 15.5), (8192, 15.5), (8192, 17.0), (8192, 19.0)])
 @pytest.mark.parametrize("strong", ["first", "middle", "last"])
