@@ -64,8 +64,16 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(
   int s = static_cast<int>(t);
   if (p.cu_new) {
     s = warp_find_sequence(p.cu_new, p.n_seq, row0 + page_of(p.units, warp_first));
-    // a later row of the warp may belong to a later sequence
-    while (s + 1 < static_cast<int>(p.n_seq) && static_cast<int64_t>(p.cu_new[s + 1]) <= t) ++s;
+    // A later row of the warp may belong to a later sequence, mostly the next; empty ones may lie between,
+    // however many: steps that double while they land at or before the row, then halve.
+    auto before = [&](uint32_t step) {
+      const int64_t to = static_cast<int64_t>(s) + step;
+      return to < p.n_seq && static_cast<int64_t>(p.cu_new[to]) <= t;
+    };
+    uint32_t step = 1;
+    for (; before(step); step *= 2) s += step;
+    while (step /= 2)
+      if (before(step)) s += step;
   }
   if (base + threadIdx.x >= total_units || s < 0 || s >= static_cast<int>(p.n_seq)) return;
   uint32_t first, end;

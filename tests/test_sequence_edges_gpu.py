@@ -269,3 +269,29 @@ def test_one_workspace_for_calls_of_any_length():
         assert torch.equal(want, dv.attention_packed(q, k, v, cu, cu_of(lens), causal=True, workspace=packed))
     for call in (lambda: dv.attention_packed_workspace(96), lambda: dv.attention_paged_workspace(4, 6, 4, 64), lambda: dv.attention_paged_workspace(0, 4, 4, 64)):
         refused(call, "no call has")
+
+
+# ---- many sequences --------------------------------------------------------------------------
+def test_append_between_many_empty_sequences():
+    """Rows of one warp whose sequences lie a million empty ones apart. Each is found in some twenty steps; a
+    walk over the empty ones took 0.19 s, so 50 ms tell the two apart."""
+    n, rows = 3_000_000, 3
+    at = [5, 1_000_000, n - 7]  # the sequences with a row
+    ends = torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    for s in at:
+        ends[s + 1:] += 1
+    lens = torch.zeros(n, dtype=torch.int32, device=DEV)
+    lens[at] = ints([1, 2, 3])
+    table = torch.full((n, 1), -1, dtype=torch.int32, device=DEV)
+    table[at, 0] = ints([2, 0, 1])
+    k_cache, v_cache = (torch.zeros(3, 1, 16, 64, device=DEV, dtype=torch.float16) for _ in range(2))
+    k, v = randn(gen(87), rows, 1, 64, dtype=torch.float16), randn(gen(88), rows, 1, 64, dtype=torch.float16)
+    marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    for _ in range(2):
+        marks[0].record()
+        dv.rope_append(None, k, v, k_cache, v_cache, table, lens, cu_new=ends)
+        marks[1].record()
+    torch.cuda.synchronize()
+    for row, (page, slot) in enumerate(((2, 0), (0, 1), (1, 2))):
+        assert torch.equal(k_cache[page, 0, slot], k[row, 0]) and torch.equal(v_cache[page, 0, slot], v[row, 0])
+    assert k_cache.count_nonzero() <= rows * 64 and marks[0].elapsed_time(marks[1]) < 50
