@@ -304,12 +304,23 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
     x.head = blocks == 1 ? x.hb : x.hb / blocks;
     x.end = x.s == end_s && x.hb == end_hb ? end_t : x.tiles;
   };
-  auto next_unit = [&](Place &x) {
-    x.t = 0;
-    if (++x.hb == pl.head_blocks) {
-      x.hb = 0;
-      ++x.s;
+  // The next sequence to visit, s or a later one. Of cut units the first with tokens, as far as the stretch
+  // goes: a batch may be mostly empty (the unused slots of a captured step), and visiting 63 empty sequences beside
+  // one of 4000 tokens (32/8 heads of 128) one by one took 534 us and not 14. Their rows are the join's. Of whole
+  // units every one, an empty one's zeros among them.
+  auto visit = [&](uint32_t s) {
+    if (pl.units) return s;
+    for (; s < p.n_seq && s <= end_s; s += 32) {
+      const uint32_t some = __ballot_sync(0xffffffffu, s + lane < p.n_seq && p.lens[s + lane] > 0);
+      if (some) return s + __ffs(some) - 1;
     }
+    return p.n_seq;
+  };
+  auto next_of = [&](const Place &x) { return x.hb + 1 < pl.head_blocks ? x.s : visit(x.s + 1); };
+  auto go_to = [&](Place &x, uint32_t s) {  // s = next_of(x)
+    x.t = 0;
+    x.hb = s == x.s ? x.hb + 1 : 0;
+    x.s = s;
     enter(x);
   };
   Place ld = {static_cast<uint32_t>(found[warp][0]), static_cast<uint32_t>(found[warp][1]),
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
   enter(ld);
   Place at = ld;
   auto settle = [&] {  // to the next tile there is
-    while (ld.t >= ld.end && !past(ld)) next_unit(ld);
+    while (ld.t >= ld.end && !past(ld)) go_to(ld, next_of(ld));
   };
   settle();
 
@@ -416,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
     x += 2 * kTileBytes;
     return x == ring + kStages * 2 * kTileBytes ? ring : x;
   };
-  for (; !past(at); next_unit(at)) {
+  for (uint32_t next = 0; !past(at); go_to(at, next)) {
     const uint32_t h0 = at.head * group + (at.hb - at.head * blocks) * 16;
     const uint32_t heads = min(16u, (at.head + 1) * group - h0);
     const bool whole = at.t == 0 && at.end == at.tiles;
@@ -434,7 +445,10 @@ __global__ void __launch_bounds__(kThreads, Ring<kDim>::kPerSm)
     for (int n = 0; n < kHeads8; ++n)
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) q[n][k][0] = qn[n][k][0], q[n][k][1] = qn[n][k][1];
-    if (!pl.team) load_q(at.hb + 1 < pl.head_blocks ? at.s : at.s + 1, at.hb + 1 < pl.head_blocks ? at.hb + 1 : 0);
+    if (!pl.team) {
+      next = next_of(at);
+      load_q(next, next == at.s ? at.hb + 1 : 0);
+    }
     // O^T: channels 16 n + lane / 4 and 8 more, heads 2 (lane % 4) and the next
     float o[kHeads8][kSteps][4];
     float m[kHeads8][2], l[kHeads8][2];
