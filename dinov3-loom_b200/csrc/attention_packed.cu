@@ -34,8 +34,8 @@
 // Bound by the exp2 unit and the tensor cores together where sequences are long (each busy 56 % of the
 // time, one tile's softmax under the other's products), by the chain of a tile's steps and its
 // items' starts and ends where they are short. Measured: 16384 causal tokens, 32/8 heads of 128, bf16,
-// 2.07 ms (1060 TFLOP/s, at the power cap); 24 such sequences of 1..2048 tokens 82 us; 64 of 201
-// tokens, 6 heads of 64, f16, 23.4 us (14.2 in the steady state of a larger batch).
+// 2.13 ms (1030 TFLOP/s, at the power cap); 24 such sequences of 1..2048 tokens 83 us; 64 of 201
+// tokens, 6 heads of 64, f16, 23.0 us (14.9 as an eighth of a batch of 512).
 //
 // Every wait is bounded; on a timeout the kernel records kErrAttentionWait, raises the CTA's
 // abort flag, lets its own copies and MMAs in flight land, frees TMEM and returns; the join then leaves

@@ -26,10 +26,12 @@
 //   - Where no sequence passes 256 keys, stretches are whole units and there is nothing to join; with
 //     no more units than CTAs, the four warps of a CTA share one and join in shared memory. So do
 //     the warps of a cluster of 2 to 8 CTAs where units are few and not so long that the rest of the
-//     SMs is missed: that spares the second launch (one sequence of 1000 keys, 32/8 heads of 128: 7.7 us,
-//     10.7 with it; 2500 keys 10.6 and 11.2; 5000 keys would take 15.6 and not 12.7).
+//     SMs is missed: that spares the second launch (one sequence of 1000 keys, 32/8 heads of 128: 8.1 us,
+//     11.4 with it; 2500 keys 11.0 and 11.8; 5000 keys would take 15.9 and not 13.2).
 // Four warps on one 64-key tile, meeting at barriers, took 24.8 us for 256 images of 201 tokens and
-// 51.5 us for 64 sequences of 1..4096 (32/8 heads of 128); these take 18 and 39. One sequence of 131072 tokens takes 96 us (5.6 TB/s with its join).
+// 51.5 us for 64 sequences of 1..4096 (32/8 heads of 128); these take 18 and 39. One sequence of 131072 tokens takes 98 us (5.5 TB/s with its join). Groups of more than 16
+// query heads read the cache once for every 16: 16 sequences of 32768 keys of one head of 128 take 60 us with 16 query
+// heads, 106 with 32 and 293 with 128 (one read: 41).
 #include <atomic>
 #include <type_traits>
 

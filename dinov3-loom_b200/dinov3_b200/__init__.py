@@ -13,8 +13,8 @@ Python face of the C ABI in include/dinov3.h, mirroring the reference crate's AP
 floats). Errors raise DINOv3Error carrying the library's status code and message (the
 reference's error texts). All compute runs in the CUDA library; there is no CPU path.
 
-For sequences beside the model's own forward (images of other sizes packed into one batch, a
-decoder behind the tokens), on CUDA tensors: attention_packed, rope_append, attention_paged, and the
+For a caller's own layers beside the model (images of other sizes packed into one batch, a decoder
+behind the tokens; the model's forward does not call them), on CUDA tensors: attention_packed, rope_append, attention_paged, and the
 sizes of their workspaces (sequence.py).
 """
 from __future__ import annotations

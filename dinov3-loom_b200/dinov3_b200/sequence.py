@@ -11,9 +11,10 @@ The calls are asynchronous on torch's current stream of the tensors' device (whi
 current device), can be captured into a CUDA graph, and allocate only what they return (and the
 attentions their scratch, unless it is given) through torch's allocator. They compute no
 gradients: a tensor that wants one, or carries a forward-mode tangent, is refused. What does not fit raises DINOv3Error
-(INVALID_ARGUMENT) before anything is launched. `status` is an optional int32 CUDA tensor of two
-words, cleared and read by the caller, that collects what only the device sees (bad pages and
-positions).
+(INVALID_ARGUMENT) before anything is launched, outputs that share memory with another tensor among
+it. `status` is an optional int32 CUDA tensor of two words, cleared and read by the caller, that collects
+what only the device sees: bad pages and positions, and a launch that gave up a wait and left its
+outputs incomplete. Without it nothing tells of these.
 """
 from __future__ import annotations
 
@@ -43,7 +44,7 @@ def attention_packed(q, k, v, cu_q, cu_k=None, *, causal=False, scale=None, out=
 
     q [total_q, q_heads, dim]; k, v [total_k, kv_heads, dim]; cu_q, cu_k int32 [n_seq + 1] (cu_k None:
     cu_q). scale defaults to dim ** -0.5. `out` may be given; rows outside the sequences are left as
-    they were. `lse`, float32 [total_q, q_heads], is filled where given. `workspace`: a uint8 tensor of
+    they were (in a new one: whatever the memory held). `lse`, float32 [total_q, q_heads], is filled where given. `workspace`: a uint8 tensor of
     attention_packed_workspace(dim) bytes to use instead of a new one."""
     return _sequence.attention_packed(q, k, v, cu_q, cu_k, causal, scale, out, lse, workspace, status)
 
@@ -76,7 +77,7 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, lens, cos=None, sin=None,
     k, v [total, kv_heads, dim]; caches [pages, kv_heads, page_size, dim]; page_table int32 [n_seq,
     max_pages]; lens int32 [n_seq], the lengths with the new rows; cu_new int32 [n_seq + 1], or None
     for one row per sequence; cos, sin float32 [positions, rot_dim / 2], or None for no rotation.
-    `q_out` may be q itself."""
+    `q_out` may be q itself; rows outside the sequences are left as they were."""
     return _sequence.rope_append(q, k, v, k_cache, v_cache, page_table, lens, cos, sin, cu_new, q_out, status)
 
 

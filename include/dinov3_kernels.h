@@ -195,8 +195,10 @@ int dv3k_matmul_swiglu(const uint16_t *h, uint32_t rows, const uint16_t *gateup_
                        const float *gateup_b, uint16_t *act, uint32_t *status, void *stream);
 
 /* ---- Packed sequences and a paged key-value cache (no counterpart in the reference, whose
- * attention is dv3k_attention's: 201 tokens, 6 heads x 64, f16, no mask). For images of other
- * sizes packed into one batch, and for a decoder that reads the tokens.
+ * attention is dv3k_attention's: 201 tokens, 6 heads x 64, f16, no mask). For a caller's own layers
+ * beside the model, whose projections give the queries, keys and values: images of other sizes packed into
+ * one batch, a decoder that reads the tokens. The model's forward calls none of them, and its patchify
+ * and projections stay at 201 tokens.
  *
  * Beyond the common rules:
  *   - `dtype` is DV3K_F16 or DV3K_BF16 and holds for every 16-bit tensor of the call; head_dim is
@@ -219,7 +221,8 @@ int dv3k_matmul_swiglu(const uint16_t *h, uint32_t rows, const uint16_t *gateup_
  *     page may stand in several rows (a shared prefix) while nobody appends to it.
  *   - status word 0 collects bit 6 (a page id outside 0..n_pages-1, or a position behind the
  *     table's max_pages) and bit 7 (a position before 0 or behind the rotation tables). Such tokens
- *     are skipped: not appended, not attended to.
+ *     are skipped: not appended, not attended to. A wait that expired sets its bit as everywhere, and
+ *     the outputs are then incomplete; without a status nothing tells of any of these.
  *   - `lens`, `cu` and the page table are read on the device: a captured call replays on their
  *     new values.
  *   - Infinities and NaN in rows and slots that a query does not see do not reach its result. */
