@@ -272,6 +272,19 @@ def test_one_workspace_for_calls_of_any_length():
 
 
 # ---- many sequences --------------------------------------------------------------------------
+def shortest(call):
+    """Milliseconds of the quickest of four calls, the host's pauses left out by that."""
+    times = []
+    for _ in range(4):
+        marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        marks[0].record()
+        call()
+        marks[1].record()
+        torch.cuda.synchronize()
+        times.append(marks[0].elapsed_time(marks[1]))
+    return min(times)
+
+
 def test_append_between_many_empty_sequences():
     """Rows of one warp whose sequences lie a million empty ones apart. Each is found in some twenty steps; a
     walk over the empty ones took 0.19 s, so 50 ms tell the two apart."""
@@ -286,15 +299,10 @@ def test_append_between_many_empty_sequences():
     table[at, 0] = ints([2, 0, 1])
     k_cache, v_cache = (torch.zeros(3, 1, 16, 64, device=DEV, dtype=torch.float16) for _ in range(2))
     k, v = randn(gen(87), rows, 1, 64, dtype=torch.float16), randn(gen(88), rows, 1, 64, dtype=torch.float16)
-    marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
-    for _ in range(2):
-        marks[0].record()
-        dv.rope_append(None, k, v, k_cache, v_cache, table, lens, cu_new=ends)
-        marks[1].record()
-    torch.cuda.synchronize()
+    took = shortest(lambda: dv.rope_append(None, k, v, k_cache, v_cache, table, lens, cu_new=ends))
     for row, (page, slot) in enumerate(((2, 0), (0, 1), (1, 2))):
         assert torch.equal(k_cache[page, 0, slot], k[row, 0]) and torch.equal(v_cache[page, 0, slot], v[row, 0])
-    assert k_cache.count_nonzero() <= rows * 64 and marks[0].elapsed_time(marks[1]) < 50
+    assert k_cache.count_nonzero() <= rows * 64 and took < 50
 
 
 @pytest.mark.parametrize("hq,hkv,dim", [(32, 8, 128), (8, 2, 64), (33, 1, 64)])
@@ -311,17 +319,12 @@ def test_paged_slots_that_are_empty(active, length, hq, hkv, dim):
     k, v, table = paged_cache(89, lens, hkv, 16, dim, torch.bfloat16, wide=256)
     q = randn(gen(90), slots, hq, dim, dtype=torch.bfloat16)
     n = ints(lens)
-    marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
     none = n == 0
     for max_len in (None, max(length, 1)):
         out, lse = torch.full_like(q, 3.0), torch.full((slots, hq), 3.0, device=DEV)
-        for _ in range(2):
-            marks[0].record()
-            dv.attention_paged(q, k, v, table, n, max_len=max_len, out=out, lse=lse)
-            marks[1].record()
-        torch.cuda.synchronize()
+        took = shortest(lambda: dv.attention_paged(q, k, v, table, n, max_len=max_len, out=out, lse=lse))
         assert (out[none] == 0).all() and (lse[none] == -math.inf).all()
-        assert marks[0].elapsed_time(marks[1]) < 3
+        assert took < 3
         for i in at:
             o, tol, l, ltol = one_sequence(q[i:i + 1], cached_rows(k, table, i, length), cached_rows(v, table, i, length), dim ** -0.5, False)
             check(out[i:i + 1], o, tol, f"slot {i}")
